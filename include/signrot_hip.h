@@ -680,6 +680,96 @@ int srq_sym_dequant_moe(const int32_t *q, const void *scale_row, const void *w_s
                         int64_t num_experts, int64_t rows, int64_t cols, void *out,
                         void *stream);
 
+/* ------------------------------------------- q/k norms and the int8 KV cache
+ * For models whose attention normalizes each query and key head, and for a
+ * cache of 8 bits.  No counterpart in the reference (its attention has no
+ * q/k norm, its cache is int4). */
+
+/* RMSNorm of each head row of q f16 [B, T, n_q_heads, D] and k f16 [B, T,
+ * n_kv_heads, D] (y = x / sqrt(mean(x^2) + eps) * weight; norm = 0: y = x) with
+ * the rotary embedding (y * cos + rotate_half(y) * sin) in the same pass, fp32
+ * with one rounding at the end, into dense q_out and k_out.  q and k may be
+ * column slices of one projection output: dense in their last two dims, token
+ * and sequence strides in elements, multiples of 8.  cos / sin f16 [cos_batch,
+ * T, D], cos_batch 1 or B; weights f16 [D] or NULL.  D 64, 128 or 256;
+ * everything 16-byte aligned.  Outputs may not overlap inputs. */
+int srq_qk_norm_rope(const void *q, const void *k, const void *cos, const void *sin,
+                     int64_t cos_batch, const void *q_weight, const void *k_weight, float eps,
+                     int norm, int64_t batch, int64_t seq_len, int64_t n_q_heads,
+                     int64_t n_kv_heads, int64_t head_dim, int64_t q_tok_stride,
+                     int64_t q_seq_stride, int64_t k_tok_stride, int64_t k_seq_stride,
+                     void *q_out, void *k_out, void *stream);
+
+/* The paged int8 cache holds one scale for each block of 16 tokens and head:
+ *   data  i8  [pages, L, 2, H, page_size, 128]   (K at 0, V at 1)
+ *   scale f32 [pages, L, 2, H, page_size / 16]   value = code * scale
+ * page_size is a multiple of 16; the page table (indptr [B + 1], indices
+ * [n_indices], last_page_offset [B]) is that of the int4 cache.  Entries that
+ * point outside `indices` or the pool are taken as pages that are not there:
+ * nothing is read or written through them.
+ *
+ * srq_append_kv_i8 stores new tokens, k and v f16 [rows, H, 128] (dense rows,
+ * token strides in elements, multiples of 8), as each request's last ones: rows
+ * new_indptr[b] .. new_indptr[b + 1] of request b (int32 [B + 1] on the device),
+ * or row b when new_indptr is NULL (rows = B).  The lengths in the table count
+ * the new tokens.  Per block and head: scale = max(the block's scale if it holds
+ * older tokens, fp32(max|new| * fp32(1 / 127))), new codes rne(x / scale), and older
+ * codes c become rne(c * old scale / scale) where it grew, all as in exact
+ * arithmetic.  A non-finite new value makes the block's scale NaN.  Rows of a
+ * page behind the last token stay as they are.  A page that is written may belong
+ * to one request only.  max_new >= the largest number of new tokens sizes the
+ * launch (any value gives the same result). */
+int srq_append_kv_i8(void *kv_data, void *kv_scale, const int32_t *kv_indptr,
+                     const int32_t *kv_indices, const int32_t *last_page_offset, int64_t pages,
+                     int64_t n_indices, int64_t batch, int64_t num_layers, int64_t layer_idx,
+                     int64_t num_kv_heads, int64_t page_size, int64_t head_dim, const void *k,
+                     const void *v, int64_t k_tok_stride, int64_t v_tok_stride, int64_t rows,
+                     const int32_t *new_indptr, int64_t max_new, void *stream);
+
+/* srq_qk_norm_rope of the q and k columns of a projection output qkv f16 [rows,
+ * (n_q_heads + 2 H) 128] and srq_append_kv_i8 of the resulting k and of v, in
+ * one launch and with the same bits; q_out f16 [rows, n_q_heads, 128] (rows of
+ * no request stay as they are).  cos / sin f16 [cos_rows, 128], cos_rows 1 or
+ * rows. */
+int srq_qkv_norm_rope_append_i8(
+    void *kv_data, void *kv_scale, const int32_t *kv_indptr, const int32_t *kv_indices,
+    const int32_t *last_page_offset, int64_t pages, int64_t n_indices, int64_t batch,
+    int64_t num_layers, int64_t layer_idx, int64_t num_kv_heads, int64_t page_size,
+    int64_t head_dim, const void *qkv, int64_t tok_stride, int64_t rows, const void *cos,
+    const void *sin, int64_t cos_rows, int64_t n_q_heads, const void *q_weight,
+    const void *k_weight, float eps, int norm, const int32_t *new_indptr, int64_t max_new,
+    void *q_out, void *stream);
+
+/* Attention of each request's last tokens over the int8 cache: rows
+ * q_indptr[b] .. q_indptr[b + 1] of q f16 [rows, n_q_heads, 128] are its last n
+ * tokens (row b, its last one, when q_indptr is NULL and rows = B); token i of
+ * them sees the first len - n + i + 1 cached tokens.  Grouped-query
+ * (n_q_heads a multiple of H); logits q . k * sm_scale (finite).  o like q; a
+ * row that sees nothing is 0, a row of no request stays as it is.  max_q_len and
+ * max_kv_len size the launch and the workspace of ..._ws_bytes (any value is
+ * correct). */
+int srq_batch_attention_i8(
+    void *o, const void *q, int64_t rows, int64_t n_q_heads, const void *kv_data,
+    const void *kv_scale, const int32_t *kv_indptr, const int32_t *kv_indices,
+    const int32_t *last_page_offset, int64_t pages, int64_t n_indices, int64_t batch,
+    int64_t num_layers, int64_t layer_idx, int64_t num_kv_heads, int64_t page_size,
+    int64_t head_dim, const int32_t *q_indptr, int64_t max_q_len, int64_t max_kv_len,
+    float sm_scale, void *ws, int64_t ws_bytes, void *stream);
+int srq_batch_attention_i8_ws_bytes(int64_t rows, int64_t batch, int64_t n_q_heads,
+                                    int64_t n_kv_heads, int64_t max_q_len, int64_t max_kv_len,
+                                    int64_t *bytes);
+
+/* fp16 activations x [M, K] through 4-bit weights with group scales:
+ *   out[m, n] = sum_k x[m, k] scale[n, k / group] (c[n, k] - zero[n, k / group])
+ * (+ bias[n]), sums in fp32, one rounding.  w u8 [N, K / 2] packed codes: signed
+ * int4 with zeros NULL, unsigned with zeros u8 [N, K / group].  scale f16 [N,
+ * K / group], bias f16 [N] or NULL, out f16 [M, N].  group is a multiple of 32
+ * that divides K.  Made for few rows; any M is correct.  No counterpart in the
+ * reference, whose linears take one scale per output channel. */
+int srq_w4a16_linear(const void *x, const void *w, const void *scales, const void *zeros,
+                     const void *bias, int64_t M, int64_t N, int64_t K, int64_t group, void *out,
+                     void *stream);
+
 #ifdef __cplusplus
 }
 #endif

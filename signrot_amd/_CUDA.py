@@ -24,6 +24,11 @@ Added ops (no reference counterpart, fused forms of reference chains):
                                                               kv_cache.py:144-170, 295-415
   qkv_decode_i4         = qkv_rope_had_append + batch_decode_i4 kv_cache.py:144-170, 295-415
   prefill_qkv_cache     = rope_qk + K Hadamard + kv_quant_pack + init_kv_i4 kv_cache.py:295-395
+
+Added ops for models and formats that the reference does not serve:
+  qk_norm_rope, append_kv_i8, qkv_norm_rope_append_i8, batch_attention_i8: q/k
+  norms, and a paged int8 KV cache with a scale per block of 16 tokens and head
+  w4a16_linear: fp16 activations through 4-bit weights with group scales
 """
 import ctypes
 import functools
@@ -926,6 +931,235 @@ def swiglu(gate, up):
         raise RuntimeError("swiglu expects fp16 input")
     out = torch.empty_like(gate)
     _call("srq_swiglu", _ptr(gate), _ptr(up), gate.numel(), _ptr(out), _stream(gate))
+    return out
+
+
+# ------------------------------------------ q/k norms and the int8 KV cache
+
+I8_BLOCK = 16   # tokens of a head that share a scale in the int8 cache
+
+
+def _head_strides(name, t, tname, T):
+    """Token and sequence strides of [B, T, H, D], dense in its last two dims
+    (those of a size-1 dim are never used to address)."""
+    B, _, H, D = t.shape
+    if (D > 1 and t.stride(3) != 1) or (H > 1 and t.stride(2) != D):
+        raise RuntimeError(f"{name}: {tname} must be dense in its last two dims")
+    tok = t.stride(1) if T > 1 else H * D
+    return tok, (t.stride(0) if B > 1 else T * tok)
+
+
+def qk_norm_rope(q, k, cos, sin, q_weight=None, k_weight=None, eps=1e-6):
+    """RMSNorm of each head of q [B, T, Hq, D] and k [B, T, Hk, D] with the
+    rotary embedding in the same pass: y = x / sqrt(mean(x^2) + eps) * weight,
+    then y * cos + rotate_half(y) * sin, in fp32 with one rounding.  Returns
+    dense (q, k).  eps=None leaves the norm out.  q and k may be column slices
+    of one projection output (dense last two dims); cos / sin [1 or B, T, D];
+    D is 64, 128 or 256; everything fp16."""
+    f16 = torch.float16
+    _check("qk_norm_rope", [(q, "q"), (k, "k")], [f16, f16], contiguous=False)
+    _check("qk_norm_rope", [(cos, "cos"), (sin, "sin"), (q_weight, "q_weight"),
+                            (k_weight, "k_weight"), (q, "q")], [f16] * 5, contiguous=False)
+    _check("qk_norm_rope", [(cos, "cos"), (sin, "sin"), (q_weight, "q_weight"),
+                            (k_weight, "k_weight")])
+    if q.dim() != 4 or k.dim() != 4 or q.shape[:2] != k.shape[:2] or q.shape[3] != k.shape[3]:
+        raise RuntimeError("qk_norm_rope: q and k must be [B, T, H, D] with the same B, T and D")
+    B, T, Hq, D = q.shape
+    if cos.shape != sin.shape or tuple(cos.shape) not in ((1, T, D), (B, T, D)):
+        raise RuntimeError(f"qk_norm_rope: cos/sin must be [1 or {B}, {T}, {D}]")
+    _check_norm("qk_norm_rope", q_weight, k_weight, eps, D)
+    (q_tok, q_seq), (k_tok, k_seq) = (_head_strides("qk_norm_rope", t, n, T)
+                                      for t, n in ((q, "q"), (k, "k")))
+    qo = torch.empty((B, T, Hq, D), dtype=f16, device=q.device)
+    ko = torch.empty(k.shape, dtype=f16, device=q.device)
+    _call("srq_qk_norm_rope", _ptr(q), _ptr(k), _ptr(cos), _ptr(sin), cos.shape[0],
+          _ptr(q_weight), _ptr(k_weight), 0.0 if eps is None else float(eps),
+          0 if eps is None else 1, B, T, Hq, k.shape[2], D, q_tok, q_seq, k_tok, k_seq, _ptr(qo),
+          _ptr(ko), _stream(q))
+    return qo, ko
+
+
+def _check_norm(name, q_weight, k_weight, eps, D):
+    for w, wname in ((q_weight, "q_weight"), (k_weight, "k_weight")):
+        if w is None:
+            continue
+        if eps is None:
+            raise RuntimeError(f"{name}: {wname} without a norm (eps=None)")
+        if w.dim() != 1 or w.shape[0] != D:
+            raise RuntimeError(f"{name}: {wname} must be [{D}]")
+
+
+def _check_cache_i8(name, kv_data, kv_scale, kv_indptr, kv_indices, last_page_offset):
+    """The cache's tensors; returns the arguments that the entry points share
+    behind the five pointers, without the layer: pages, indices, batch, L and
+    H, page, D."""
+    _check(name, [(kv_data, "kv_data"), (kv_scale, "kv_scale"), (kv_indptr, "kv_indptr"),
+                  (kv_indices, "kv_indices"), (last_page_offset, "last_page_offset")],
+           [torch.int8, torch.float32, torch.int32, torch.int32, torch.int32])
+    if kv_data.dim() != 6 or kv_data.shape[2] != 2:
+        raise RuntimeError(f"{name}: kv_data must be [pages, L, 2, H, page, 128]")
+    pages, L, _, H, page, D = kv_data.shape
+    if D != 128:
+        raise RuntimeError(f"CHECK_EQ(head_dim, 128) failed. {D} vs 128")
+    if page == 0 or page % I8_BLOCK:
+        raise RuntimeError(f"{name}: the page size {page} must be a multiple of {I8_BLOCK}")
+    if tuple(kv_scale.shape) != (pages, L, 2, H, page // I8_BLOCK):
+        raise RuntimeError(f"{name}: kv_scale must be "
+                           f"{(pages, L, 2, H, page // I8_BLOCK)}, got {tuple(kv_scale.shape)}")
+    if kv_indptr.dim() != 1 or kv_indices.dim() != 1 or last_page_offset.dim() != 1:
+        raise RuntimeError(f"{name}: index tensors must be 1D")
+    B = last_page_offset.shape[0]
+    if kv_indptr.shape[0] != B + 1:
+        raise RuntimeError(f"{name}: kv_indptr must have batch + 1 entries")
+    return (pages, kv_indices.shape[0], B, L), (H, page, D)
+
+
+def _check_new(name, indptr, iname, rows, B, hint, kv_data):
+    """Row index of the new tokens (or None: one row per request) and its hint."""
+    _check(name, [(kv_data, "kv_data"), (indptr, iname)], [None, torch.int32])
+    if indptr is None:
+        if rows != B:
+            raise RuntimeError(f"{name}: {rows} rows for {B} requests, without {iname}")
+        return 1
+    if indptr.dim() != 1 or indptr.shape[0] != B + 1:
+        raise RuntimeError(f"{name}: {iname} must have batch + 1 entries")
+    return int(rows if hint is None else hint)
+
+
+def append_kv_i8(kv_data, kv_scale, kv_indptr, kv_indices, last_page_offset, layer_idx, k, v,
+                 new_indptr=None, max_new=None):
+    """Store new keys and values, k and v fp16 [rows, H, 128], as the last
+    tokens of each request in the paged int8 cache: kv_data i8 [pages, L, 2, H,
+    page, 128], kv_scale fp32 [pages, L, 2, H, page / 16], one scale for each
+    block of 16 tokens and head (page a multiple of 16).  Request b gets rows
+    new_indptr[b] .. new_indptr[b + 1] (int32), or row b without an index; the
+    page table counts them already.  A block that holds older tokens keeps the
+    larger of its scale and the new one, its codes requantized where it grew; a
+    non-finite value makes its block read as NaN.  k and v may be column slices
+    (dense rows [H, 128]).  max_new: the largest number of new tokens, which sizes
+    the launch."""
+    name = "append_kv_i8"
+    head, tail = _check_cache_i8(name, kv_data, kv_scale, kv_indptr, kv_indices, last_page_offset)
+    H, B = tail[0], head[2]
+    _check(name, [(k, "k"), (v, "v"), (kv_data, "kv_data")], [torch.float16, torch.float16, None],
+           contiguous=False)
+    if k.dim() != 3 or tuple(k.shape[1:]) != (H, 128) or v.shape != k.shape:
+        raise RuntimeError(f"{name}: k and v must be [rows, {H}, 128]")
+    rows = k.shape[0]
+    hint = _check_new(name, new_indptr, "new_indptr", rows, B, max_new, kv_data)
+    toks = []
+    for t, tname in ((k, "k"), (v, "v")):
+        if t.stride(2) != 1 or (H > 1 and t.stride(1) != 128):
+            raise RuntimeError(f"{name}: {tname} must be dense in its last two dims")
+        toks.append(t.stride(0) if rows > 1 else H * 128)
+    _call("srq_append_kv_i8", _ptr(kv_data), _ptr(kv_scale), _ptr(kv_indptr), _ptr(kv_indices),
+          _ptr(last_page_offset), *head, int(layer_idx), *tail, _ptr(k), _ptr(v), *toks, rows,
+          _ptr(new_indptr), hint, _stream(kv_data))
+
+
+def qkv_norm_rope_append_i8(kv_data, kv_scale, kv_indptr, kv_indices, last_page_offset, layer_idx,
+                            qkv, cos, sin, n_q_heads, q_weight=None, k_weight=None, eps=1e-6,
+                            new_indptr=None, max_new=None):
+    """qk_norm_rope of the q and k columns of a projection output qkv fp16
+    [rows, (n_q_heads + 2 H) 128], and append_kv_i8 of the resulting keys and of
+    the v columns, in one launch and with the same bits.  cos / sin [1 or rows,
+    128]; eps=None leaves the norms out.  Returns q [rows, n_q_heads, 128], ready
+    for batch_attention_i8 (rows of no request are not written)."""
+    name = "qkv_norm_rope_append_i8"
+    head, tail = _check_cache_i8(name, kv_data, kv_scale, kv_indptr, kv_indices, last_page_offset)
+    H, B = tail[0], head[2]
+    f16 = torch.float16
+    _check(name, [(cos, "cos"), (sin, "sin"), (q_weight, "q_weight"), (k_weight, "k_weight"),
+                  (kv_data, "kv_data")], [f16, f16, f16, f16, None])
+    _check(name, [(qkv, "qkv"), (kv_data, "kv_data")], [f16, None], contiguous=False)
+    n_q_heads = int(n_q_heads)
+    cols = (n_q_heads + 2 * H) * 128
+    if qkv.dim() != 2 or qkv.shape[1] != cols or qkv.stride(1) != 1:
+        raise RuntimeError(f"{name}: qkv must be [rows, {cols}] with dense rows")
+    rows = qkv.shape[0]
+    if cos.shape != sin.shape or tuple(cos.shape) not in ((1, 128), (rows, 128)):
+        raise RuntimeError(f"{name}: cos/sin must be [1 or {rows}, 128]")
+    _check_norm(name, q_weight, k_weight, eps, 128)
+    hint = _check_new(name, new_indptr, "new_indptr", rows, B, max_new, kv_data)
+    q = torch.empty((rows, n_q_heads, 128), dtype=f16, device=qkv.device)
+    _call("srq_qkv_norm_rope_append_i8", _ptr(kv_data), _ptr(kv_scale), _ptr(kv_indptr),
+          _ptr(kv_indices), _ptr(last_page_offset), *head, int(layer_idx), *tail, _ptr(qkv),
+          qkv.stride(0) if rows > 1 else cols, rows, _ptr(cos), _ptr(sin), cos.shape[0], n_q_heads,
+          _ptr(q_weight), _ptr(k_weight), 0.0 if eps is None else float(eps),
+          0 if eps is None else 1, _ptr(new_indptr), hint, _ptr(q), _stream(kv_data))
+    return q
+
+
+@functools.lru_cache(maxsize=512)
+def _attention_i8_bytes(rows, B, Hq, H, max_q_len, max_kv_len):
+    n = ctypes.c_int64()
+    _call("srq_batch_attention_i8_ws_bytes", rows, B, Hq, H, max_q_len, max_kv_len,
+          ctypes.byref(n))
+    return n.value
+
+
+def batch_attention_i8(o, q, kv_data, kv_scale, kv_indptr, kv_indices, last_page_offset, layer_idx,
+                       q_indptr=None, max_q_len=None, max_kv_len=None, softmax_scale=None):
+    """Causal attention of each request's last tokens over the paged int8
+    cache, into o (like q): q fp16 [rows, Hq, 128], rows q_indptr[b] ..
+    q_indptr[b + 1] being the last tokens of request b (row b its last one
+    without an index).  Hq is a multiple of the cache's heads.  A row that sees no
+    token is 0; rows of no request are left as they are.  max_q_len (largest number
+    of rows of a request) and max_kv_len (longest request; the whole table when
+    None) size the launch and the workspace, any value gives a correct result;
+    softmax_scale defaults to 1 / sqrt(128)."""
+    name = "batch_attention_i8"
+    head, tail = _check_cache_i8(name, kv_data, kv_scale, kv_indptr, kv_indices, last_page_offset)
+    H, page = tail[0], tail[1]
+    _check(name, [(o, "o"), (q, "q"), (kv_data, "kv_data")], [torch.float16, torch.float16, None])
+    if q.dim() != 3 or o.shape != q.shape or q.shape[2] != 128:
+        raise RuntimeError(f"{name}: o and q must be the same [rows, Hq, 128]")
+    rows, Hq = q.shape[:2]
+    if H == 0 or Hq == 0 or Hq % H:
+        raise RuntimeError(f"{name}: {Hq} query heads for {H} KV heads")
+    B = head[2]
+    hint = max(1, _check_new(name, q_indptr, "q_indptr", rows, B, max_q_len, kv_data))
+    kv = max(1, int(page * head[1] if max_kv_len is None else max_kv_len))
+    ws = None
+    n = _attention_i8_bytes(rows, B, Hq, H, hint, kv)
+    if n:
+        ws = torch.empty(n, dtype=torch.uint8, device=q.device)
+    scale = 128 ** -0.5 if softmax_scale is None else float(softmax_scale)
+    _call("srq_batch_attention_i8", _ptr(o), _ptr(q), rows, Hq, _ptr(kv_data), _ptr(kv_scale),
+          _ptr(kv_indptr), _ptr(kv_indices), _ptr(last_page_offset), *head, int(layer_idx), *tail,
+          _ptr(q_indptr), hint, kv, scale, _ptr(ws), n, _stream(q))
+    return o
+
+
+# ------------------------------------------------ 4-bit weights with groups
+
+def w4a16_linear(x, w, scales, zeros=None, bias=None):
+    """fp16 x [..., K] through 4-bit weights with a scale for each group of
+    input columns: out[n] = sum_k x[k] scales[n, k / group] (c[n, k] - zeros[n,
+    k / group]) (+ bias), fp32 sums, one rounding.  w u8 [N, K / 2]: signed int4
+    codes, or unsigned ones with zeros u8 [N, K / group]; scales fp16 [N, K /
+    group], group = K / scales.shape[1], a multiple of 32.  Made for few rows."""
+    f16 = torch.float16
+    _check("w4a16_linear", [(x, "x"), (w, "w"), (scales, "scales"), (zeros, "zeros"),
+                            (bias, "bias")], [f16, torch.uint8, f16, torch.uint8, f16])
+    if w.dim() != 2 or scales.dim() != 2 or x.dim() < 1:
+        raise RuntimeError("w4a16_linear: expected x [..., K], w [N, K/2] and scales [N, K/group]")
+    N, K = w.shape[0], w.shape[1] * 2
+    groups = scales.shape[1]
+    if x.shape[-1] != K or scales.shape[0] != N:
+        raise RuntimeError(f"w4a16_linear: x {tuple(x.shape)} and scales {tuple(scales.shape)} do "
+                           f"not fit weights of {N} x {K}")
+    if groups == 0 or K % groups or (K // groups) % 32:
+        raise RuntimeError(f"w4a16_linear: {groups} groups of {K} columns: a group must be a "
+                           "multiple of 32 columns")
+    if zeros is not None and zeros.shape != scales.shape:
+        raise RuntimeError("w4a16_linear: zeros must have the shape of scales")
+    if bias is not None and bias.numel() != N:
+        raise RuntimeError("w4a16_linear: bias must have N elements")
+    M = x.numel() // K
+    out = torch.empty((*x.shape[:-1], N), dtype=f16, device=x.device)
+    _call("srq_w4a16_linear", _ptr(x), _ptr(w), _ptr(scales), _ptr(zeros), _ptr(bias), M, N, K,
+          K // groups, _ptr(out), _stream(x))
     return out
 
 

@@ -87,6 +87,17 @@ SIGNATURES = {
     "srq_moe_combine": [_p, _p, _p, _i64, _i64, _i64, _p, _p],
     "srq_sym_quant_dynamic_moe": [_p, _p, _p, _i64, _i64, _i64, _f32, _p, _p, _p],
     "srq_sym_dequant_moe": [_p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _p, _p],
+    "srq_qk_norm_rope": [_p, _p, _p, _p, _i64, _p, _p, _f32, _i32, _i64, _i64, _i64, _i64, _i64,
+                         _i64, _i64, _i64, _i64, _p, _p, _p],
+    "srq_append_kv_i8": [_p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
+                         _p, _p, _i64, _i64, _i64, _p, _i64, _p],
+    "srq_qkv_norm_rope_append_i8": [_p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
+                                    _i64, _p, _i64, _i64, _p, _p, _i64, _i64, _p, _p, _f32, _i32,
+                                    _p, _i64, _p, _p],
+    "srq_batch_attention_i8": [_p, _p, _i64, _i64, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64,
+                               _i64, _i64, _i64, _i64, _p, _i64, _i64, _f32, _p, _i64, _p],
+    "srq_batch_attention_i8_ws_bytes": [_i64, _i64, _i64, _i64, _i64, _i64, _p],
+    "srq_w4a16_linear": [_p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _p, _p],
 }
 
 
