@@ -956,6 +956,9 @@ def qk_norm_rope(q, k, cos, sin, q_weight=None, k_weight=None, eps=1e-6):
     dense (q, k).  eps=None leaves the norm out.  q and k may be column slices
     of one projection output (dense last two dims); cos / sin [1 or B, T, D];
     D is 64, 128 or 256; everything fp16."""
+    out = _host.qk_norm_rope(q, k, cos, sin, q_weight, k_weight, eps)
+    if out is not None:
+        return out
     f16 = torch.float16
     _check("qk_norm_rope", [(q, "q"), (k, "k")], [f16, f16], contiguous=False)
     _check("qk_norm_rope", [(cos, "cos"), (sin, "sin"), (q_weight, "q_weight"),
@@ -1038,6 +1041,9 @@ def append_kv_i8(kv_data, kv_scale, kv_indptr, kv_indices, last_page_offset, lay
     non-finite value makes its block read as NaN.  k and v may be column slices
     (dense rows [H, 128]).  max_new: the largest number of new tokens, which sizes
     the launch."""
+    if _host.append_kv_i8(kv_data, kv_scale, kv_indptr, kv_indices, last_page_offset, layer_idx,
+                          k, v, new_indptr, max_new):
+        return
     name = "append_kv_i8"
     head, tail = _check_cache_i8(name, kv_data, kv_scale, kv_indptr, kv_indices, last_page_offset)
     H, B = tail[0], head[2]
@@ -1065,6 +1071,11 @@ def qkv_norm_rope_append_i8(kv_data, kv_scale, kv_indptr, kv_indices, last_page_
     the v columns, in one launch and with the same bits.  cos / sin [1 or rows,
     128]; eps=None leaves the norms out.  Returns q [rows, n_q_heads, 128], ready
     for batch_attention_i8 (rows of no request are not written)."""
+    q = _host.qkv_norm_rope_append_i8(kv_data, kv_scale, kv_indptr, kv_indices, last_page_offset,
+                                      layer_idx, qkv, cos, sin, n_q_heads, q_weight, k_weight, eps,
+                                      new_indptr, max_new)
+    if q is not None:
+        return q
     name = "qkv_norm_rope_append_i8"
     head, tail = _check_cache_i8(name, kv_data, kv_scale, kv_indptr, kv_indices, last_page_offset)
     H, B = tail[0], head[2]
@@ -1108,6 +1119,9 @@ def batch_attention_i8(o, q, kv_data, kv_scale, kv_indptr, kv_indices, last_page
     of rows of a request) and max_kv_len (longest request; the whole table when
     None) size the launch and the workspace, any value gives a correct result;
     softmax_scale defaults to 1 / sqrt(128)."""
+    if _host.batch_attention_i8(o, q, kv_data, kv_scale, kv_indptr, kv_indices, last_page_offset,
+                                layer_idx, q_indptr, max_q_len, max_kv_len, softmax_scale):
+        return o
     name = "batch_attention_i8"
     head, tail = _check_cache_i8(name, kv_data, kv_scale, kv_indptr, kv_indices, last_page_offset)
     H, page = tail[0], tail[1]
@@ -1139,6 +1153,9 @@ def w4a16_linear(x, w, scales, zeros=None, bias=None):
     k / group]) (+ bias), fp32 sums, one rounding.  w u8 [N, K / 2]: signed int4
     codes, or unsigned ones with zeros u8 [N, K / group]; scales fp16 [N, K /
     group], group = K / scales.shape[1], a multiple of 32.  Made for few rows."""
+    out = _host.w4a16_linear(x, w, scales, zeros, bias)
+    if out is not None:
+        return out
     f16 = torch.float16
     _check("w4a16_linear", [(x, "x"), (w, "w"), (scales, "scales"), (zeros, "zeros"),
                             (bias, "bias")], [f16, torch.uint8, f16, torch.uint8, f16])

@@ -39,15 +39,21 @@ struct NoGil {
 
 // a torch.Tensor or Parameter itself: a subclass may see every attribute and
 // call that the Python op makes of it
-const at::Tensor &plain(PyObject *o, at::ScalarType dt) {
+const at::Tensor &strided(PyObject *o, at::ScalarType dt) {
     if (!THPVariable_CheckExact(o)) throw Bad();
     const at::Tensor &t = THPVariable_Unpack(o);
     if (!t.defined() || !t.is_cuda() || t.layout() != at::kStrided || t.scalar_type() != dt ||
-        !t.has_storage() || !t.is_contiguous() || t.is_neg() || t.is_conj() ||
+        !t.has_storage() || t.is_neg() || t.is_conj() ||
         t.key_set().has(c10::DispatchKey::Python) ||
         t.key_set().has(c10::DispatchKey::FuncTorchBatched) ||
         t.key_set().has(c10::DispatchKey::Functionalize))
         throw Bad();
+    return t;
+}
+
+const at::Tensor &plain(PyObject *o, at::ScalarType dt) {
+    const at::Tensor &t = strided(o, dt);
+    if (!t.is_contiguous()) throw Bad();
     return t;
 }
 
@@ -419,6 +425,220 @@ PyObject *w4a4_linear_swiglu(PyObject *, PyObject *const *a, Py_ssize_t n_args) 
     });
 }
 
+// token stride of rows [H, 128] that are dense in themselves
+int64_t token_stride(const at::Tensor &t, int64_t H) {
+    if (t.stride(2) != 1 || (H > 1 && t.stride(1) != 128)) throw Bad();
+    return t.size(0) > 1 ? t.stride(0) : H * 128;
+}
+
+// token and sequence strides of [B, T, H, D], dense in its last two dims
+void head_strides(const at::Tensor &t, int64_t &tok, int64_t &seq) {
+    const int64_t B = t.size(0), T = t.size(1), H = t.size(2), D = t.size(3);
+    if (t.stride(3) != 1 || (H > 1 && t.stride(2) != D)) throw Bad();
+    tok = T > 1 ? t.stride(1) : H * D;
+    seq = B > 1 ? t.stride(0) : T * tok;
+}
+
+// eps, or no norm for None
+int as_norm(PyObject *o, float &eps) {
+    eps = o == Py_None ? 0.f : as_float(o);
+    return o == Py_None ? 0 : 1;
+}
+
+// qk_norm_rope(q, k, cos, sin, q_weight, k_weight, eps) -> (q, k)
+PyObject *qk_norm_rope(PyObject *, PyObject *const *a, Py_ssize_t n_args) {
+    return guarded(n_args, 7, [&]() -> PyObject * {
+        const at::Tensor &q = strided(a[0], kF16), &k = strided(a[1], kF16);
+        const at::Tensor &c = plain(a[2], kF16);
+        const at::Device dev = q.device();
+        if (q.dim() != 4 || k.dim() != 4 || c.dim() != 3 || k.device() != dev || c.device() != dev)
+            throw Bad();
+        const int64_t B = q.size(0), T = q.size(1), Hq = q.size(2), Hk = k.size(2), D = q.size(3);
+        if (q.numel() == 0 || k.numel() == 0 || k.size(0) != B || k.size(1) != T ||
+            k.size(3) != D || c.size(1) != T || c.size(2) != D || (c.size(0) != 1 && c.size(0) != B))
+            throw Bad();
+        const at::Tensor &s = plain(a[3], kF16);
+        if (s.sizes() != c.sizes() || s.device() != dev) throw Bad();
+        for (int i = 4; i < 6; ++i)
+            if (a[i] != Py_None && plain(a[i], kF16).dim() != 1) throw Bad();
+        void *qw = opt_ptr(a[4], kF16, D, dev), *kw = opt_ptr(a[5], kF16, D, dev);
+        float eps;
+        const int norm = as_norm(a[6], eps);
+        int64_t q_tok, q_seq, k_tok, k_seq;
+        head_strides(q, q_tok, q_seq);
+        head_strides(k, k_tok, k_seq);
+        at::Tensor qo, ko;
+        int rc;
+        {
+            NoGil nogil;
+            qo = alloc({B, T, Hq, D}, kF16, dev);
+            ko = alloc({B, T, Hk, D}, kF16, dev);
+            rc = srq_qk_norm_rope(q.data_ptr(), k.data_ptr(), c.data_ptr(), s.data_ptr(), c.size(0),
+                                  qw, kw, eps, norm, B, T, Hq, Hk, D, q_tok, q_seq, k_tok, k_seq,
+                                  qo.data_ptr(), ko.data_ptr(), stream_of(dev));
+        }
+        check(rc, "srq_qk_norm_rope");
+        return wrap({qo, ko});
+    });
+}
+
+// The int8 cache's tensors and the layer: a[0] .. a[5] of the ops below.
+struct CacheI8 {
+    const at::Tensor &data, &scale, &indptr, &indices, &last;
+    at::Device dev;
+    int64_t layer, pages, L, H, page, B;
+    explicit CacheI8(PyObject *const *a)
+        : data(plain(a[0], kI8)), scale(plain(a[1], kF32)), indptr(plain(a[2], kI32)),
+          indices(plain(a[3], kI32)), last(plain(a[4], kI32)), dev(data.device()),
+          layer(as_int(a[5])) {
+        if (data.dim() != 6 || scale.dim() != 5 || indptr.dim() != 1 || indices.dim() != 1 ||
+            last.dim() != 1 || scale.device() != dev || indptr.device() != dev ||
+            indices.device() != dev || last.device() != dev)
+            throw Bad();
+        pages = data.size(0);
+        L = data.size(1);
+        H = data.size(3);
+        page = data.size(4);
+        B = last.size(0);
+        if (data.size(2) != 2 || data.size(5) != 128 || page == 0 || page % 16 || H == 0 ||
+            scale.size(0) != pages || scale.size(1) != L || scale.size(2) != 2 ||
+            scale.size(3) != H || scale.size(4) != page / 16 || indptr.size(0) != B + 1 || B == 0)
+            throw Bad();
+    }
+    // the row index of the new tokens (null: one row per request) and its hint
+    const int32_t *index(PyObject *o, PyObject *hint_o, int64_t rows, int64_t &hint) const {
+        hint = 1;
+        if (o == Py_None) {
+            if (rows != B) throw Bad();
+            return nullptr;
+        }
+        hint = hint_o == Py_None ? rows : as_int(hint_o);
+        if (plain(o, kI32).dim() != 1) throw Bad();
+        return (const int32_t *)ptr(o, kI32, B + 1, dev);
+    }
+};
+
+#define CACHE_ARGS(c)                                                                          \
+    c.data.data_ptr(), c.scale.data_ptr(), (const int32_t *)c.indptr.data_ptr(),               \
+        (const int32_t *)c.indices.data_ptr(), (const int32_t *)c.last.data_ptr(), c.pages,    \
+        c.indices.size(0), c.B, c.L, c.layer, c.H, c.page, 128
+
+// append_kv_i8(cache .. layer, k, v, new_indptr, max_new) -> True
+PyObject *append_kv_i8(PyObject *, PyObject *const *a, Py_ssize_t n_args) {
+    return guarded(n_args, 10, [&]() -> PyObject * {
+        const CacheI8 c(a);
+        const at::Tensor &k = strided(a[6], kF16), &v = strided(a[7], kF16);
+        if (k.dim() != 3 || v.sizes() != k.sizes() || k.size(1) != c.H || k.size(2) != 128 ||
+            k.device() != c.dev || v.device() != c.dev)
+            throw Bad();
+        int64_t hint;
+        const int32_t *idx = c.index(a[8], a[9], k.size(0), hint);
+        const int64_t kt = token_stride(k, c.H), vt = token_stride(v, c.H);
+        int rc;
+        {
+            NoGil nogil;
+            rc = srq_append_kv_i8(CACHE_ARGS(c), k.data_ptr(), v.data_ptr(), kt, vt, k.size(0), idx,
+                                  hint, stream_of(c.dev));
+        }
+        check(rc, "srq_append_kv_i8");
+        Py_RETURN_TRUE;
+    });
+}
+
+// qkv_norm_rope_append_i8(cache .. layer, qkv, cos, sin, n_q_heads, q_weight,
+// k_weight, eps, new_indptr, max_new) -> q
+PyObject *qkv_norm_rope_append_i8(PyObject *, PyObject *const *a, Py_ssize_t n_args) {
+    return guarded(n_args, 15, [&]() -> PyObject * {
+        const CacheI8 c(a);
+        const at::Tensor &x = strided(a[6], kF16), &cs = plain(a[7], kF16), &sn = plain(a[8], kF16);
+        const int64_t hq = as_int(a[9]);
+        if (hq < 0 || x.dim() != 2 || x.size(1) != (hq + 2 * c.H) * 128 || x.stride(1) != 1 ||
+            cs.dim() != 2 || sn.sizes() != cs.sizes() || cs.size(1) != 128 ||
+            x.device() != c.dev || cs.device() != c.dev || sn.device() != c.dev)
+            throw Bad();
+        const int64_t rows = x.size(0);
+        if (cs.size(0) != 1 && cs.size(0) != rows) throw Bad();
+        for (int i = 10; i < 12; ++i)
+            if (a[i] != Py_None && plain(a[i], kF16).dim() != 1) throw Bad();
+        void *qw = opt_ptr(a[10], kF16, 128, c.dev), *kw = opt_ptr(a[11], kF16, 128, c.dev);
+        float eps;
+        const int norm = as_norm(a[12], eps);
+        int64_t hint;
+        const int32_t *idx = c.index(a[13], a[14], rows, hint);
+        at::Tensor q;
+        int rc;
+        {
+            NoGil nogil;
+            q = alloc({rows, hq, 128}, kF16, c.dev);
+            rc = srq_qkv_norm_rope_append_i8(CACHE_ARGS(c), x.data_ptr(),
+                                             rows > 1 ? x.stride(0) : x.size(1), rows,
+                                             cs.data_ptr(), sn.data_ptr(), cs.size(0), hq, qw, kw,
+                                             eps, norm, idx, hint, q.data_ptr(),
+                                             stream_of(c.dev));
+        }
+        check(rc, "srq_qkv_norm_rope_append_i8");
+        return wrap({q});
+    });
+}
+
+// batch_attention_i8(o, q, cache .. layer, q_indptr, max_q_len, max_kv_len,
+// softmax_scale) -> True
+PyObject *batch_attention_i8(PyObject *, PyObject *const *a, Py_ssize_t n_args) {
+    return guarded(n_args, 12, [&]() -> PyObject * {
+        const at::Tensor &o = plain(a[0], kF16), &q = plain(a[1], kF16);
+        const CacheI8 c(a + 2);
+        if (q.dim() != 3 || o.sizes() != q.sizes() || q.size(2) != 128 || q.device() != c.dev ||
+            o.device() != c.dev)
+            throw Bad();
+        const int64_t rows = q.size(0), hq = q.size(1);
+        int64_t hint;
+        const int32_t *idx = c.index(a[8], a[9], rows, hint);
+        if (hint < 1) hint = 1;
+        int64_t kv = a[10] == Py_None ? c.page * c.indices.size(0) : as_int(a[10]);
+        if (kv < 1) kv = 1;
+        const float scale = a[11] == Py_None ? 0.08838834764831845f : as_float(a[11]);
+        int64_t wb = 0;
+        check(srq_batch_attention_i8_ws_bytes(rows, c.B, hq, c.H, hint, kv, &wb),
+              "srq_batch_attention_i8_ws_bytes");
+        int rc;
+        {
+            NoGil nogil;
+            at::Tensor ws;
+            if (wb > 0) ws = alloc({wb}, kU8, c.dev);
+            rc = srq_batch_attention_i8(o.data_ptr(), q.data_ptr(), rows, hq, CACHE_ARGS(c), idx,
+                                        hint, kv, scale, wb > 0 ? ws.data_ptr() : nullptr, wb,
+                                        stream_of(c.dev));
+        }
+        check(rc, "srq_batch_attention_i8");
+        Py_RETURN_TRUE;
+    });
+}
+
+// w4a16_linear(x, w, scales, zeros, bias) -> out
+PyObject *w4a16_linear(PyObject *, PyObject *const *a, Py_ssize_t n_args) {
+    return guarded(n_args, 5, [&]() -> PyObject * {
+        const at::Tensor &x = plain(a[0], kF16), &w = plain(a[1], kU8), &s = plain(a[2], kF16);
+        const at::Device dev = x.device();
+        if (x.dim() < 1 || w.dim() != 2 || s.dim() != 2 || w.device() != dev || s.device() != dev)
+            throw Bad();
+        const int64_t N = w.size(0), K = 2 * w.size(1), groups = s.size(1);
+        if (K == 0 || x.size(-1) != K || s.size(0) != N || groups == 0 || K % groups) throw Bad();
+        if (a[3] != Py_None && plain(a[3], kU8).sizes() != s.sizes()) throw Bad();
+        void *z = opt_ptr(a[3], kU8, N * groups, dev), *bias = opt_ptr(a[4], kF16, N, dev);
+        const int64_t M = x.numel() / K;
+        at::Tensor out;
+        int rc;
+        {
+            NoGil nogil;
+            out = alloc(with_last(x, N), kF16, dev);
+            rc = srq_w4a16_linear(x.data_ptr(), w.data_ptr(), s.data_ptr(), z, bias, M, N, K,
+                                  K / groups, out.data_ptr(), stream_of(dev));
+        }
+        check(rc, "srq_w4a16_linear");
+        return wrap({out});
+    });
+}
+
 // stream(t): the current stream of the tensor's device, as an address
 PyObject *stream(PyObject *, PyObject *const *a, Py_ssize_t n_args) {
     return guarded(n_args, 1, [&]() -> PyObject * {
@@ -434,7 +654,10 @@ PyMethodDef kMethods[] = {OP(had_sign_quant),       OP(had_sign_asym_quant),
                           OP(sym_quant_dynamic),    OP(rmsnorm_quant),
                           OP(head_had_quant),       OP(w4a4_linear),
                           OP(w4a4_linear_residual), OP(w4a4_linear_asym),
-                          OP(w4a4_linear_swiglu),   OP(stream),
+                          OP(w4a4_linear_swiglu),   OP(qk_norm_rope),
+                          OP(append_kv_i8),         OP(qkv_norm_rope_append_i8),
+                          OP(batch_attention_i8),   OP(w4a16_linear),
+                          OP(stream),
                           {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "srq_host",
