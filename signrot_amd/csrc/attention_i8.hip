@@ -31,6 +31,8 @@
 
 #include <math.h>
 
+#include <type_traits>
+
 namespace {
 
 constexpr int kTileTok = 32;
@@ -56,8 +58,19 @@ SRQ_DEV v4f mfma16(v8h a, v8h b, v4f c) {
 // 128) -> the signed codes
 SRQ_DEV v2h unbias(u32 w) { return __builtin_bit_cast(v2h, w) - (v2h){1152, 1152}; }
 
-// 8 int8 codes -> fp16, in order
+// 8 int8 codes -> fp16 subnormals (code + 128) 2^-24, in order: a byte below a
+// zero byte, exact.  The 128 and the 2^-24 are taken out of the fp32 scores.
 SRQ_DEV v8h codes8(u32 a, u32 b) {
+    const u32 x = a ^ 0x80808080u, y = b ^ 0x80808080u;
+    const v2h p0 = __builtin_bit_cast(v2h, __builtin_amdgcn_perm(0u, x, 0x0c010c00u));
+    const v2h p1 = __builtin_bit_cast(v2h, __builtin_amdgcn_perm(0u, x, 0x0c030c02u));
+    const v2h p2 = __builtin_bit_cast(v2h, __builtin_amdgcn_perm(0u, y, 0x0c010c00u));
+    const v2h p3 = __builtin_bit_cast(v2h, __builtin_amdgcn_perm(0u, y, 0x0c030c02u));
+    return (v8h){p0[0], p0[1], p1[0], p1[1], p2[0], p2[1], p3[0], p3[1]};
+}
+
+// 8 int8 codes -> fp16, in order
+SRQ_DEV v8h signed8(u32 a, u32 b) {
     const u32 x = a ^ 0x80808080u, y = b ^ 0x80808080u, k = 0x64646464u;
     const v2h p0 = unbias(__builtin_amdgcn_perm(k, x, 0x04010400u));
     const v2h p1 = unbias(__builtin_amdgcn_perm(k, x, 0x04030402u));
@@ -87,12 +100,15 @@ SRQ_DEV float read_lane(float v, int lane) {
     return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
 }
 
-// RT row tiles of 16 rows per block
+// RT row tiles of 16 rows per block.  With one, a wave has two tiles in flight (the
+// registers of two waves per SIMD).
 template <int RT>
-__global__ __launch_bounds__(kWaves * 64) void attn_i8_kernel(AttnI8Args a, PagedI8 p) {
+__global__ __launch_bounds__(kWaves * 64, 2) void attn_i8_kernel(AttnI8Args a, PagedI8 p) {
+    constexpr int DEPTH = RT == 1 ? 2 : 1;
     __shared__ float so[kWaves][16][kI8D + 4];
     __shared__ float sm[kWaves][16], sl[kWaves][16];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int col = lane & 15, g = lane >> 4;
     const int hk = blockIdx.y;
     const int64_t b = blockIdx.z;
@@ -105,6 +121,7 @@ __global__ __launch_bounds__(kWaves * 64) void attn_i8_kernel(AttnI8Args a, Page
          r0 += (int64_t)a.tiles * 16 * RT) {
         // this lane's rows: query token, head, first token that it does not see
         v8h qf[RT][4];
+        float qsum[RT];
         int lim[RT];
         int64_t orow[RT];
         int lo = 0x7fffffff, hi = 0;   // least and largest limit of the block's rows
@@ -118,10 +135,17 @@ __global__ __launch_bounds__(kWaves * 64) void attn_i8_kernel(AttnI8Args a, Page
             const int64_t pos = rq.len - n + i + 1;
             lim[t] = ok && pos > 0 ? (int)pos : 0;
             const f16 *src = a.q + (ok ? orow[t] : 0) * kI8D + 16 * g;
+            float sum = 0.f;
 #pragma unroll
-            for (int s = 0; s < 4; ++s)
+            for (int s = 0; s < 4; ++s) {
                 qf[t][s] = *reinterpret_cast<const v8h *>(src + 64 * (s >> 1) + 8 * (s & 1)) *
                            (f16)a.qmul;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) sum += (float)qf[t][s][e];
+            }
+            sum += __shfl_xor(sum, 16, 64);
+            sum += __shfl_xor(sum, 32, 64);
+            qsum[t] = sum * -0x1p-17f;   // -128 sum(q) 2^-24
         }
         {
             const int64_t last = r0 + 16 * RT < nrows ? r0 + 16 * RT : nrows;
@@ -145,50 +169,55 @@ __global__ __launch_bounds__(kWaves * 64) void attn_i8_kernel(AttnI8Args a, Page
             for (int i = 0; i < 8; ++i) o[t][i] = (v4f)0.f;
         }
 
+        const int64_t v_part = (int64_t)p.H * p.page * kI8D;
+        const uint32_t k_lane = col * kI8D + 16 * g, v_lane = 4 * g * kI8D + 8 * col;
         // The wave's tiles are t_lo + wave, + kWaves, ...; lane j looks up the
         // page and the scales of block j of the next 64 (32 tiles).
         for (int base = t_lo + wave; base < t_hi; base += 32 * kWaves) {
             const int mine = base + (lane >> 1) * kWaves;
             const int blk = 2 * mine + (lane & 1);
             int pg = -1;
-            float ks = 0.f, vs = 0.f;
-            uint32_t in_page = 0;
+            float ks = 0.f, vs = 0.f, lv, rv;
+            int64_t at = 0;   // its K codes; any block where there is none
             if (mine < t_hi && blk * kI8Block < hi) {
                 pg = (int)i8_page(p, rq.first, blk);
-                in_page = (uint32_t)blk % (uint32_t)p.bpp;
                 if (pg >= 0) {
-                    const int64_t si = i8_scale_index(p, pg, hk, in_page);
+                    const int64_t si =
+                        i8_scale_index(p, pg, hk, (uint32_t)blk % (uint32_t)p.bpp);
+                    at = si * (kI8Block * kI8D);
                     ks = p.scale[si];
                     vs = p.scale[si + (int64_t)p.H * p.bpp];
                 }
             }
-            const float lv = vs != 0.f ? __builtin_amdgcn_logf(vs) : 0.f;
-            const float rv = vs != 0.f ? 1.f / vs : 1.f;
-            ks *= a.c;
-
-            auto load = [&](Tile &x, int j) __attribute__((always_inline)) {
+            const int at_lo = (int)at, at_hi = (int)(at >> 32);
+            auto block_of = [&](int j, int bk) __attribute__((always_inline)) {
+                const uint32_t lo32 = (uint32_t)read_lane(at_lo, 2 * j + bk);
+                const int hi32 = read_lane(at_hi, 2 * j + bk);
+                return p.data + ((int64_t)hi32 << 32 | lo32);
+            };
+            auto load_k = [&](Tile &x, int j) __attribute__((always_inline)) {
 #pragma unroll
                 for (int bk = 0; bk < 2; ++bk) {
-                    const int pgj = read_lane(pg, 2 * j + bk);
-                    const uint32_t in = (uint32_t)read_lane((int)in_page, 2 * j + bk);
-                    const int8_t *kb =
-                        p.data + i8_scale_index(p, pgj < 0 ? 0 : pgj, hk, in) * (kI8Block * kI8D);
-                    const int8_t *vb = kb + (int64_t)p.H * p.page * kI8D;
-                    const int8_t *kr = kb + col * kI8D + 16 * g;
-                    x.k[bk][0] = *reinterpret_cast<const v4i *>(kr);
-                    x.k[bk][1] = *reinterpret_cast<const v4i *>(kr + 64);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        x.v[4 * bk + e] =
-                            *reinterpret_cast<const uint2 *>(vb + (4 * g + e) * kI8D + 8 * col);
+                    const int8_t *kb = block_of(j, bk) + k_lane;
+                    x.k[bk][0] = *reinterpret_cast<const v4i *>(kb);
+                    x.k[bk][1] = *reinterpret_cast<const v4i *>(kb + 64);
                 }
             };
-            auto step = [&](const Tile &x, int j) __attribute__((always_inline)) {
+            auto load_v = [&](Tile &x, int j) __attribute__((always_inline)) {
+#pragma unroll
+                for (int bk = 0; bk < 2; ++bk) {
+                    const int8_t *vb = block_of(j, bk) + v_part + v_lane;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        x.v[4 * bk + e] = *reinterpret_cast<const uint2 *>(vb + e * kI8D);
+                }
+            };
+            auto step = [&](Tile &x, int j, auto more) __attribute__((always_inline)) {
                 const int tok = (base + j * kWaves) * kTileTok;
                 v8h pb[RT];
                 v4f s[RT][2];
 #pragma unroll
-                for (int t = 0; t < RT; ++t) s[t][0] = s[t][1] = (v4f)0.f;
+                for (int t = 0; t < RT; ++t) s[t][0] = s[t][1] = (v4f)qsum[t];
 #pragma unroll
                 for (int bk = 0; bk < 2; ++bk)
 #pragma unroll
@@ -198,6 +227,8 @@ __global__ __launch_bounds__(kWaves * 64) void attn_i8_kernel(AttnI8Args a, Page
 #pragma unroll
                         for (int t = 0; t < RT; ++t) s[t][bk] = mfma16(kf, qf[t][q], s[t][bk]);
                     }
+                __builtin_amdgcn_sched_barrier(0);
+                if constexpr (more.value) load_k(x, j + DEPTH);
                 const bool full = tok + kTileTok <= lo && read_lane(pg, 2 * j) >= 0 &&
                                   read_lane(pg, 2 * j + 1) >= 0;
 #pragma unroll
@@ -256,13 +287,47 @@ __global__ __launch_bounds__(kWaves * 64) void attn_i8_kernel(AttnI8Args a, Page
                         for (int t = 0; t < RT; ++t)
                             o[t][4 * half + i] = mfma16(vf, pb[t], o[t][4 * half + i]);
                     }
+                    // half the converted codes at a time in registers
+                    __builtin_amdgcn_sched_barrier(0);
                 }
+                if constexpr (more.value) load_v(x, j + DEPTH);
             };
             const int cnt = min(32, (t_hi - base + kWaves - 1) / kWaves);
-            for (int j = 0; j < cnt; ++j) {
-                Tile x;
-                load(x, j);
-                step(x, j);
+            // the next tile's K is loaded as soon as this one's scores have
+            // taken its registers, its V after the second product; the first
+            // tile's loads come before its scales are used
+            Tile x;
+            load_k(x, 0);
+            __builtin_amdgcn_sched_barrier(0);   // K first: its wait leaves V in flight
+            load_v(x, 0);
+            __builtin_amdgcn_sched_barrier(0);
+            lv = vs != 0.f ? __builtin_amdgcn_logf(vs) : 0.f;
+            rv = vs != 0.f ? 1.f / vs : 1.f;
+            ks *= a.c * 0x1p24f;
+            // (the last tiles apart: with their loads under a condition every wait
+            // would be for all that are in flight)
+            if constexpr (DEPTH == 1) {
+                for (int j = 0; j + 1 < cnt; ++j) step(x, j, std::true_type());
+                step(x, cnt - 1, std::false_type());
+            } else {
+                Tile y;
+                load_k(y, cnt > 1 ? 1 : 0);
+                __builtin_amdgcn_sched_barrier(0);
+                load_v(y, cnt > 1 ? 1 : 0);
+                __builtin_amdgcn_sched_barrier(0);
+                int j = 0;
+                for (; j + 3 < cnt; j += 2) {
+                    step(x, j, std::true_type());
+                    step(y, j + 1, std::true_type());
+                }
+                if (j + 2 < cnt) {
+                    step(x, j, std::true_type());
+                    step(y, j + 1, std::false_type());
+                    step(x, j + 2, std::false_type());
+                } else {
+                    step(x, j, std::false_type());
+                    if (j + 1 < cnt) step(y, j + 1, std::false_type());
+                }
             }
         }
 
@@ -287,7 +352,7 @@ __global__ __launch_bounds__(kWaves * 64) void attn_i8_kernel(AttnI8Args a, Page
             // thread -> row threadIdx.x / 16, dims 8 (threadIdx.x % 16) .. + 7
             const int rr = threadIdx.x >> 4, d0 = 8 * (threadIdx.x & 15);
             const int64_t r = r0 + 16 * t + rr;
-            if (r < nrows) {
+            if (rr < 16 && r < nrows) {
                 const int64_t i = (uint32_t)r / (uint32_t)a.group;
                 const int64_t row = (s0 + i) * a.hq + hk * a.group + (r - i * a.group);
                 float mx = sm[0][rr];
@@ -326,10 +391,281 @@ __global__ __launch_bounds__(kWaves * 64) void attn_i8_kernel(AttnI8Args a, Page
     }
 }
 
-// Join of the chunks: a wave per (row, head), two dims per lane.
+// ----------------------------------------------------------- many query rows
+// The same attention for pieces of a prompt, where the products bound it and
+// not the cache's bytes: four waves of 32 rows each (v_mfma_f32_32x32x16_f16)
+// share tiles of 64 keys in LDS, double-buffered, with codes converted to
+// fp16 once per block on the way in.  A lane owns one row (column l % 32 of the
+// transposed scores); register v of a 32-key block is key 8 (v / 4) + 4 (l / 32) +
+// v % 4, so registers 0-7 and 8-15 each belong to one block of 16 keys, whose
+// scales reach the scores as above, and P^T is the second product's operand
+// straight from registers.  V's operand comes from the transposing LDS read.
+constexpr int KT = 64;
+constexpr int kRowsBlock = 32 * kWaves;
+constexpr int KS = kI8D + 8;     // row strides in halves: 16-byte reads of K and the
+constexpr int VR = kI8D + 16;    // transposing reads of V fall on distinct banks
+typedef short v4s __attribute__((vector_size(8)));
+
+SRQ_DEV v16f mfma32(v8h a, v8h b, v16f c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+
+// what a tile's scores need of a block of 16 keys
+struct BlockScale {
+    float kc, lv, rv, pad;
+};
+
+// A wave per SIMD from each of the two blocks that fit a CU.
+__global__ __launch_bounds__(kWaves * 64, 2) void attn_i8_rows_kernel(AttnI8Args a, PagedI8 p) {
+    constexpr int NT = kWaves * 64, RB = kRowsBlock;
+    constexpr int KR = NT / KT, KB = kI8D / KR;     // threads per key row, bytes of each
+    __shared__ __align__(16) f16 Ks_[2][KT * KS];
+    __shared__ __align__(16) f16 Vs_[2][KT * VR];
+    __shared__ BlockScale Bs_[2][KT / kI8Block];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int g = lane >> 5, ln = lane & 31;
+    const int hk = blockIdx.y;
+    const int64_t b = blockIdx.z;
+    const int chunk = blockIdx.x % a.chunks;
+    int64_t s0, n;
+    i8_new_rows(a.q_indptr, b, a.rows, s0, n);
+    const I8Request rq = i8_request(p, b);
+    const int64_t nrows = n * a.group;
+    const int64_t rtiles = (nrows + RB - 1) / RB;
+    // the last rows see most keys: their tiles come first
+    for (int64_t rt = rtiles - 1 - (int64_t)(blockIdx.x / a.chunks); rt >= 0; rt -= a.tiles) {
+        const int64_t r0 = rt * RB, r = r0 + 32 * wave + ln;
+        const bool ok = r < nrows;
+        const int64_t qi = ok ? (uint32_t)r / (uint32_t)a.group : 0;
+        const int64_t orow = (s0 + qi) * a.hq + hk * a.group + (ok ? (int)(r - qi * a.group) : 0);
+        const int64_t past = rq.len - n;
+        int lim = ok && past + qi + 1 > 0 ? (int)(past + qi + 1) : 0;
+        // limits of the wave's first row and of the block's last one
+        const int64_t wrow = r0 + 32 * wave < nrows ? r0 + 32 * wave : nrows - 1;
+        const int64_t brow = r0 + RB < nrows ? r0 + RB - 1 : nrows - 1;
+        const int64_t wlast = wrow + 31 < nrows ? wrow + 31 : nrows - 1;
+        const int64_t lo64 = past + (uint32_t)wrow / (uint32_t)a.group + 1;
+        const int64_t wh64 = past + (uint32_t)wlast / (uint32_t)a.group + 1;
+        const int64_t hi64 = past + (uint32_t)brow / (uint32_t)a.group + 1;
+        const int lo = lo64 > 0 ? (int)lo64 : 0, hi = hi64 > 0 ? (int)hi64 : 0;
+        const int wave_hi = r0 + 32 * wave < nrows && wh64 > 0 ? (int)wh64 : 0;
+        const int ntile = (hi + KT - 1) / KT;
+        const int per = (ntile + a.chunks - 1) / a.chunks;
+        const int t_lo = min(chunk * per, ntile), t_hi = min(ntile, t_lo + per);
+
+        v8h qf[kI8D / 16];
+        {
+            const f16 *src = a.q + (ok ? orow : 0) * kI8D + 8 * g;
+#pragma unroll
+            for (int kk = 0; kk < kI8D / 16; ++kk) {
+                const v8h x = *reinterpret_cast<const v8h *>(src + 16 * kk);
+                qf[kk] = ok ? x * (f16)a.qmul : (v8h)(f16)0;
+            }
+        }
+        v16f o[kI8D / 32];
+#pragma unroll
+        for (int i = 0; i < kI8D / 32; ++i) o[i] = (v16f)0.f;
+        float m = -INFINITY, l = 0.f;
+
+        // staging: thread -> key row tid / KR, KB bytes of its K and V codes
+        const int kr = tid / KR, kd = (tid % KR) * KB;
+        v4i kx[KB / 16], vx[KB / 16];
+        float ksc = 0.f, vsc = 0.f;
+        bool there = false;
+        int64_t page_next;
+        auto find = [&](int t) __attribute__((always_inline)) {
+            // the block's scale index, or -1; for the row that this thread loads
+            const int key = t * KT + kr;
+            int64_t si = -1;
+            if (t < t_hi && key < hi) {
+                const uint32_t blk = (uint32_t)key / kI8Block;
+                const int64_t pg = i8_page(p, rq.first, blk);
+                if (pg >= 0) si = i8_scale_index(p, pg, hk, blk % (uint32_t)p.bpp);
+            }
+            return si;
+        };
+        auto load_tile = [&](int64_t si, int t) __attribute__((always_inline)) {
+            there = si >= 0;
+            const int64_t at = there ? si : 0;
+            const int8_t *kb = p.data + (at * kI8Block + (kr & (kI8Block - 1))) * kI8D + kd;
+            const int8_t *vb = kb + (int64_t)p.H * p.page * kI8D;
+#pragma unroll
+            for (int i = 0; i < KB / 16; ++i) {
+                kx[i] = *reinterpret_cast<const v4i *>(kb + 16 * i);
+                vx[i] = *reinterpret_cast<const v4i *>(vb + 16 * i);
+            }
+            ksc = p.scale[at];
+            vsc = p.scale[at + (int64_t)p.H * p.bpp];
+        };
+        auto store_tile = [&](int buf) __attribute__((always_inline)) {
+            f16 *kd_ = &Ks_[buf][kr * KS + kd], *vd_ = &Vs_[buf][kr * VR + kd];
+#pragma unroll
+            for (int i = 0; i < KB / 16; ++i) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    *reinterpret_cast<v8h *>(kd_ + 16 * i + 8 * h) =
+                        signed8((u32)kx[i][2 * h], (u32)kx[i][2 * h + 1]);
+                    *reinterpret_cast<v8h *>(vd_ + 16 * i + 8 * h) =
+                        signed8((u32)vx[i][2 * h], (u32)vx[i][2 * h + 1]);
+                }
+            }
+            if (tid % (KR * kI8Block) == 0) {
+                const float v = vsc != 0.f ? vsc : 1.f;   // a block of zeros
+                BlockScale s;
+                s.kc = there ? ksc * a.c : 0.f;
+                s.lv = there ? __builtin_amdgcn_logf(v) : -INFINITY;
+                s.rv = there ? 1.f / v : 0.f;
+                s.pad = 0.f;
+                Bs_[buf][tid / (KR * kI8Block)] = s;
+            }
+        };
+
+        if (t_lo < t_hi) {
+            load_tile(find(t_lo), t_lo);
+            page_next = find(t_lo + 1);
+            store_tile(t_lo & 1);
+        }
+        __syncthreads();
+        for (int t = t_lo; t < t_hi; ++t) {
+            const int k0 = t * KT, buf = t & 1;
+            const f16 *Ks = Ks_[buf];
+            const f16 *Vs = Vs_[buf];
+            if (t + 1 < t_hi) {
+                load_tile(page_next, t + 1);    // in flight during this tile's products
+                page_next = find(t + 2);
+            }
+            [&]() __attribute__((always_inline)) {
+                if (k0 >= wave_hi) return;      // no key of this tile is visible
+                v16f s[2];
+#pragma unroll
+                for (int sb = 0; sb < 2; ++sb) {
+                    s[sb] = (v16f)0.f;
+                    const f16 *row = &Ks[(32 * sb + ln) * KS + 8 * g];
+#pragma unroll
+                    for (int kk = 0; kk < kI8D / 16; ++kk)
+                        s[sb] = mfma32(*reinterpret_cast<const v8h *>(row + 16 * kk), qf[kk], s[sb]);
+                }
+                // the K operand reads run 4 ahead of the products that take them
+                __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+                for (int i = 0; i < 12; ++i) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                }
+                __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
+                BlockScale bs[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) bs[i] = Bs_[buf][i];
+                if (k0 + KT > lo) {
+                    // A block that this row does not see, or that is not there,
+                    // may hold any scale: its exponents become 0 * 0 - inf.
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const bool seen = k0 + 16 * i < lim && bs[i].lv != -INFINITY;
+                        const float out = seen ? -INFINITY : 0.f;
+                        bs[i].kc = seen ? bs[i].kc : 0.f;
+                        bs[i].lv = seen ? bs[i].lv : -INFINITY;
+#pragma unroll
+                        for (int v = 0; v < 8; ++v) {
+                            const int key = k0 + 16 * i + 8 * (v / 4) + 4 * g + (v % 4);
+                            const int at = 8 * (i % 2) + v;
+                            s[i / 2][at] = seen && key < lim ? s[i / 2][at] : out;
+                        }
+                    }
+                }
+                // the largest exponent: scales are positive, so a block's largest
+                // score is its largest exponent
+                float mt = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float mb = -INFINITY;
+#pragma unroll
+                    for (int v = 0; v < 8; ++v) mb = fmaxf(mb, s[i / 2][8 * (i % 2) + v]);
+                    mt = fmaxf(mt, __builtin_fmaf(mb, bs[i].kc, bs[i].lv));
+                }
+                mt = fmaxf(mt, __shfl_xor(mt, 32));
+                const bool grow = mt > m + kSlack;
+                if (__builtin_amdgcn_ballot_w64(grow)) {
+                    const float f = grow ? __builtin_amdgcn_exp2f(m - mt) : 1.f;
+                    m = grow ? mt : m;
+                    l *= f;
+#pragma unroll
+                    for (int i = 0; i < kI8D / 32; ++i) o[i] *= f;
+                }
+                const float sub = m == -INFINITY ? 0.f : m;
+                v8h pb[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float add = bs[i].lv - sub, kc = bs[i].kc;
+                    float ps0 = 0.f, ps1 = 0.f;
+#pragma unroll
+                    for (int v = 0; v < 8; ++v) {
+                        const float x = s[i / 2][8 * (i % 2) + v];
+                        const float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(x, kc, add));
+                        if (v & 1) ps1 += pr; else ps0 += pr;
+                        pb[i][v] = (f16)pr;
+                    }
+                    const float sum = ps0 + ps1;
+                    if (sum != 0.f) l = __builtin_fmaf(sum, bs[i].rv, l);
+                }
+#pragma unroll
+                for (int st = 0; st < 4; ++st)
+#pragma unroll
+                    for (int db = 0; db < kI8D / 32; ++db) {
+                        const f16 *vr = &Vs[(16 * st + 4 * g + ((lane & 15) >> 2)) * VR + 32 * db +
+                                            16 * ((lane >> 4) & 1) + 4 * (lane & 3)];
+                        v4s x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                            (__attribute__((address_space(3))) v4s *)vr);
+                        v4s y = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                            (__attribute__((address_space(3))) v4s *)(vr + 8 * VR));
+                        const v4h xh = __builtin_bit_cast(v4h, x), yh = __builtin_bit_cast(v4h, y);
+                        const v8h av = {xh[0], xh[1], xh[2], xh[3], yh[0], yh[1], yh[2], yh[3]};
+                        o[db] = mfma32(av, pb[st], o[db]);
+                    }
+            }();
+            if (t + 1 < t_hi) store_tile(buf ^ 1);
+            __syncthreads();
+        }
+        l += __shfl_xor(l, 32);
+        if (ok && a.chunks == 1) {
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+            f16 *to = a.o + orow * kI8D;
+#pragma unroll
+            for (int db = 0; db < kI8D / 32; ++db)
+#pragma unroll
+                for (int grp = 0; grp < 4; ++grp) {
+                    v4h x;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[i] = (f16)(o[db][4 * grp + i] * inv);
+                    *reinterpret_cast<v4h *>(to + 32 * db + 8 * grp + 4 * g) = x;
+                }
+        } else if (ok) {
+            float *rec = a.tmp + (orow * a.chunks + chunk) * kRec;
+#pragma unroll
+            for (int db = 0; db < kI8D / 32; ++db)
+#pragma unroll
+                for (int grp = 0; grp < 4; ++grp)
+                    *reinterpret_cast<v4f *>(rec + 32 * db + 8 * grp + 4 * g) =
+                        (v4f){o[db][4 * grp], o[db][4 * grp + 1], o[db][4 * grp + 2],
+                              o[db][4 * grp + 3]};
+            if (g == 0) {
+                rec[kI8D] = m;
+                rec[kI8D + 1] = l;
+            }
+        }
+    }
+}
+
+// Join of the chunks: a block of 4 waves per (row, head), each wave a quarter of
+// the chunks, two dims per lane.  Lane c of a wave holds chunk c's maximum and
+// sum, so the weights need one reduction; the records are then read with all
+// loads in flight.
 __global__ __launch_bounds__(256) void attn_i8_merge_kernel(AttnI8Args a, int64_t batch) {
+    __shared__ float sx[4][kI8D], sm[4], ss[4];
     const int lane = threadIdx.x & 63;
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int64_t row = blockIdx.x;
     int64_t lo = 0, hi = a.rows;   // rows of the requests
     if (a.q_indptr) {
         lo = a.q_indptr[0];
@@ -338,40 +674,97 @@ __global__ __launch_bounds__(256) void attn_i8_merge_kernel(AttnI8Args a, int64_
     }
     if (row < lo * a.hq || row >= hi * a.hq) return;
     const float *rec = a.tmp + row * a.chunks * kRec;
-    float mx = -INFINITY;
-    for (int c = 0; c < a.chunks; ++c) mx = fmaxf(mx, rec[(int64_t)c * kRec + kI8D]);
-    float x = 0.f, y = 0.f, sum = 0.f;
-    for (int c = 0; c < a.chunks; ++c) {
-        const float *r = rec + (int64_t)c * kRec;
-        const float mc = r[kI8D];
-        const float f = mc == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mc - mx);
-        sum = __builtin_fmaf(r[kI8D + 1], f, sum);
-        x = __builtin_fmaf(r[2 * lane], f, x);
-        y = __builtin_fmaf(r[2 * lane + 1], f, y);
+    float m = -INFINITY, x = 0.f, y = 0.f, sum = 0.f;
+    const int per = (a.chunks + 3) / 4, end = min(a.chunks, (wave + 1) * per);
+    for (int c0 = wave * per; c0 < end; c0 += 64) {
+        const int c = c0 + lane;
+        float mc = -INFINITY, lc = 0.f;
+        if (c < end) {
+            const float2 v = *reinterpret_cast<const float2 *>(rec + (int64_t)c * kRec + kI8D);
+            mc = v.x;
+            lc = v.y;
+        }
+        const float to = fmaxf(m, wave_max(mc));
+        const float f = m == to ? 1.f : __builtin_amdgcn_exp2f(m - to);
+        // an empty chunk's record is zeros; NaN stays NaN
+        const float w = mc == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mc - to);
+        m = to;
+        sum = __builtin_fmaf(sum, f, wave_sum(lc * w));
+        x *= f;
+        y *= f;
+        const int n = min(64, end - c0);
+        const float *r = rec + (int64_t)c0 * kRec + 2 * lane;
+        for (int i0 = 0; i0 < n; i0 += 8) {
+            float2 v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i)   // past the end: the last record, weight 0
+                v[i] = *reinterpret_cast<const float2 *>(r + (int64_t)min(i0 + i, n - 1) * kRec);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float wi = i0 + i < n ? read_lane(w, i0 + i) : 0.f;
+                x = __builtin_fmaf(v[i].x, wi, x);
+                y = __builtin_fmaf(v[i].y, wi, y);
+            }
+        }
+    }
+    sx[wave][2 * lane] = x;
+    sx[wave][2 * lane + 1] = y;
+    if (lane == 0) {
+        sm[wave] = m;
+        ss[wave] = sum;
+    }
+    __syncthreads();
+    if (wave) return;
+    const float mx = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
+    x = y = sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        const float f = sm[w] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sm[w] - mx);
+        sum = __builtin_fmaf(ss[w], f, sum);
+        x = __builtin_fmaf(sx[w][2 * lane], f, x);
+        y = __builtin_fmaf(sx[w][2 * lane + 1], f, y);
     }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     reinterpret_cast<v2h *>(a.o + row * kI8D)[lane] = (v2h){(f16)(x * inv), (f16)(y * inv)};
 }
 
-// Row tiles per block and chunks of a request.
+// Kernel, row tiles and chunks of a request, from the sizes alone.  us on one
+// MI355X, B x (cached + new tokens), query / KV heads; "rows" are new tokens x
+// group.
+//  * Up to 16 rows, attn_i8_kernel<1>; a request and KV head is split until there
+//    is a block per CU (256), into pieces of 512 tokens or more: 8 x 2048 tokens
+//    over 8 heads in 1 / 2 / 4 / 8 chunks 19.8 / 15.9 / 13.9 / 15.1, 1 x 4096 33.8 /
+//    22.3 / 15.3 / 12.7, 1 x 60000 in 16 / 24 / 32 / 48 / 64 chunks 41 / 34 / 37 / 45 /
+//    45; 32 x 4096 (256 blocks) unsplit 45.2, in two 45.9.
+//  * Where blocks of 128 rows fill the CUs, attn_i8_rows_kernel: 4 x (5000 + 512),
+//    32 / 8 heads, 186 against 267 for the next form; 1 x 2048 new 85 against 102; at
+//    256 blocks, 2 x (1000 + 256) of 64 / 8 heads, 43.1 against 44.8.
+//  * Otherwise attn_i8_kernel<2>, four times as many blocks: 1 x (5000 + 512) 90
+//    against 158 (94 with the 128-row form in 4 chunks), 2 x (2000 + 128) of 64 / 8
+//    heads 34 against 65; split below 256 blocks until there are 512: 4 x (8000 + 8)
+//    in 2 / 4 / 8 / 16 chunks 55 / 35 / 28 / 37, 8 x (3000 + 8) 31 / 28.5 / 34 in 2 / 4 / 8
+//    (256 blocks, 2 x (1000 + 128) over 32 heads: unsplit 20.4, in two 28.6).
+enum { kRows16, kRows32, kRows128 };
 struct Plan {
-    int rt, tiles, chunks;
+    int form, tiles, chunks;
 };
 
 Plan plan_of(int64_t batch, int64_t group, int64_t H, int64_t max_q, int64_t max_kv) {
+    constexpr int64_t kCUs = 256;
     const int64_t rows = (max_q < 1 ? 1 : max_q) * group;
     Plan pl;
-    pl.rt = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-    int64_t tiles = srq_cdiv(rows, 16 * pl.rt);
-    if (tiles > 65536) tiles = 65536;
-    pl.tiles = (int)tiles;
+    pl.form = rows <= 16 ? kRows16
+              : batch * H * srq_cdiv(rows, kRowsBlock) >= kCUs ? kRows128 : kRows32;
+    int64_t tiles = srq_cdiv(rows, pl.form == kRows16 ? 16 : pl.form == kRows32 ? 32 : kRowsBlock);
+    if (tiles > 65536) tiles = 65536;   // the kernels' loops reach the rest
     const int64_t blocks = batch * H * tiles;
     int64_t chunks = 1;
-    if (blocks < 256) {
-        chunks = srq_cdiv(512, blocks);
-        const int64_t most = max_kv / 256 < 1 ? 1 : max_kv / 256;
+    if (blocks < kCUs) {
+        chunks = srq_cdiv(pl.form == kRows16 ? kCUs : 2 * kCUs, blocks);
+        const int64_t most = max_kv / 512 < 1 ? 1 : max_kv / 512;
         if (chunks > most) chunks = most;
     }
+    pl.tiles = (int)tiles;
     pl.chunks = (int)chunks;
     return pl;
 }
@@ -439,13 +832,13 @@ extern "C" int srq_batch_attention_i8(
     a.qmul = sm_scale > 0.f ? 1.f : sm_scale < 0.f ? -1.f : 0.f;
     hipStream_t st = (hipStream_t)stream;
     const dim3 grid((unsigned)(pl.chunks * pl.tiles), (unsigned)num_kv_heads, (unsigned)batch);
-    switch (pl.rt) {
-    case 1: attn_i8_kernel<1><<<grid, kWaves * 64, 0, st>>>(a, p); break;
-    case 2: attn_i8_kernel<2><<<grid, kWaves * 64, 0, st>>>(a, p); break;
-    default: attn_i8_kernel<4><<<grid, kWaves * 64, 0, st>>>(a, p); break;
+    switch (pl.form) {
+    case kRows16: attn_i8_kernel<1><<<grid, kWaves * 64, 0, st>>>(a, p); break;
+    case kRows32: attn_i8_kernel<2><<<grid, kWaves * 64, 0, st>>>(a, p); break;
+    default: attn_i8_rows_kernel<<<grid, kWaves * 64, 0, st>>>(a, p); break;
     }
     if (pl.chunks > 1)
-        attn_i8_merge_kernel<<<(unsigned)srq_cdiv(rows * n_q_heads, 4), 256, 0, st>>>(a, batch);
+        attn_i8_merge_kernel<<<(unsigned)(rows * n_q_heads), 256, 0, st>>>(a, batch);
     SRQ_LAUNCH_CHECK("batch_attention_i8");
     return SRQ_OK;
 }
