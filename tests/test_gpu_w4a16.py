@@ -35,7 +35,11 @@ def _run(x, c, s, z=None, bias=None):
 
 SHAPES = [(1, 1, 32, 32), (1, 16, 128, 128), (3, 17, 96, 32), (16, 48, 256, 64), (17, 33, 384, 128),
           (2, 1111, 1056, 96), (33, 80, 2048, 256), (5, 64, 11008, 128), (1, 4096, 4096, 128),
-          (7, 130, 1024, 1024), (64, 48, 640, 32), (70, 257, 512, 64), (4, 4096, 160, 160)]
+          (7, 130, 1024, 1024), (64, 48, 640, 32), (70, 257, 512, 64), (4, 4096, 160, 160),
+          # two row tiles a wave
+          (5, 8200, 384, 128), (1, 8193, 640, 32), (20, 8192, 1024, 64), (3, 8208, 1056, 96),
+          # more groups a wave than it holds in LDS at a time
+          (1, 16, 40960, 128), (3, 20, 20480, 64), (2, 16, 12288, 32), (16, 33, 9312, 96)]
 
 
 @pytest.mark.parametrize("M,N,K,group", SHAPES)
