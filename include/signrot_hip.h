@@ -746,7 +746,7 @@ int srq_qkv_norm_rope_append_i8(
  * them sees the first len - n + i + 1 cached tokens.  Grouped-query
  * (n_q_heads a multiple of H); logits q . k * sm_scale (finite).  o like q; a
  * row that sees nothing is 0, a row of no request stays as it is.  max_q_len and
- * max_kv_len size the launch and the workspace of ..._ws_bytes (any value is
+ * max_kv_len size the launch and the workspace of ..._workspace (any value is
  * correct). */
 int srq_batch_attention_i8(
     void *o, const void *q, int64_t rows, int64_t n_q_heads, const void *kv_data,
@@ -755,7 +755,7 @@ int srq_batch_attention_i8(
     int64_t num_layers, int64_t layer_idx, int64_t num_kv_heads, int64_t page_size,
     int64_t head_dim, const int32_t *q_indptr, int64_t max_q_len, int64_t max_kv_len,
     float sm_scale, void *ws, int64_t ws_bytes, void *stream);
-int srq_batch_attention_i8_ws_bytes(int64_t rows, int64_t batch, int64_t n_q_heads,
+int srq_batch_attention_i8_workspace(int64_t rows, int64_t batch, int64_t n_q_heads,
                                     int64_t n_kv_heads, int64_t max_q_len, int64_t max_kv_len,
                                     int64_t *bytes);
 

@@ -1104,7 +1104,7 @@ def qkv_norm_rope_append_i8(kv_data, kv_scale, kv_indptr, kv_indices, last_page_
 @functools.lru_cache(maxsize=512)
 def _attention_i8_bytes(rows, B, Hq, H, max_q_len, max_kv_len):
     n = ctypes.c_int64()
-    _call("srq_batch_attention_i8_ws_bytes", rows, B, Hq, H, max_q_len, max_kv_len,
+    _call("srq_batch_attention_i8_workspace", rows, B, Hq, H, max_q_len, max_kv_len,
           ctypes.byref(n))
     return n.value
 

@@ -96,7 +96,7 @@ SIGNATURES = {
                                     _p, _i64, _p, _p],
     "srq_batch_attention_i8": [_p, _p, _i64, _i64, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64,
                                _i64, _i64, _i64, _i64, _p, _i64, _i64, _f32, _p, _i64, _p],
-    "srq_batch_attention_i8_ws_bytes": [_i64, _i64, _i64, _i64, _i64, _i64, _p],
+    "srq_batch_attention_i8_workspace": [_i64, _i64, _i64, _i64, _i64, _i64, _p],
     "srq_w4a16_linear": [_p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _p, _p],
 }
 

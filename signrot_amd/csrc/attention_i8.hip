@@ -543,8 +543,10 @@ __global__ __launch_bounds__(kWaves * 64, 2) void attn_i8_rows_kernel(AttnI8Args
                     s[sb] = (v16f)0.f;
                     const f16 *row = &Ks[(32 * sb + ln) * KS + 8 * g];
 #pragma unroll
-                    for (int kk = 0; kk < kI8D / 16; ++kk)
-                        s[sb] = mfma32(*reinterpret_cast<const v8h *>(row + 16 * kk), qf[kk], s[sb]);
+                    for (int kk = 0; kk < kI8D / 16; ++kk) {
+                        const v8h kf = *reinterpret_cast<const v8h *>(row + 16 * kk);
+                        s[sb] = mfma32(kf, qf[kk], s[sb]);
+                    }
                 }
                 // the K operand reads run 4 ahead of the products that take them
                 __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
@@ -771,10 +773,10 @@ Plan plan_of(int64_t batch, int64_t group, int64_t H, int64_t max_q, int64_t max
 
 }  // namespace
 
-extern "C" int srq_batch_attention_i8_ws_bytes(int64_t rows, int64_t batch, int64_t n_q_heads,
+extern "C" int srq_batch_attention_i8_workspace(int64_t rows, int64_t batch, int64_t n_q_heads,
                                                int64_t n_kv_heads, int64_t max_q_len,
                                                int64_t max_kv_len, int64_t *bytes) {
-    SRQ_CHECK_ARG(bytes, "batch_attention_i8_ws_bytes: null pointer");
+    SRQ_CHECK_ARG(bytes, "batch_attention_i8_workspace: null pointer");
     SRQ_CHECK_ARG(rows >= 0 && batch >= 0 && n_kv_heads > 0 && n_q_heads > 0 &&
                       n_q_heads % n_kv_heads == 0,
                   "batch_attention_i8: %lld query heads for %lld KV heads", (long long)n_q_heads,

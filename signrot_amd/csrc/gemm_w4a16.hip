@@ -208,7 +208,7 @@ __global__ __launch_bounds__(W * 64) void w4a16_kernel(W4Args a) {
 #pragma unroll
             for (int s = 0; s < 4; ++s) {
                 if (s * G % 4 == 0) pair = own.s[t][col][G * j + s * G / 4];
-                const u32 zz = __builtin_amdgcn_perm(0u, pair, 0x03020302u);   // its high half twice
+                const u32 zz = __builtin_amdgcn_perm(0u, pair, 0x03020302u);   // its zero twice
                 const u32 c = ASYM ? (u32)w[s] : (u32)w[s] ^ 0x88888888u;      // signed: code + 8
                 p = mfma16(xv[s], codes8(c, __builtin_bit_cast(v2h, zz)), p);
                 if ((s + 1) * G % 4 == 0) {

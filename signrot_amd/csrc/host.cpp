@@ -598,8 +598,8 @@ PyObject *batch_attention_i8(PyObject *, PyObject *const *a, Py_ssize_t n_args) 
         if (kv < 1) kv = 1;
         const float scale = a[11] == Py_None ? 0.08838834764831845f : as_float(a[11]);
         int64_t wb = 0;
-        check(srq_batch_attention_i8_ws_bytes(rows, c.B, hq, c.H, hint, kv, &wb),
-              "srq_batch_attention_i8_ws_bytes");
+        check(srq_batch_attention_i8_workspace(rows, c.B, hq, c.H, hint, kv, &wb),
+              "srq_batch_attention_i8_workspace");
         int rc;
         {
             NoGil nogil;

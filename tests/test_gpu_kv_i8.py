@@ -182,7 +182,8 @@ def test_append_far_pages():
     q = rng.standard_normal((2, 16, D)).astype(np.float16)
     o = torch.zeros(2, 16, D, dtype=torch.float16, device=DEV)
     _CUDA.batch_attention_i8(o, to_dev(q), data, scale, *t, 0)
-    small = [np.zeros((2, 1, 2, H, page, D), np.int8), np.zeros((2, 1, 2, H, page // 16), np.float32)]
+    small = [np.zeros((2, 1, 2, H, page, D), np.int8),
+             np.zeros((2, 1, 2, H, page // 16), np.float32)]
     host = [np.array(a, np.int32) for a in ([0, 1, 2], [0, 1], [7, 200])]
     i8_ref.append(*small, *host, 0, k, v, new)
     for i, pg in enumerate((pages - 1, 8300)):

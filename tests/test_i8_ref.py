@@ -84,7 +84,8 @@ def test_cache_refusals(lib, kw, msg):
 
 @pytest.mark.parametrize("args,msg", [
     ([P, P, 256, 256, 3, None, 1, None], "3 rows"), ([None, P, 256, 256, 2, None, 1, None], "null"),
-    ([P, P, 128, 256, 2, None, 1, None], "strides"), ([P, P, 260, 256, 2, None, 1, None], "strides"),
+    ([P, P, 128, 256, 2, None, 1, None], "strides"),
+    ([P, P, 260, 256, 2, None, 1, None], "strides"),
     ([ctypes.c_void_p(8), P, 256, 256, 2, None, 1, None], "aligned"),
     ([P, P, 256, 256, -1, P, 1, None], "rows")])
 def test_append_refusals(lib, args, msg):
@@ -104,8 +105,8 @@ def test_attention_refusals(lib):
         assert call(**kw) == -1
         assert msg in lib.srq_last_error().decode()
     n = ctypes.c_int64()
-    assert lib.srq_batch_attention_i8_ws_bytes(2, 2, 5, 2, 1, 100, ctypes.byref(n)) == -1
-    assert lib.srq_batch_attention_i8_ws_bytes(2, 2, 4, 2, 1, 100, None) == -1
+    assert lib.srq_batch_attention_i8_workspace(2, 2, 5, 2, 1, 100, ctypes.byref(n)) == -1
+    assert lib.srq_batch_attention_i8_workspace(2, 2, 4, 2, 1, 100, None) == -1
 
 
 def test_norm_rope_refusals(lib):
