@@ -29,6 +29,8 @@ __all__ = [
     "matmul_colrow_i8_i32",
     "w4a4_linear_asym",
     "w4a4_linear_moe_asym",
+    "qk_norm_rope",
+    "w4a16_linear",
     "PackedQuantizedTensor",
 ]
 
@@ -219,6 +221,19 @@ def rope_qk(q, k, cos, sin):
     rounding (signrot/functional/kernel.py:158-165)."""
     _CUDA.rope_qk(q, k, cos.contiguous(), sin.contiguous())
     return q, k
+
+
+def qk_norm_rope(q, k, cos, sin, q_weight=None, k_weight=None, eps=1e-6):
+    """RMSNorm of each query and key head with the rotary embedding in the same
+    pass, fp32 with one rounding: new dense (q, k) of q [B, T, Hq, D] and k [B, T,
+    Hk, D], which may be column slices of one projection output."""
+    return _CUDA.qk_norm_rope(q, k, cos.contiguous(), sin.contiguous(), q_weight, k_weight, eps)
+
+
+def w4a16_linear(x, weight, scales, zeros=None, bias=None):
+    """fp16 x [..., K] through 4-bit weights u8 [N, K / 2] with scales (and zero
+    points) [N, K / group] for each group of input columns: fp16 [..., N]."""
+    return _CUDA.w4a16_linear(x.contiguous(), weight, scales, zeros, bias)
 
 
 def swiglu(gate, up):

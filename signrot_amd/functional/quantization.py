@@ -82,6 +82,35 @@ def unpack_ui4(x: torch.Tensor):
     return torch.stack((lo, hi), dim=-1).reshape(*x.shape[:-1], x.shape[-1] * 2)
 
 
+def rtn_group_pack(w: torch.Tensor, groupsize: int, sym: bool = True, scales=None, zeros=None):
+    """Round-to-nearest int4 of an fp16 weight [N, K] with a scale for each group
+    of `groupsize` columns, on the grid that the kernels compute with (the fp16
+    scales): symmetric, s = fp16(max|W| / 7), codes clamp(round(W / s), -8, 7);
+    else over the range widened to 0, s = fp16((max - min) / 15), z = round(-min /
+    s), codes clamp(round(W / s) + z, 0, 15).  Given scales (and zeros), as those
+    that a weight was quantized with, only the codes are made.  Returns (packed
+    u8 [N, K / 2], scales f16 [N, K / groupsize], zeros u8 or None)."""
+    n, k = w.shape
+    g = w.float().view(n, k // groupsize, groupsize)
+    if scales is None:
+        lo, hi = g.amin(-1).clamp(max=0), g.amax(-1).clamp(min=0)
+        if sym:
+            scales = torch.maximum(-lo, hi).clamp(min=1e-5) / 7
+        else:
+            scales = (hi - lo).clamp(min=1e-5) / 15
+            zeros = torch.round(-lo / scales.half().float()).clamp(0, 15)
+    scales = scales.half()
+    c = torch.round(g / scales.float()[..., None])
+    if sym:
+        q = c.clamp(-8, 7).to(torch.int8).view(torch.uint8) & 15
+    else:
+        zeros = zeros.to(torch.uint8)
+        q = (c + zeros.float()[..., None]).clamp(0, 15).to(torch.uint8)
+    q = q.view(n, k)
+    return (q[:, 0::2] | (q[:, 1::2] << 4)).contiguous(), scales.contiguous(), \
+        None if sym else zeros.contiguous()
+
+
 def rtn_weight_pack(w: torch.Tensor, symmetric_grid: bool = False):
     """Per-output-channel symmetric int4 RTN of an fp16 weight [N, K] and its
     kernel form (fake_quant/quant_utils.py:453-529 WeightQuantizer

@@ -1,4 +1,4 @@
-from .linear import Linear4bit, AsymSymmLinear4bit
+from .linear import Linear4bit, AsymSymmLinear4bit, GroupLinear4bit
 from .quantization import Quantizer, SymQuantizer, AsymQuantizer
 from .hadamard import OnlineHadamard, HadamardQuantizer, fuse_online_hadamard
 from .normalization import RMSNorm

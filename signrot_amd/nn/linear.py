@@ -143,3 +143,82 @@ class AsymSymmLinear4bit(torch.nn.Module):
             if module.bias is not None:
                 int_module.bias.copy_(module.bias)
         return int_module
+
+
+class GroupLinear4bit(torch.nn.Module):
+    """4-bit weights with a scale (and a zero point) for each group of input
+    columns, over fp16 activations: what group-wise quantized checkpoints and
+    GPTQ with a groupsize need, which one scale per output channel cannot hold.
+
+    Buffers: weight u8 [out, in/2] packed int4 (signed codes; unsigned with
+    weight_zeros), weight_scales f16 [out, in/group], weight_zeros u8 [out, in/group]
+    when not sym, optional fp16 bias [out].
+
+    forward(tensor): up to `MAX_ROWS` tokens on the GPU go through w4a16_linear,
+    which reads the packed weight once; more of them, an input that wants a
+    gradient or one on the host are a matrix product with the dequantized weight."""
+
+    # us on one MI355X, w4a16_linear against dequantization and product: 512 rows
+    # through 4096 x 4096 85 / 231, 8192 x 28672 902 / 3409, 28672 x 4096 611 / 1569
+    MAX_ROWS = 1024
+
+    weight: torch.Tensor
+    weight_scales: torch.Tensor
+    weight_zeros: torch.Tensor | None
+    bias: torch.Tensor | None
+
+    def __init__(self, in_features, out_features, groupsize=128, sym=True, bias=False):
+        super().__init__()
+        if groupsize <= 0 or groupsize % 32 or in_features % groupsize:
+            raise ValueError("groupsize must be a multiple of 32 that divides in_features")
+        self.in_features, self.out_features = in_features, out_features
+        self.groupsize, self.sym = groupsize, sym
+        groups = in_features // groupsize
+        self.register_buffer("weight", torch.zeros((out_features, in_features // 2),
+                                                   dtype=torch.uint8))
+        self.register_buffer("weight_scales", torch.zeros((out_features, groups),
+                                                          dtype=torch.float16))
+        if sym:
+            self.weight_zeros = None
+        else:
+            self.register_buffer("weight_zeros", torch.zeros((out_features, groups),
+                                                             dtype=torch.uint8))
+        if bias:
+            self.register_buffer("bias", torch.zeros(out_features, dtype=torch.float16))
+        else:
+            self.bias = None
+
+    def dequantized(self):
+        """The fp16 weight [out, in]: scale * (code - zero), rounded once."""
+        if self.sym:
+            c = quant_utils.unpack_i4(self.weight).float()
+        else:
+            c = quant_utils.unpack_ui4(self.weight).float()
+        c = c.view(self.out_features, -1, self.groupsize)
+        if not self.sym:
+            c = c - self.weight_zeros.float()[..., None]
+        return (c * self.weight_scales.float()[..., None]).view(self.out_features,
+                                                                self.in_features).half()
+
+    def forward(self, x):
+        if (x.is_cuda and x.numel() <= self.MAX_ROWS * self.in_features
+                and not (x.requires_grad and torch.is_grad_enabled())):
+            return kernel.w4a16_linear(x, self.weight, self.weight_scales, self.weight_zeros,
+                                       self.bias)
+        return torch.nn.functional.linear(x, self.dequantized(), self.bias)
+
+    @staticmethod
+    def from_float(module: torch.nn.Linear, groupsize=128, sym=True, scales=None, zeros=None):
+        """Round-to-nearest quantization of an fp16 Linear, or with given scales
+        (and zeros) [out, in / groupsize] the codes of a weight that lies on their
+        grid."""
+        w = module.weight.data
+        out = GroupLinear4bit(module.in_features, module.out_features, groupsize, sym,
+                              module.bias is not None)
+        packed, s, z = quant_utils.rtn_group_pack(w, groupsize, sym, scales, zeros)
+        out.weight, out.weight_scales = packed, s
+        if not sym:
+            out.weight_zeros = z
+        if module.bias is not None:
+            out.bias = module.bias.data.half().clone()
+        return out

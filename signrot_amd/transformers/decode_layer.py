@@ -25,6 +25,7 @@ from ..functional.quantization import rtn_weight_pack
 from ..nn.derived import derived
 from ..nn.normalization import RMSNorm
 from .kv_cache import qkv_prefill_of
+from .kv_cache_i8 import MultiLayerPagedKVCache8Bit
 
 
 def rope_cos_sin(positions, head_dim, theta, device):
@@ -43,10 +44,15 @@ class W4A4LlamaDecodeLayer(torch.nn.Module):
       w_qkv [Hq*D + 2*Hkv*D, hidden/2], w_o [hidden, hidden/2],
       w_gu [2*ffn, hidden/2] (gate rows then up rows), w_down [hidden, ffn/2],
     and down_sign int8 [ffn] (the SignRot ±1 vector of the down-proj
-    rotation)."""
+    rotation).  qk_norm: each query and key head goes through an RMSNorm before
+    the rotary embedding (fp16 weights q_norm, k_norm [head_dim]).
+
+    The cache may also be a MultiLayerPagedKVCache8Bit.  Its decode step runs the
+    q/k/v pass in fp32 with one rounding, so there the fused and the op-by-op form
+    agree within fp16 roundings, and not bit for bit."""
 
     def __init__(self, hidden, n_heads, n_kv_heads, head_dim, ffn, layer_idx=0, eps=1e-5,
-                 rope_theta=500000.0):
+                 rope_theta=500000.0, qk_norm=False):
         super().__init__()
         assert hidden == n_heads * head_dim and n_heads % n_kv_heads == 0
         self.hidden, self.n_heads, self.n_kv = hidden, n_heads, n_kv_heads
@@ -60,6 +66,10 @@ class W4A4LlamaDecodeLayer(torch.nn.Module):
             self.register_buffer(f"w_{name}", torch.zeros(rows, cols // 2, dtype=torch.uint8))
             self.register_buffer(f"s_{name}", torch.zeros(rows, dtype=torch.float16))
         self.register_buffer("down_sign", torch.ones(ffn, dtype=torch.int8))
+        self.qk_norm, self.eps = qk_norm, eps
+        if qk_norm:
+            self.register_buffer("q_norm", torch.ones(head_dim, dtype=torch.float16))
+            self.register_buffer("k_norm", torch.ones(head_dim, dtype=torch.float16))
         had, k = get_hadK(ffn)
         self.down_k = k
         self.register_buffer("down_hadk", had.half() if had is not None else None)
@@ -96,6 +106,13 @@ class W4A4LlamaDecodeLayer(torch.nn.Module):
         return _CUDA.w4a4_linear(q.view(-1, q.shape[-1]), s.view(-1), getattr(self, f"w_{name}"),
                                  getattr(self, f"s_{name}"))
 
+    def _rope(self, q, k, cos, sin):
+        """RoPE of q and k [B, T, H, D], behind their norms where the layer has
+        them (dense new tensors then, else in place)."""
+        if self.qk_norm:
+            return kernel.qk_norm_rope(q, k, cos, sin, self.q_norm, self.k_norm, self.eps)
+        return kernel.rope_qk(q, k, cos, sin)
+
     def forward(self, hidden_states, cache, cos, sin, trace=None, fused=True,
                 attention_mask=None):
         """hidden_states fp16 [B, 1, hidden]; cos/sin fp16 [1 or B, 1, head_dim]
@@ -124,8 +141,21 @@ class W4A4LlamaDecodeLayer(torch.nn.Module):
         n1, n2 = self.input_layernorm, self.post_attention_layernorm
         q1, s1 = _CUDA.rmsnorm_quant(x2, n1.eps, n1.mean_dim)
         qkv = _CUDA.w4a4_linear(q1, s1.view(-1), self.w_qkv, self.s_qkv)
-        qa, sa = cache.update_qkv_decode_quant(qkv, cos, sin, self.layer_idx, self.n_heads,
-                                               _inv_sqrt_f32(self.n_heads), attention_mask)
+        had = _inv_sqrt_f32(self.n_heads)
+        if not self.qk_norm:
+            qa, sa = cache.update_qkv_decode_quant(qkv, cos, sin, self.layer_idx, self.n_heads,
+                                                   had, attention_mask)
+        elif isinstance(cache, MultiLayerPagedKVCache8Bit):
+            qa, sa = cache.update_qkv_decode_quant(qkv, cos, sin, self.layer_idx, self.n_heads,
+                                                   had, attention_mask, self.q_norm, self.k_norm,
+                                                   self.eps)
+        else:   # the norms, then the cache's own update
+            heads = qkv.view(B, 1, -1, self.head_dim)
+            q, k, v = heads.split((self.n_heads, self.n_kv, self.n_kv), dim=2)
+            q, k = self._rope(q, k, cos, sin)
+            attend = cache.update(k, v.contiguous(), self.layer_idx,
+                                  {"attention_mask": attention_mask})
+            qa, sa = _CUDA.head_had_quant(attend(q).view(B, self.n_heads, self.head_dim), had)
         x2 = _CUDA.w4a4_linear_residual(qa, sa.view(-1), self.w_o, self.s_o, x2)
         q2, s2 = _CUDA.rmsnorm_quant(x2, n2.eps, n2.mean_dim)
         if self.ffn % 8 == 0:
@@ -165,7 +195,7 @@ class W4A4LlamaDecodeLayer(torch.nn.Module):
         q = qkv[:, : Hq * D].contiguous().view(B, 1, Hq, D)
         k = qkv[:, Hq * D: (Hq + Hk) * D].contiguous().view(B, 1, Hk, D)
         v = qkv[:, (Hq + Hk) * D:].contiguous().view(B, 1, Hk, D)
-        kernel.rope_qk(q, k, cos, sin)
+        q, k = self._rope(q, k, cos, sin)
         keep("q_rope", q)
         keep("k_rope", k)
         attend = cache.update(k, v, self.layer_idx, {"attention_mask": attention_mask})
@@ -201,7 +231,7 @@ class W4A4LlamaDecodeLayer(torch.nn.Module):
         q = qkv[:, : Hq * D].reshape(B, T, Hq, D).contiguous()
         k = qkv[:, Hq * D: (Hq + Hk) * D].reshape(B, T, Hk, D).contiguous()
         v = qkv[:, (Hq + Hk) * D:].reshape(B, T, Hk, D).contiguous()
-        kernel.rope_qk(q, k, cos, sin)
+        q, k = self._rope(q, k, cos, sin)
         keep("q_rope", q)
         keep("k_rope", k)
         out = cache.update(k, v, self.layer_idx, {"attention_mask": attention_mask})
@@ -233,8 +263,8 @@ class W4A4LlamaDecodeLayer(torch.nn.Module):
     def _prefill_fused(self, hidden_states, cache, cos, sin, attention_mask):
         """rmsnorm_quant -> q/k/v GEMM -> prefill_qkv_cache (RoPE in place, K
         Hadamard, KV quantize + cache fill; the op-by-op update when padding
-        has to be left out of the cache, or the cache has only an update(), or
-        one of its own) -> prefill attention over the strided
+        has to be left out of the cache, the heads have norms, or the cache has
+        only an update(), or one of its own) -> prefill attention over the strided
         views -> head_had_quant -> o_proj GEMM + residual -> rmsnorm_quant ->
         gate/up GEMM -> swiglu_had_sign_quant -> down GEMM + residual."""
         B, T, _ = hidden_states.shape
@@ -243,13 +273,19 @@ class W4A4LlamaDecodeLayer(torch.nn.Module):
         n1, n2 = self.input_layernorm, self.post_attention_layernorm
         q1, s1 = _CUDA.rmsnorm_quant(x2, n1.eps, n1.mean_dim)
         qkv = _CUDA.w4a4_linear(q1, s1.view(-1), self.w_qkv, self.s_qkv)
-        fill = None if attention_mask is not None else qkv_prefill_of(cache)
+        fill = None
+        if attention_mask is None and not self.qk_norm:
+            fill = qkv_prefill_of(cache)
         if fill is not None:
             q, k, v = fill(qkv.view(B, T, -1), cos, sin, self.layer_idx, Hq)
         else:
             heads = qkv.view(B, T, Hq + 2 * Hk, D).split((Hq, Hk, Hk), dim=2)
-            q, k, v = (t.contiguous() for t in heads)
-            kernel.rope_qk(q, k, cos, sin)
+            if self.qk_norm:
+                q, k = self._rope(heads[0], heads[1], cos, sin)
+                v = heads[2].contiguous()
+            else:
+                q, k, v = (t.contiguous() for t in heads)
+                kernel.rope_qk(q, k, cos, sin)
             out = cache.update(k, v, self.layer_idx, {"attention_mask": attention_mask})
             if not isinstance(out, tuple):
                 raise RuntimeError("prefill: the cache already holds this layer's context")
