@@ -37,19 +37,35 @@ struct AppendArgs {
     float eps;
 };
 
-SRQ_DEV float code_of(float t, double num, double den) {
-    float c = __builtin_rintf(t);
-    if (fabsf(fabsf(t - c) - 0.5f) < 0x1p-14f) c = (float)__builtin_rint(num / den);
-    return fminf(fmaxf(c, -127.f), 127.f);
-}
-
-SRQ_DEV uint2 pack8_i8(const float (&c)[8]) {
+// rne(f num / den) of eight values, |f num / den| <= 127 (and under 128 with the
+// fp32 quotient's error), packed; r = num / den in fp32.  Adding 1.5 2^23 rounds to
+// nearest and leaves the code in the low byte; what the quotient then is off its
+// code tells the ones that lie near a half.
+SRQ_DEV uint2 codes_row(const float (&f)[8], float r, double num, double den) {
+    constexpr float kMagic = 12582912.f, kNear = 0.5f - 0x1p-14f;
+    float y[8];
+    bool near = false;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const float t = f[e] * r;
+        y[e] = t + kMagic;
+        near |= fabsf(t - (y[e] - kMagic)) > kNear;
+    }
+    if (__builtin_amdgcn_ballot_w64(near)) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (fabsf(f[e] * r - (y[e] - kMagic)) > kNear)
+                y[e] = (float)__builtin_rint(f[e] * num / den) + kMagic;
+    }
     u32 w[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        w[h] = 0;
+        u32 u[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) w[h] |= ((u32)(int)c[4 * h + e] & 0xFF) << (8 * e);
+        for (int e = 0; e < 4; ++e) u[e] = __builtin_bit_cast(u32, y[4 * h + e]);
+        const u32 lo = __builtin_amdgcn_perm(u[1], u[0], 0x0c0c0400u);
+        const u32 hi = __builtin_amdgcn_perm(u[3], u[2], 0x04000c0cu);
+        w[h] = lo | hi;
     }
     return make_uint2(w[0], w[1]);
 }
@@ -57,7 +73,8 @@ SRQ_DEV uint2 pack8_i8(const float (&c)[8]) {
 template <bool FUSED>
 __global__ __launch_bounds__(256) void append_kernel(AppendArgs a, PagedI8 p) {
     const int64_t b = blockIdx.y;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int l = lane & 15, r4 = lane >> 4;
     int64_t s0, n;
     i8_new_rows(a.new_indptr, b, a.rows, s0, n);
@@ -95,26 +112,33 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a, PagedI8 p) {
         const int64_t jj = (uint32_t)it / (uint32_t)(2 * p.H);
         const int hv = (int)(it - jj * 2 * p.H), kv = hv / p.H, h = hv - kv * p.H;
         const int64_t j = j0 + jj, t0 = j * kI8Block;
+        const int held = (int)(old > t0 ? old - t0 : 0);   // older tokens of the block
+        const int fill = (int)(rq.len - t0 < kI8Block ? rq.len - t0 : kI8Block);
+        const f16 *src = kv ? a.v : a.k;
+        const int64_t tok = kv ? a.v_tok : a.k_tok;
+        // the new rows first: the table's dependent reads overlap them (a row that is
+        // not new reads the block's first one that is)
+        v8h x[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int e = 4 * i + r4;                       // row of the block
+            const int64_t row = s0 + t0 + (e >= held && e < fill ? e : held) - old;
+            x[i] = *reinterpret_cast<const v8h *>(src + row * tok + h * kI8D + 8 * l);
+        }
         const int64_t pg = i8_page(p, rq.first, j);
         if (pg < 0) continue;
         const int64_t si = i8_scale_index(p, pg, h, (uint32_t)j % (uint32_t)p.bpp) +
                            (int64_t)kv * p.H * p.bpp;
         int8_t *codes = p.data + si * (kI8Block * kI8D);   // a block's rows are consecutive
-        const int held = (int)(old > t0 ? old - t0 : 0);   // older tokens of the block
-        const int fill = (int)(rq.len - t0 < kI8Block ? rq.len - t0 : kI8Block);
         const float was = held > 0 ? p.scale[si] : 0.f;
-        const f16 *src = kv ? a.v : a.k;
-        const int64_t tok = kv ? a.v_tok : a.k_tok;
-        v8h x[4];
         float amax = 0.f;
         bool bad = !(was <= 3e38f);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int e = 4 * i + r4;                       // row of the block
+            const int e = 4 * i + r4;
             const bool fresh = e >= held && e < fill;
             const int64_t row = s0 + t0 + e - old;
-            x[i] = (v8h){};
-            if (fresh) x[i] = *reinterpret_cast<const v8h *>(src + row * tok + h * kI8D + 8 * l);
+            if (!fresh) x[i] = (v8h){};
             if (FUSED && kv == 0) {
                 const int64_t ct = (a.cos_one || !fresh ? 0 : row) * kI8D + 8 * l;
                 const v8h c = *reinterpret_cast<const v8h *>(a.cs + ct);
@@ -139,23 +163,19 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a, PagedI8 p) {
         for (int i = 0; i < 4; ++i) {
             const int e = 4 * i + r4;
             uint2 *at = reinterpret_cast<uint2 *>(codes + e * kI8D + 8 * l);
-            float c[8];
+            float f[8];
             if (e >= held && e < fill) {
 #pragma unroll
-                for (int d = 0; d < 8; ++d) {
-                    const float f = (float)x[i][d];
-                    c[d] = live ? code_of(f * rs, f, now) : 0.f;
-                }
-                *at = pack8_i8(c);
+                for (int d = 0; d < 8; ++d) f[d] = live ? (float)x[i][d] : 0.f;
+                *at = codes_row(f, rs, 1.0, now);
             } else if (moved && e < held) {
                 const uint2 o = *at;
 #pragma unroll
                 for (int d = 0; d < 8; ++d) {
                     const u32 w = d < 4 ? o.x : o.y;
-                    const float f = (float)(int)(int8_t)(w >> (8 * (d & 3)));
-                    c[d] = live ? code_of(f * ratio, (double)f * was, now) : 0.f;
+                    f[d] = live ? (float)(int)(int8_t)(w >> (8 * (d & 3))) : 0.f;
                 }
-                *at = pack8_i8(c);
+                *at = codes_row(f, ratio, was, now);
             }
         }
         if (lane == 0 && (held == 0 || now != was)) p.scale[si] = now;
