@@ -46,6 +46,12 @@ def _stream(t):
     return torch.cuda.current_stream(t.device).cuda_stream if s is None else s
 
 
+def _call_on(t, name, *args):
+    """_call with t's device current, whichever the caller's is."""
+    with torch.cuda.device(t.device):
+        _call(name, *args)
+
+
 def _check(name, tensors, dtypes=None, contiguous=True):
     dev = None
     for i, (t, tname) in enumerate(tensors):
@@ -975,10 +981,10 @@ def qk_norm_rope(q, k, cos, sin, q_weight=None, k_weight=None, eps=1e-6):
                                       for t, n in ((q, "q"), (k, "k")))
     qo = torch.empty((B, T, Hq, D), dtype=f16, device=q.device)
     ko = torch.empty(k.shape, dtype=f16, device=q.device)
-    _call("srq_qk_norm_rope", _ptr(q), _ptr(k), _ptr(cos), _ptr(sin), cos.shape[0],
-          _ptr(q_weight), _ptr(k_weight), 0.0 if eps is None else float(eps),
-          0 if eps is None else 1, B, T, Hq, k.shape[2], D, q_tok, q_seq, k_tok, k_seq, _ptr(qo),
-          _ptr(ko), _stream(q))
+    _call_on(q, "srq_qk_norm_rope", _ptr(q), _ptr(k), _ptr(cos), _ptr(sin), cos.shape[0],
+             _ptr(q_weight), _ptr(k_weight), 0.0 if eps is None else float(eps),
+             0 if eps is None else 1, B, T, Hq, k.shape[2], D, q_tok, q_seq, k_tok, k_seq, _ptr(qo),
+             _ptr(ko), _stream(q))
     return qo, ko
 
 
@@ -1058,9 +1064,9 @@ def append_kv_i8(kv_data, kv_scale, kv_indptr, kv_indices, last_page_offset, lay
         if t.stride(2) != 1 or (H > 1 and t.stride(1) != 128):
             raise RuntimeError(f"{name}: {tname} must be dense in its last two dims")
         toks.append(t.stride(0) if rows > 1 else H * 128)
-    _call("srq_append_kv_i8", _ptr(kv_data), _ptr(kv_scale), _ptr(kv_indptr), _ptr(kv_indices),
-          _ptr(last_page_offset), *head, int(layer_idx), *tail, _ptr(k), _ptr(v), *toks, rows,
-          _ptr(new_indptr), hint, _stream(kv_data))
+    _call_on(kv_data, "srq_append_kv_i8", _ptr(kv_data), _ptr(kv_scale), _ptr(kv_indptr),
+             _ptr(kv_indices), _ptr(last_page_offset), *head, int(layer_idx), *tail, _ptr(k),
+             _ptr(v), *toks, rows, _ptr(new_indptr), hint, _stream(kv_data))
 
 
 def qkv_norm_rope_append_i8(kv_data, kv_scale, kv_indptr, kv_indices, last_page_offset, layer_idx,
@@ -1093,11 +1099,11 @@ def qkv_norm_rope_append_i8(kv_data, kv_scale, kv_indptr, kv_indices, last_page_
     _check_norm(name, q_weight, k_weight, eps, 128)
     hint = _check_new(name, new_indptr, "new_indptr", rows, B, max_new, kv_data)
     q = torch.empty((rows, n_q_heads, 128), dtype=f16, device=qkv.device)
-    _call("srq_qkv_norm_rope_append_i8", _ptr(kv_data), _ptr(kv_scale), _ptr(kv_indptr),
-          _ptr(kv_indices), _ptr(last_page_offset), *head, int(layer_idx), *tail, _ptr(qkv),
-          qkv.stride(0) if rows > 1 else cols, rows, _ptr(cos), _ptr(sin), cos.shape[0], n_q_heads,
-          _ptr(q_weight), _ptr(k_weight), 0.0 if eps is None else float(eps),
-          0 if eps is None else 1, _ptr(new_indptr), hint, _ptr(q), _stream(kv_data))
+    _call_on(qkv, "srq_qkv_norm_rope_append_i8", _ptr(kv_data), _ptr(kv_scale), _ptr(kv_indptr),
+             _ptr(kv_indices), _ptr(last_page_offset), *head, int(layer_idx), *tail, _ptr(qkv),
+             qkv.stride(0) if rows > 1 else cols, rows, _ptr(cos), _ptr(sin), cos.shape[0], n_q_heads,
+             _ptr(q_weight), _ptr(k_weight), 0.0 if eps is None else float(eps),
+             0 if eps is None else 1, _ptr(new_indptr), hint, _ptr(q), _stream(kv_data))
     return q
 
 
@@ -1139,9 +1145,9 @@ def batch_attention_i8(o, q, kv_data, kv_scale, kv_indptr, kv_indices, last_page
     if n:
         ws = torch.empty(n, dtype=torch.uint8, device=q.device)
     scale = 128 ** -0.5 if softmax_scale is None else float(softmax_scale)
-    _call("srq_batch_attention_i8", _ptr(o), _ptr(q), rows, Hq, _ptr(kv_data), _ptr(kv_scale),
-          _ptr(kv_indptr), _ptr(kv_indices), _ptr(last_page_offset), *head, int(layer_idx), *tail,
-          _ptr(q_indptr), hint, kv, scale, _ptr(ws), n, _stream(q))
+    _call_on(q, "srq_batch_attention_i8", _ptr(o), _ptr(q), rows, Hq, _ptr(kv_data), _ptr(kv_scale),
+             _ptr(kv_indptr), _ptr(kv_indices), _ptr(last_page_offset), *head, int(layer_idx), *tail,
+             _ptr(q_indptr), hint, kv, scale, _ptr(ws), n, _stream(q))
     return o
 
 
@@ -1175,8 +1181,8 @@ def w4a16_linear(x, w, scales, zeros=None, bias=None):
         raise RuntimeError("w4a16_linear: bias must have N elements")
     M = x.numel() // K
     out = torch.empty((*x.shape[:-1], N), dtype=f16, device=x.device)
-    _call("srq_w4a16_linear", _ptr(x), _ptr(w), _ptr(scales), _ptr(zeros), _ptr(bias), M, N, K,
-          K // groups, _ptr(out), _stream(x))
+    _call_on(x, "srq_w4a16_linear", _ptr(x), _ptr(w), _ptr(scales), _ptr(zeros), _ptr(bias), M, N,
+             K, K // groups, _ptr(out), _stream(x))
     return out
 
 

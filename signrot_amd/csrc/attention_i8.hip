@@ -31,6 +31,7 @@
 
 #include <math.h>
 
+#include <algorithm>
 #include <type_traits>
 
 namespace {
@@ -663,18 +664,10 @@ __global__ __launch_bounds__(kWaves * 64, 2) void attn_i8_rows_kernel(AttnI8Args
 // the chunks, two dims per lane.  Lane c of a wave holds chunk c's maximum and
 // sum, so the weights need one reduction; the records are then read with all
 // loads in flight.
-__global__ __launch_bounds__(256) void attn_i8_merge_kernel(AttnI8Args a, int64_t batch) {
-    __shared__ float sx[4][kI8D], sm[4], ss[4];
+SRQ_DEV void merge_row(const AttnI8Args &a, int64_t row, float (&sx)[4][kI8D], float (&sm)[4],
+                       float (&ss)[4]) {
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const int64_t row = blockIdx.x;
-    int64_t lo = 0, hi = a.rows;   // rows of the requests
-    if (a.q_indptr) {
-        lo = a.q_indptr[0];
-        hi = a.q_indptr[batch];
-        hi = hi > a.rows ? a.rows : hi;
-    }
-    if (row < lo * a.hq || row >= hi * a.hq) return;
     const float *rec = a.tmp + row * a.chunks * kRec;
     float m = -INFINITY, x = 0.f, y = 0.f, sum = 0.f;
     const int per = (a.chunks + 3) / 4, end = min(a.chunks, (wave + 1) * per);
@@ -716,7 +709,7 @@ __global__ __launch_bounds__(256) void attn_i8_merge_kernel(AttnI8Args a, int64_
         ss[wave] = sum;
     }
     __syncthreads();
-    if (wave) return;
+    if (wave) return;   // to the caller's barrier
     const float mx = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
     x = y = sum = 0.f;
 #pragma unroll
@@ -728,6 +721,23 @@ __global__ __launch_bounds__(256) void attn_i8_merge_kernel(AttnI8Args a, int64_
     }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     reinterpret_cast<v2h *>(a.o + row * kI8D)[lane] = (v2h){(f16)(x * inv), (f16)(y * inv)};
+}
+
+constexpr int64_t kMergeBlocks = 1 << 20;
+
+__global__ __launch_bounds__(256) void attn_i8_merge_kernel(AttnI8Args a, int64_t batch) {
+    __shared__ float sx[4][kI8D], sm[4], ss[4];
+    int64_t lo = 0, hi = a.rows;   // rows of the requests
+    if (a.q_indptr) {
+        lo = a.q_indptr[0];
+        lo = lo < 0 ? 0 : lo;
+        hi = a.q_indptr[batch];
+        hi = hi > a.rows ? a.rows : hi;
+    }
+    for (int64_t row = lo * a.hq + blockIdx.x; row < hi * a.hq; row += gridDim.x) {
+        merge_row(a, row, sx, sm, ss);
+        __syncthreads();   // before the next row's parts
+    }
 }
 
 // Kernel, row tiles and chunks of a request, from the sizes alone.  us on one
@@ -751,9 +761,11 @@ struct Plan {
     int form, tiles, chunks;
 };
 
-Plan plan_of(int64_t batch, int64_t group, int64_t H, int64_t max_q, int64_t max_kv) {
+Plan plan_of(int64_t n_rows, int64_t batch, int64_t group, int64_t H, int64_t max_q,
+             int64_t max_kv) {
     constexpr int64_t kCUs = 256;
-    const int64_t rows = (max_q < 1 ? 1 : max_q) * group;
+    // (the largest request has at least the mean, whatever the caller says)
+    const int64_t rows = std::max(max_q, srq_cdiv(n_rows, batch)) * group;
     Plan pl;
     pl.form = rows <= 16 ? kRows16
               : batch * H * srq_cdiv(rows, kRowsBlock) >= kCUs ? kRows128 : kRows32;
@@ -783,7 +795,8 @@ extern "C" int srq_batch_attention_i8_workspace(int64_t rows, int64_t batch, int
                   (long long)n_kv_heads);
     *bytes = 0;
     if (rows == 0 || batch == 0) return SRQ_OK;
-    const Plan pl = plan_of(batch, n_q_heads / n_kv_heads, n_kv_heads, max_q_len, max_kv_len);
+    const Plan pl =
+        plan_of(rows, batch, n_q_heads / n_kv_heads, n_kv_heads, max_q_len, max_kv_len);
     if (pl.chunks > 1) *bytes = rows * n_q_heads * pl.chunks * kRec * 4;
     return SRQ_OK;
 }
@@ -807,13 +820,14 @@ extern "C" int srq_batch_attention_i8(
                   "batch_attention_i8: %lld rows for %lld requests", (long long)rows,
                   (long long)batch);
     SRQ_CHECK_ARG(rows <= 0x7fffffff / n_q_heads, "batch_attention_i8: rows x heads >= 2^31");
-    SRQ_CHECK_ARG(__builtin_isfinite(sm_scale), "batch_attention_i8: sm_scale is not finite");
+    SRQ_CHECK_ARG(__builtin_isfinite(sm_scale * 1.4426950408889634f),
+                  "batch_attention_i8: sm_scale is not finite in base 2");
     if (batch == 0 || rows == 0) return SRQ_OK;
     SRQ_CHECK_ARG(o && q, "batch_attention_i8: null pointer");
     SRQ_CHECK_ARG(srq_aligned(o, 16) && srq_aligned(q, 16),
                   "batch_attention_i8: o and q must be 16-byte aligned");
     const int64_t group = n_q_heads / num_kv_heads;
-    const Plan pl = plan_of(batch, group, num_kv_heads, max_q_len, max_kv_len);
+    const Plan pl = plan_of(rows, batch, group, num_kv_heads, max_q_len, max_kv_len);
     int64_t need = 0;
     if (pl.chunks > 1) need = rows * n_q_heads * pl.chunks * kRec * 4;
     SRQ_CHECK_ARG(need == 0 || (ws && ws_bytes >= need && srq_aligned(ws, 16)),
@@ -840,7 +854,8 @@ extern "C" int srq_batch_attention_i8(
     default: attn_i8_rows_kernel<<<grid, kWaves * 64, 0, st>>>(a, p); break;
     }
     if (pl.chunks > 1)
-        attn_i8_merge_kernel<<<(unsigned)(rows * n_q_heads), 256, 0, st>>>(a, batch);
+        attn_i8_merge_kernel<<<(unsigned)std::min(rows * n_q_heads, kMergeBlocks), 256, 0, st>>>(
+            a, batch);
     SRQ_LAUNCH_CHECK("batch_attention_i8");
     return SRQ_OK;
 }

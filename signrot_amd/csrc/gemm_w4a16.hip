@@ -308,7 +308,7 @@ extern "C" int srq_w4a16_linear(const void *x, const void *w, const void *scales
     SRQ_CHECK_ARG(group > 0 && group % 32 == 0 && K % group == 0,
                   "w4a16_linear: group=%lld must be a multiple of 32 that divides K=%lld",
                   (long long)group, (long long)K);
-    SRQ_CHECK_ARG(K <= 1 << 24 && N <= 1 << 28 && M <= 16 * 65535,
+    SRQ_CHECK_ARG(K <= 1 << 24 && N <= 1 << 26 && M <= 16 * 65535,
                   "w4a16_linear: shape out of range");
     if (M == 0 || N == 0) return SRQ_OK;
     SRQ_CHECK_ARG(out && (K == 0 || (x && w && scales)), "w4a16_linear: null pointer");

@@ -18,6 +18,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -455,7 +456,8 @@ PyObject *qk_norm_rope(PyObject *, PyObject *const *a, Py_ssize_t n_args) {
             throw Bad();
         const int64_t B = q.size(0), T = q.size(1), Hq = q.size(2), Hk = k.size(2), D = q.size(3);
         if (q.numel() == 0 || k.numel() == 0 || k.size(0) != B || k.size(1) != T ||
-            k.size(3) != D || c.size(1) != T || c.size(2) != D || (c.size(0) != 1 && c.size(0) != B))
+            k.size(3) != D || c.size(1) != T || c.size(2) != D ||
+            (c.size(0) != 1 && c.size(0) != B))
             throw Bad();
         const at::Tensor &s = plain(a[3], kF16);
         if (s.sizes() != c.sizes() || s.device() != dev) throw Bad();
@@ -471,6 +473,7 @@ PyObject *qk_norm_rope(PyObject *, PyObject *const *a, Py_ssize_t n_args) {
         int rc;
         {
             NoGil nogil;
+            const c10::DeviceGuard on(dev);
             qo = alloc({B, T, Hq, D}, kF16, dev);
             ko = alloc({B, T, Hk, D}, kF16, dev);
             rc = srq_qk_norm_rope(q.data_ptr(), k.data_ptr(), c.data_ptr(), s.data_ptr(), c.size(0),
@@ -537,6 +540,7 @@ PyObject *append_kv_i8(PyObject *, PyObject *const *a, Py_ssize_t n_args) {
         int rc;
         {
             NoGil nogil;
+            const c10::DeviceGuard on(c.dev);
             rc = srq_append_kv_i8(CACHE_ARGS(c), k.data_ptr(), v.data_ptr(), kt, vt, k.size(0), idx,
                                   hint, stream_of(c.dev));
         }
@@ -569,6 +573,7 @@ PyObject *qkv_norm_rope_append_i8(PyObject *, PyObject *const *a, Py_ssize_t n_a
         int rc;
         {
             NoGil nogil;
+            const c10::DeviceGuard on(c.dev);
             q = alloc({rows, hq, 128}, kF16, c.dev);
             rc = srq_qkv_norm_rope_append_i8(CACHE_ARGS(c), x.data_ptr(),
                                              rows > 1 ? x.stride(0) : x.size(1), rows,
@@ -603,6 +608,7 @@ PyObject *batch_attention_i8(PyObject *, PyObject *const *a, Py_ssize_t n_args) 
         int rc;
         {
             NoGil nogil;
+            const c10::DeviceGuard on(c.dev);
             at::Tensor ws;
             if (wb > 0) ws = alloc({wb}, kU8, c.dev);
             rc = srq_batch_attention_i8(o.data_ptr(), q.data_ptr(), rows, hq, CACHE_ARGS(c), idx,
@@ -630,6 +636,7 @@ PyObject *w4a16_linear(PyObject *, PyObject *const *a, Py_ssize_t n_args) {
         int rc;
         {
             NoGil nogil;
+            const c10::DeviceGuard on(dev);
             out = alloc(with_last(x, N), kF16, dev);
             rc = srq_w4a16_linear(x.data_ptr(), w.data_ptr(), s.data_ptr(), z, bias, M, N, K,
                                   K / groups, out.data_ptr(), stream_of(dev));

@@ -83,8 +83,9 @@ static inline int i8_check(const char *name, const void *data, const void *scale
                   name);
     if (batch == 0) return SRQ_OK;
     SRQ_CHECK_ARG(pages > 0, "%s: the cache holds no pages", name);
-    SRQ_CHECK_ARG(n_indices <= (int64_t)0x7fffffff / page, "%s: table x page_size >= 2^31 tokens",
-                  name);
+    // (a tile of keys past the longest request still counts in 32 bits)
+    SRQ_CHECK_ARG(n_indices <= (int64_t)(0x7fffffff - 64) / page,
+                  "%s: table x page_size >= 2^31 tokens", name);
     SRQ_CHECK_ARG(data && scale && indptr && last && (indices || n_indices == 0),
                   "%s: null pointer", name);
     SRQ_CHECK_ARG(srq_aligned(data, 16) && srq_aligned(scale, 4),

@@ -71,7 +71,8 @@ extern "C" int srq_qk_norm_rope(const void *q, const void *k, const void *cos, c
                       (n_kv_heads == 0 || (k && k_out)),
                   "qk_norm_rope: null pointer");
     SRQ_CHECK_ARG(n_q_heads + n_kv_heads <= 65536, "qk_norm_rope: too many heads");
-    SRQ_CHECK_ARG(batch <= 0x7fffffff / seq_len, "qk_norm_rope: batch x seq_len >= 2^31");
+    // a block of 256 threads per token, and fewer than 2^32 threads a launch
+    SRQ_CHECK_ARG(batch <= 0xffffff / seq_len, "qk_norm_rope: batch x seq_len >= 2^24");
     SRQ_CHECK_ARG(q_tok_stride >= n_q_heads * head_dim && k_tok_stride >= n_kv_heads * head_dim &&
                       q_seq_stride >= 0 && k_seq_stride >= 0,
                   "qk_norm_rope: strides smaller than the [H, D] extent");

@@ -221,6 +221,24 @@ class MultiLayerPagedKVCache8Bit(Cache):
             self._table.set_uniform(self.length, self.page_size)
         return self._spec
 
+    def mark_prefilled(self, length: int):
+        """Declare that every layer holds `length` tokens per request, written into
+        `pages` / `scales` directly; the next update() of each layer appends."""
+        self._reserve(length)
+        self.length = length
+        self._filled = [True] * len(self._filled)
+
+    def clone(self):
+        """An independent copy: own pages, scales and index tensors, same state."""
+        c = object.__new__(type(self))
+        c.__dict__.update(self.__dict__)
+        c.pages, c.scales = self.pages.clone(), self.scales.clone()
+        c._filled = list(self._filled)
+        c._table = self._table.clone()
+        c._spec = {}
+        c._point_spec()
+        return c
+
     def reset(self):
         self.length = 0
         self._filled = [False] * len(self._filled)

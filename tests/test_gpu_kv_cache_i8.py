@@ -104,6 +104,23 @@ def test_update_qkv_is_norm_append_and_attend():
         pos += T
 
 
+def test_clone_and_mark_prefilled():
+    g = _gen(11)
+    a = MultiLayerPagedKVCache8Bit(2, 16, 64, DEV, 1, 2, D)
+    k, q = _rand(g, 2, 20, 2, D), _rand(g, 2, 1, 4, D)
+    a.update(k, k, 0)
+    b = a.clone()
+    c = MultiLayerPagedKVCache8Bit(2, 16, 64, DEV, 1, 2, D)
+    c.pages.copy_(a.pages)
+    c.scales.copy_(a.scales)
+    c.mark_prefilled(20)
+    before = a.pages.clone()
+    outs = [x.update(k[:, :1], k[:, 1:2], 0)(q) for x in (b, c)]
+    assert torch.equal(a.pages, before) and a.length == 20 and b.length == c.length == 21
+    assert torch.equal(outs[0], outs[1])
+    assert torch.equal(a.update(k[:, :1], k[:, 1:2], 0)(q), outs[0])
+
+
 def test_left_padded_prefill_then_decode():
     B, T, H, Hq, g = 3, 20, 2, 4, _gen(2)
     cache = MultiLayerPagedKVCache8Bit(B, 32, 40, DEV, 1, H, D)

@@ -278,6 +278,14 @@ def test_decode_lengths(Hq, H, page):
     assert (got[1] == 0).all()
 
 
+@pytest.mark.parametrize("Hq,H", [(64, 1), (130, 1), (66, 2)])
+def test_large_groups(Hq, H):
+    rng = np.random.default_rng(Hq)
+    c = Cache(rng, [1, 40, 0, 333], H, 16)
+    q = (2 * rng.standard_normal((4, Hq, D))).astype(np.float16)
+    _check(c, q)
+
+
 @pytest.mark.parametrize("kv", [1, 300, 5000, 10 ** 6])
 @pytest.mark.parametrize("lens", [[5000], [1, 3000], [2500, 0, 17]])
 def test_decode_split(lens, kv):

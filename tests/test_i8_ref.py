@@ -98,6 +98,7 @@ def test_attention_refusals(lib):
         return lib.srq_batch_attention_i8(o, q, rows, hq, *_cache(), idx, 1, kv,
                                           ctypes.c_float(scale), ws, n, None)
     for kw, msg in ((dict(hq=3), "query heads"), (dict(hq=0), "query heads"),
+                    (dict(scale=3e38), "finite"),
                     (dict(rows=3), "3 rows"), (dict(scale=float("nan")), "finite"),
                     (dict(o=None), "null"), (dict(q=ctypes.c_void_p(8)), "aligned"),
                     (dict(rows=1 << 30, idx=P), "2^31"), (dict(kv=10000, ws=None), "workspace"),
@@ -107,6 +108,9 @@ def test_attention_refusals(lib):
     n = ctypes.c_int64()
     assert lib.srq_batch_attention_i8_workspace(2, 2, 5, 2, 1, 100, ctypes.byref(n)) == -1
     assert lib.srq_batch_attention_i8_workspace(2, 2, 4, 2, 1, 100, None) == -1
+    # a hint of one token for a request of 100000 does not split all of its rows
+    assert lib.srq_batch_attention_i8_workspace(100000, 1, 32, 8, 1, 100000, ctypes.byref(n)) == 0
+    assert n.value == 0
 
 
 def test_norm_rope_refusals(lib):
@@ -117,7 +121,7 @@ def test_norm_rope_refusals(lib):
                     (dict(eps=float("inf")), "eps"), (dict(norm=0, w=P), "without"),
                     (dict(tok=256), "strides"), (dict(tok=516), "multiples"),
                     (dict(q=ctypes.c_void_p(8)), "aligned"), (dict(q=None), "null"),
-                    (dict(B=-1), "shape"), (dict(T=1 << 31), "2^31")):
+                    (dict(B=-1), "shape"), (dict(T=1 << 24), "2^24")):
         assert call(**kw) == -1, kw
         assert msg in lib.srq_last_error().decode(), kw
     assert call(T=0, q=None) == 0
@@ -128,7 +132,8 @@ def test_linear_refusals(lib):
         return lib.srq_w4a16_linear(x, w, P, None, None, M, N, K, group, out, None)
     for kw, msg in ((dict(group=48), "multiple of 32"), (dict(K=100), "divides"),
                     (dict(group=0), "multiple"), (dict(M=-1), "negative"), (dict(x=None), "null"),
-                    (dict(w=ctypes.c_void_p(8)), "aligned"), (dict(M=1 << 21), "range")):
+                    (dict(w=ctypes.c_void_p(8)), "aligned"), (dict(M=1 << 21), "range"),
+                    (dict(N=(1 << 26) + 1), "range")):
         assert call(**kw) == -1, kw
         assert msg in lib.srq_last_error().decode(), kw
     assert call(M=0, x=None) == 0 and call(N=0) == 0
