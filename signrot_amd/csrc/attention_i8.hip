@@ -514,7 +514,8 @@ __global__ __launch_bounds__(kWaves * 64, 2) void attn_i8_rows_kernel(AttnI8Args
             if (tid % (KR * kI8Block) == 0) {
                 const float v = vsc != 0.f ? vsc : 1.f;   // a block of zeros
                 BlockScale s;
-                s.kc = there ? ksc * a.c : 0.f;
+                // (a block of zeros: any factor, but -inf * 0 would not be -inf)
+                s.kc = there ? (ksc != 0.f ? ksc : 0x1p-100f) * a.c : 0.f;
                 s.lv = there ? __builtin_amdgcn_logf(v) : -INFINITY;
                 s.rv = there ? 1.f / v : 0.f;
                 s.pad = 0.f;

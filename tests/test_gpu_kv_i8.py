@@ -350,6 +350,21 @@ def test_scales_far_apart_and_zero():
         _close(got[b], want[b], size[b], 96)
 
 
+@pytest.mark.parametrize("new", [[257, 130, 65, 20], [9, 40, 33, 1]])
+def test_blocks_of_zero_keys(new):
+    """Key blocks that hold only zeros (scale 0), among them those that a causal row
+    sees in part: their scores are 0, and what is behind the row stays out."""
+    rng = np.random.default_rng(sum(new))
+    held = [0, 5, 30, 63]
+    c = Cache(rng, [h + n for h, n in zip(held, new)], 8, 16)
+    for pg in c.indices[::2]:
+        c.scale[pg, 1, 0] = 0
+        c.data[pg, 1, 0] = 0
+    c.upload()
+    q = (2 * rng.standard_normal((sum(new), 32, D))).astype(np.float16)
+    _check(c, q, _starts(new), max(new))
+
+
 def test_what_no_row_sees_does_not_matter():
     """Garbage codes behind the last token, NaN scales of blocks behind it, of
     other heads' V and of unused pages; then a poisoned block that only the later
