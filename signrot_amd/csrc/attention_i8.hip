@@ -420,6 +420,7 @@ struct BlockScale {
 __global__ __launch_bounds__(kWaves * 64, 2) void attn_i8_rows_kernel(AttnI8Args a, PagedI8 p) {
     constexpr int NT = kWaves * 64, RB = kRowsBlock;
     constexpr int KR = NT / KT, KB = kI8D / KR;     // threads per key row, bytes of each
+    static_assert(KR * kI8Block == 64, "a wave stages a block of keys");
     __shared__ __align__(16) f16 Ks_[2][KT * KS];
     __shared__ __align__(16) f16 Vs_[2][KT * VR];
     __shared__ BlockScale Bs_[2][KT / kI8Block];
@@ -456,41 +457,53 @@ __global__ __launch_bounds__(kWaves * 64, 2) void attn_i8_rows_kernel(AttnI8Args
         const int t_lo = min(chunk * per, ntile), t_hi = min(ntile, t_lo + per);
 
         v8h qf[kI8D / 16];
+        float qs = 0.f;
         {
             const f16 *src = a.q + (ok ? orow : 0) * kI8D + 8 * g;
 #pragma unroll
             for (int kk = 0; kk < kI8D / 16; ++kk) {
                 const v8h x = *reinterpret_cast<const v8h *>(src + 16 * kk);
                 qf[kk] = ok ? x * (f16)a.qmul : (v8h)(f16)0;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) qs += (float)qf[kk][e];
             }
+            qs += __shfl_xor(qs, 32);
+            qs *= -0x1p-17f;   // -128 sum(q) 2^-24, what K's codes + 128 add to a score
         }
         v16f o[kI8D / 32];
 #pragma unroll
         for (int i = 0; i < kI8D / 32; ++i) o[i] = (v16f)0.f;
         float m = -INFINITY, l = 0.f;
 
-        // staging: thread -> key row tid / KR, KB bytes of its K and V codes
+        // staging: wave w -> the tile's w-th block of 16 keys, KB bytes of a row's K
+        // and V codes a lane; the block's place is the same for the whole wave, so
+        // its arithmetic is scalar
         const int kr = tid / KR, kd = (tid % KR) * KB;
+        const int64_t v_part = (int64_t)p.H * p.page * kI8D;
+        const uint32_t in_block = (kr & (kI8Block - 1)) * kI8D + kd;
         v4i kx[KB / 16], vx[KB / 16];
         float ksc = 0.f, vsc = 0.f;
         bool there = false;
-        int64_t page_next;
+        int page_next = -1;                          // in every lane
+        int slot = (uint32_t)(t_lo * (KT / kI8Block) + wave) / (uint32_t)p.bpp;
+        int in_page = t_lo * (KT / kI8Block) + wave - slot * p.bpp, in_next = 0;
+        // the page of the wave's block of tile t, looked up in order of t
         auto find = [&](int t) __attribute__((always_inline)) {
-            // the block's scale index, or -1; for the row that this thread loads
-            const int key = t * KT + kr;
-            int64_t si = -1;
-            if (t < t_hi && key < hi) {
-                const uint32_t blk = (uint32_t)key / kI8Block;
-                const int64_t pg = i8_page(p, rq.first, blk);
-                if (pg >= 0) si = i8_scale_index(p, pg, hk, blk % (uint32_t)p.bpp);
+            const bool in = t < t_hi && (t * (KT / kI8Block) + wave) * kI8Block < hi;
+            page_next = in ? p.indices[rq.first + slot] : -1;
+            in_next = in_page;
+            in_page += KT / kI8Block;
+            while (in_page >= p.bpp) {
+                in_page -= p.bpp;
+                ++slot;
             }
-            return si;
         };
-        auto load_tile = [&](int64_t si, int t) __attribute__((always_inline)) {
-            there = si >= 0;
-            const int64_t at = there ? si : 0;
-            const int8_t *kb = p.data + (at * kI8Block + (kr & (kI8Block - 1))) * kI8D + kd;
-            const int8_t *vb = kb + (int64_t)p.H * p.page * kI8D;
+        auto load_tile = [&]() __attribute__((always_inline)) {
+            const int64_t pg = __builtin_amdgcn_readfirstlane(page_next);
+            there = pg >= 0 && pg < p.pages;
+            const int64_t at = there ? i8_scale_index(p, pg, hk, in_next) : 0;
+            const int8_t *kb = p.data + at * (kI8Block * kI8D) + in_block;
+            const int8_t *vb = kb + v_part;
 #pragma unroll
             for (int i = 0; i < KB / 16; ++i) {
                 kx[i] = *reinterpret_cast<const v4i *>(kb + 16 * i);
@@ -506,26 +519,27 @@ __global__ __launch_bounds__(kWaves * 64, 2) void attn_i8_rows_kernel(AttnI8Args
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     *reinterpret_cast<v8h *>(kd_ + 16 * i + 8 * h) =
-                        signed8((u32)kx[i][2 * h], (u32)kx[i][2 * h + 1]);
+                        codes8((u32)kx[i][2 * h], (u32)kx[i][2 * h + 1]);
                     *reinterpret_cast<v8h *>(vd_ + 16 * i + 8 * h) =
                         signed8((u32)vx[i][2 * h], (u32)vx[i][2 * h + 1]);
                 }
             }
-            if (tid % (KR * kI8Block) == 0) {
+            if (lane == 0) {
                 const float v = vsc != 0.f ? vsc : 1.f;   // a block of zeros
                 BlockScale s;
                 // (a block of zeros: any factor, but -inf * 0 would not be -inf)
-                s.kc = there ? (ksc != 0.f ? ksc : 0x1p-100f) * a.c : 0.f;
+                s.kc = there ? (ksc != 0.f ? ksc : 0x1p-100f) * a.c * 0x1p24f : 0.f;
                 s.lv = there ? __builtin_amdgcn_logf(v) : -INFINITY;
                 s.rv = there ? 1.f / v : 0.f;
                 s.pad = 0.f;
-                Bs_[buf][tid / (KR * kI8Block)] = s;
+                Bs_[buf][wave] = s;
             }
         };
 
         if (t_lo < t_hi) {
-            load_tile(find(t_lo), t_lo);
-            page_next = find(t_lo + 1);
+            find(t_lo);
+            load_tile();
+            find(t_lo + 1);
             store_tile(t_lo & 1);
         }
         __syncthreads();
@@ -534,8 +548,8 @@ __global__ __launch_bounds__(kWaves * 64, 2) void attn_i8_rows_kernel(AttnI8Args
             const f16 *Ks = Ks_[buf];
             const f16 *Vs = Vs_[buf];
             if (t + 1 < t_hi) {
-                load_tile(page_next, t + 1);    // in flight during this tile's products
-                page_next = find(t + 2);
+                load_tile();    // in flight during this tile's products
+                find(t + 2);
             }
             [&]() __attribute__((always_inline)) {
                 if (k0 >= wave_hi) return;      // no key of this tile is visible
@@ -586,7 +600,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void attn_i8_rows_kernel(AttnI8Args
                     float mb = -INFINITY;
 #pragma unroll
                     for (int v = 0; v < 8; ++v) mb = fmaxf(mb, s[i / 2][8 * (i % 2) + v]);
-                    mt = fmaxf(mt, __builtin_fmaf(mb, bs[i].kc, bs[i].lv));
+                    mt = fmaxf(mt, __builtin_fmaf(mb + qs, bs[i].kc, bs[i].lv));
                 }
                 mt = fmaxf(mt, __shfl_xor(mt, 32));
                 const bool grow = mt > m + kSlack;
@@ -601,7 +615,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void attn_i8_rows_kernel(AttnI8Args
                 v8h pb[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float add = bs[i].lv - sub, kc = bs[i].kc;
+                    const float kc = bs[i].kc, add = __builtin_fmaf(qs, kc, bs[i].lv - sub);
                     float ps0 = 0.f, ps1 = 0.f;
 #pragma unroll
                     for (int v = 0; v < 8; ++v) {
@@ -750,8 +764,8 @@ __global__ __launch_bounds__(256) void attn_i8_merge_kernel(AttnI8Args a, int64_
 //    22.3 / 15.3 / 12.7, 1 x 60000 in 16 / 24 / 32 / 48 / 64 chunks 41 / 34 / 37 / 45 /
 //    45; 32 x 4096 (256 blocks) unsplit 45.2, in two 45.9.
 //  * Where blocks of 128 rows fill the CUs, attn_i8_rows_kernel: 4 x (5000 + 512),
-//    32 / 8 heads, 186 against 267 for the next form; 1 x 2048 new 85 against 102; at
-//    256 blocks, 2 x (1000 + 256) of 64 / 8 heads, 43.1 against 44.8.
+//    32 / 8 heads, 182 against 267 for the next form; 1 x 2048 new 79 against 102; at
+//    256 blocks, 2 x (1000 + 256) of 64 / 8 heads, 37.5 against 44.8.
 //  * Otherwise attn_i8_kernel<2>, four times as many blocks: 1 x (5000 + 512) 90
 //    against 158 (94 with the 128-row form in 4 chunks), 2 x (2000 + 128) of 64 / 8
 //    heads 34 against 65; split below 256 blocks until there are 512: 4 x (8000 + 8)
