@@ -744,10 +744,10 @@ int srq_qkv_norm_rope_append_i8(
  * q_indptr[b] .. q_indptr[b + 1] of q f16 [rows, n_q_heads, 128] are its last n
  * tokens (row b, its last one, when q_indptr is NULL and rows = B); token i of
  * them sees the first len - n + i + 1 cached tokens.  Grouped-query
- * (n_q_heads a multiple of H); logits q . k * sm_scale (finite).  o like q; a
- * row that sees nothing is 0, a row of no request stays as it is.  max_q_len and
- * max_kv_len size the launch and the workspace of ..._workspace (any value is
- * correct). */
+ * (n_q_heads a multiple of H); logits q . k * sm_scale (0, or 2^-20 to 2^60 in
+ * magnitude).  o like q; a row that sees nothing is 0, a row of no request stays
+ * as it is.  max_q_len and max_kv_len size the launch and the workspace of
+ * ..._workspace (any value is correct). */
 int srq_batch_attention_i8(
     void *o, const void *q, int64_t rows, int64_t n_q_heads, const void *kv_data,
     const void *kv_scale, const int32_t *kv_indptr, const int32_t *kv_indices,

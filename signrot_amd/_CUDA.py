@@ -1124,7 +1124,7 @@ def batch_attention_i8(o, q, kv_data, kv_scale, kv_indptr, kv_indices, last_page
     token is 0; rows of no request are left as they are.  max_q_len (largest number
     of rows of a request) and max_kv_len (longest request; the whole table when
     None) size the launch and the workspace, any value gives a correct result;
-    softmax_scale defaults to 1 / sqrt(128)."""
+    softmax_scale (0, or 2^-20 to 2^60 in magnitude) defaults to 1 / sqrt(128)."""
     if _host.batch_attention_i8(o, q, kv_data, kv_scale, kv_indptr, kv_indices, last_page_offset,
                                 layer_idx, q_indptr, max_q_len, max_kv_len, softmax_scale):
         return o

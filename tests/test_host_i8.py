@@ -4,7 +4,7 @@ import pytest
 import torch
 from transformers.cache_utils import Cache
 
-from signrot_amd import nn
+from signrot_amd import _native, nn
 from signrot_amd.functional.quantization import rtn_group_pack, unpack_i4, unpack_ui4
 from signrot_amd.transformers import MultiLayerPagedKVCache8Bit
 
@@ -47,3 +47,12 @@ def test_group_linear_on_the_host():
     for args in ((64, 8, 24), (64, 8, 128), (96, 8, 64), (64, 8, 0)):
         with pytest.raises(ValueError):
             nn.GroupLinear4bit(*args)
+
+
+@pytest.mark.parametrize("sm", [float("nan"), float("inf"), -3e38, 1e20, 1e-7, -1e-40])
+def test_softmax_scales_that_leave_the_range_are_refused(sm):
+    """The entry point's own check, before any launch: the pointers are only
+    aligned numbers here."""
+    rc = _native.lib().srq_batch_attention_i8(
+        64, 64, 1, 1, 64, 64, 64, 64, 64, 1, 1, 1, 1, 0, 1, 16, 128, None, 1, 16, sm, None, 0, None)
+    assert rc != 0 and b"sm_scale" in _native.lib().srq_last_error()
