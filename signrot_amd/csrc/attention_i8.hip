@@ -91,6 +91,12 @@ SRQ_DEV void pair_dims(u32 a, u32 b, v2h (&d)[4]) {
     d[3] = unbias(__builtin_amdgcn_perm(k, hi, 0x04030402u));
 }
 
+// log2 and inverse of a V scale.  A block of zeros (scale 0) adds to l alone: it
+// counts as one of scale 2^-60, under the least that fp16 values have (2^-31), so
+// that m follows the blocks that do add values and p' keeps its bits for them.
+SRQ_DEV float log_scale(float v) { return v != 0.f ? __builtin_amdgcn_logf(v) : -60.f; }
+SRQ_DEV float inv_scale(float v) { return v != 0.f ? 1.f / v : 0x1p60f; }
+
 struct Tile {
     v4i k[2][2];   // [block][half of the dims]
     uint2 v[8];    // tokens of the lane's slots
@@ -302,8 +308,8 @@ __global__ __launch_bounds__(kWaves * 64, 2) void attn_i8_kernel(AttnI8Args a, P
             __builtin_amdgcn_sched_barrier(0);   // K first: its wait leaves V in flight
             load_v(x, 0);
             __builtin_amdgcn_sched_barrier(0);
-            lv = vs != 0.f ? __builtin_amdgcn_logf(vs) : 0.f;
-            rv = vs != 0.f ? 1.f / vs : 1.f;
+            lv = log_scale(vs);
+            rv = inv_scale(vs);
             ks *= a.c * 0x1p24f;
             // (the last tiles apart: with their loads under a condition every wait
             // would be for all that are in flight)
@@ -463,7 +469,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void attn_i8_rows_kernel(AttnI8Args
 #pragma unroll
             for (int kk = 0; kk < kI8D / 16; ++kk) {
                 const v8h x = *reinterpret_cast<const v8h *>(src + 16 * kk);
-                qf[kk] = ok ? x * (f16)a.qmul : (v8h)(f16)0;
+                qf[kk] = lim > 0 ? x * (f16)a.qmul : (v8h)(f16)0;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) qs += (float)qf[kk][e];
             }
@@ -525,12 +531,11 @@ __global__ __launch_bounds__(kWaves * 64, 2) void attn_i8_rows_kernel(AttnI8Args
                 }
             }
             if (lane == 0) {
-                const float v = vsc != 0.f ? vsc : 1.f;   // a block of zeros
                 BlockScale s;
                 // (a block of zeros: any factor, but -inf * 0 would not be -inf)
                 s.kc = there ? (ksc != 0.f ? ksc : 0x1p-100f) * a.c * 0x1p24f : 0.f;
-                s.lv = there ? __builtin_amdgcn_logf(v) : -INFINITY;
-                s.rv = there ? 1.f / v : 0.f;
+                s.lv = there ? log_scale(vsc) : -INFINITY;
+                s.rv = there ? inv_scale(vsc) : 0.f;
                 s.pad = 0.f;
                 Bs_[buf][wave] = s;
             }

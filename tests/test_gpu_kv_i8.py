@@ -365,6 +365,45 @@ def test_blocks_of_zero_keys(new):
     _check(c, q, _starts(new), max(new))
 
 
+@pytest.mark.parametrize("new", [None, [9, 40, 33, 1], [257, 130, 65, 20]])
+def test_small_values_beside_a_block_of_zeros(new):
+    """A block whose values are all 0 (scale 0) takes most of the weight; what the
+    others, of scale 2^-15, add keeps its precision."""
+    rng = np.random.default_rng(36)
+    count = [1] * 4 if new is None else new
+    c = Cache(rng, [64 + n for n in count], 8, 16)
+    q = rng.standard_normal(D).astype(np.float16)
+    c.scale[:, 1, 0] = 1e-4
+    c.scale[:, 1, 1] = 2.0 ** -15
+    for pg in c.indices[c.indptr[:-1]]:          # the first block of each request
+        c.scale[pg, 1, 1] = 0
+        c.data[pg, 1, 1] = 0
+        c.data[pg, 1, 0] = 100 * np.sign(q).astype(np.int8)
+        c.scale[pg, 1, 0] = 4 * D ** 0.5 / (100 * np.abs(q.astype(np.float64)).sum())
+    c.upload()
+    q = np.broadcast_to(q, (sum(count), 32, D)).copy()
+    if new is None:
+        _check(c, q)
+    else:
+        _check(c, q, _starts(new), max(new))
+
+
+@pytest.mark.parametrize("new,room", [([9, 20, 33, 1], [3, 12, 40, 0]),
+                                      ([300, 130, 65, 20], [40, 150, 10, 0])])
+def test_rows_that_see_nothing_may_hold_anything(new, room):
+    """More queries than tokens: the first rows of a request see none.  They are 0
+    whatever they hold, and the rows beside them are as without it."""
+    rng = np.random.default_rng(37)
+    c = Cache(rng, room, 8, 16)
+    q = rng.standard_normal((sum(new), 32, D)).astype(np.float16)
+    idx = _starts(new)
+    want = _check(c, q, idx, max(new))
+    for b, (n, r) in enumerate(zip(new, room)):
+        q[idx[b]: idx[b] + max(0, n - r)] = [np.nan, np.inf, 3e4, -np.inf][b]
+    got = _attend(c, q, idx, max(new))
+    assert np.array_equal(got, want)
+
+
 def test_what_no_row_sees_does_not_matter():
     """Garbage codes behind the last token, NaN scales of blocks behind it, of
     other heads' V and of unused pages; then a poisoned block that only the later
