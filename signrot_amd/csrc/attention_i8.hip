@@ -435,14 +435,13 @@ __global__ __launch_bounds__(kWaves * 64, 2) void attn_i8_rows_kernel(AttnI8Args
     const int g = lane >> 5, ln = lane & 31;
     const int hk = blockIdx.y;
     const int64_t b = blockIdx.z;
-    const int chunk = blockIdx.x % a.chunks;
     int64_t s0, n;
     i8_new_rows(a.q_indptr, b, a.rows, s0, n);
     const I8Request rq = i8_request(p, b);
     const int64_t nrows = n * a.group;
     const int64_t rtiles = (nrows + RB - 1) / RB;
     // the last rows see most keys: their tiles come first
-    for (int64_t rt = rtiles - 1 - (int64_t)(blockIdx.x / a.chunks); rt >= 0; rt -= a.tiles) {
+    for (int64_t rt = rtiles - 1 - (int64_t)blockIdx.x; rt >= 0; rt -= a.tiles) {
         const int64_t r0 = rt * RB, r = r0 + 32 * wave + ln;
         const bool ok = r < nrows;
         const int64_t qi = ok ? (uint32_t)r / (uint32_t)a.group : 0;
@@ -459,8 +458,6 @@ __global__ __launch_bounds__(kWaves * 64, 2) void attn_i8_rows_kernel(AttnI8Args
         const int lo = lo64 > 0 ? (int)lo64 : 0, hi = hi64 > 0 ? (int)hi64 : 0;
         const int wave_hi = r0 + 32 * wave < nrows && wh64 > 0 ? (int)wh64 : 0;
         const int ntile = (hi + KT - 1) / KT;
-        const int per = (ntile + a.chunks - 1) / a.chunks;
-        const int t_lo = min(chunk * per, ntile), t_hi = min(ntile, t_lo + per);
 
         v8h qf[kI8D / 16];
         float qs = 0.f;
@@ -491,11 +488,10 @@ __global__ __launch_bounds__(kWaves * 64, 2) void attn_i8_rows_kernel(AttnI8Args
         float ksc = 0.f, vsc = 0.f;
         bool there = false;
         int page_next = -1;                          // in every lane
-        int slot = (uint32_t)(t_lo * (KT / kI8Block) + wave) / (uint32_t)p.bpp;
-        int in_page = t_lo * (KT / kI8Block) + wave - slot * p.bpp, in_next = 0;
+        int slot = wave / p.bpp, in_page = wave - slot * p.bpp, in_next = 0;
         // the page of the wave's block of tile t, looked up in order of t
         auto find = [&](int t) __attribute__((always_inline)) {
-            const bool in = t < t_hi && (t * (KT / kI8Block) + wave) * kI8Block < hi;
+            const bool in = t < ntile && (t * (KT / kI8Block) + wave) * kI8Block < hi;
             page_next = in ? p.indices[rq.first + slot] : -1;
             in_next = in_page;
             in_page += KT / kI8Block;
@@ -541,18 +537,18 @@ __global__ __launch_bounds__(kWaves * 64, 2) void attn_i8_rows_kernel(AttnI8Args
             }
         };
 
-        if (t_lo < t_hi) {
-            find(t_lo);
+        if (ntile > 0) {
+            find(0);
             load_tile();
-            find(t_lo + 1);
-            store_tile(t_lo & 1);
+            find(1);
+            store_tile(0);
         }
         __syncthreads();
-        for (int t = t_lo; t < t_hi; ++t) {
+        for (int t = 0; t < ntile; ++t) {
             const int k0 = t * KT, buf = t & 1;
             const f16 *Ks = Ks_[buf];
             const f16 *Vs = Vs_[buf];
-            if (t + 1 < t_hi) {
+            if (t + 1 < ntile) {
                 load_tile();    // in flight during this tile's products
                 find(t + 2);
             }
@@ -647,11 +643,11 @@ __global__ __launch_bounds__(kWaves * 64, 2) void attn_i8_rows_kernel(AttnI8Args
                         o[db] = mfma32(av, pb[st], o[db]);
                     }
             }();
-            if (t + 1 < t_hi) store_tile(buf ^ 1);
+            if (t + 1 < ntile) store_tile(buf ^ 1);
             __syncthreads();
         }
         l += __shfl_xor(l, 32);
-        if (ok && a.chunks == 1) {
+        if (ok) {
             const float inv = l == 0.f ? 0.f : 1.f / l;
             f16 *to = a.o + orow * kI8D;
 #pragma unroll
@@ -663,19 +659,6 @@ __global__ __launch_bounds__(kWaves * 64, 2) void attn_i8_rows_kernel(AttnI8Args
                     for (int i = 0; i < 4; ++i) x[i] = (f16)(o[db][4 * grp + i] * inv);
                     *reinterpret_cast<v4h *>(to + 32 * db + 8 * grp + 4 * g) = x;
                 }
-        } else if (ok) {
-            float *rec = a.tmp + (orow * a.chunks + chunk) * kRec;
-#pragma unroll
-            for (int db = 0; db < kI8D / 32; ++db)
-#pragma unroll
-                for (int grp = 0; grp < 4; ++grp)
-                    *reinterpret_cast<v4f *>(rec + 32 * db + 8 * grp + 4 * g) =
-                        (v4f){o[db][4 * grp], o[db][4 * grp + 1], o[db][4 * grp + 2],
-                              o[db][4 * grp + 3]};
-            if (g == 0) {
-                rec[kI8D] = m;
-                rec[kI8D + 1] = l;
-            }
         }
     }
 }
@@ -768,7 +751,7 @@ __global__ __launch_bounds__(256) void attn_i8_merge_kernel(AttnI8Args a, int64_
 //    over 8 heads in 1 / 2 / 4 / 8 chunks 19.8 / 15.9 / 13.9 / 15.1, 1 x 4096 33.8 /
 //    22.3 / 15.3 / 12.7, 1 x 60000 in 16 / 24 / 32 / 48 / 64 chunks 41 / 34 / 37 / 45 /
 //    45; 32 x 4096 (256 blocks) unsplit 45.2, in two 45.9.
-//  * Where blocks of 128 rows fill the CUs, attn_i8_rows_kernel: 4 x (5000 + 512),
+//  * Where blocks of 128 rows fill the CUs, attn_i8_rows_kernel, unsplit: 4 x (5000 + 512),
 //    32 / 8 heads, 182 against 267 for the next form; 1 x 2048 new 79 against 102; at
 //    256 blocks, 2 x (1000 + 256) of 64 / 8 heads, 37.5 against 44.8.
 //  * Otherwise attn_i8_kernel<2>, four times as many blocks: 1 x (5000 + 512) 90
