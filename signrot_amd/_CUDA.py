@@ -1046,7 +1046,8 @@ def append_kv_i8(kv_data, kv_scale, kv_indptr, kv_indices, last_page_offset, lay
     larger of its scale and the new one, its codes requantized where it grew; a
     non-finite value makes its block read as NaN.  k and v may be column slices
     (dense rows [H, 128]).  max_new: the largest number of new tokens, which sizes
-    the launch."""
+    the launch.  Requests may share pages, but not the block that one of them
+    appends to."""
     if _host.append_kv_i8(kv_data, kv_scale, kv_indptr, kv_indices, last_page_offset, layer_idx,
                           k, v, new_indptr, max_new):
         return

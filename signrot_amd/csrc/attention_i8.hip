@@ -759,6 +759,7 @@ __global__ __launch_bounds__(256) void attn_i8_merge_kernel(AttnI8Args a, int64_
 //    heads 34 against 65; split below 256 blocks until there are 512: 4 x (8000 + 8)
 //    in 2 / 4 / 8 / 16 chunks 55 / 35 / 28 / 37, 8 x (3000 + 8) 31 / 28.5 / 34 in 2 / 4 / 8
 //    (256 blocks, 2 x (1000 + 128) over 32 heads: unsplit 20.4, in two 28.6).
+constexpr int64_t kMaxBlocks = 1 << 18;
 enum { kRows16, kRows32, kRows128 };
 struct Plan {
     int form, tiles, chunks;
@@ -767,13 +768,16 @@ struct Plan {
 Plan plan_of(int64_t n_rows, int64_t batch, int64_t group, int64_t H, int64_t max_q,
              int64_t max_kv) {
     constexpr int64_t kCUs = 256;
-    // (the largest request has at least the mean, whatever the caller says)
-    const int64_t rows = std::max(max_q, srq_cdiv(n_rows, batch)) * group;
+    // (the largest request has at least the mean and at most all, whatever the
+    // caller says)
+    const int64_t rows = std::max(std::min(max_q, n_rows), srq_cdiv(n_rows, batch)) * group;
     Plan pl;
     pl.form = rows <= 16 ? kRows16
               : batch * H * srq_cdiv(rows, kRowsBlock) >= kCUs ? kRows128 : kRows32;
     int64_t tiles = srq_cdiv(rows, pl.form == kRows16 ? 16 : pl.form == kRows32 ? 32 : kRowsBlock);
-    if (tiles > 65536) tiles = 65536;   // the kernels' loops reach the rest
+    // no swarm of empty blocks where many uneven requests come without a hint; the
+    // kernels' loops reach the rest
+    tiles = std::min(tiles, std::max<int64_t>(64, kMaxBlocks / (batch * H)));
     const int64_t blocks = batch * H * tiles;
     int64_t chunks = 1;
     if (blocks < kCUs) {

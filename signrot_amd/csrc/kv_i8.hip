@@ -21,6 +21,8 @@
 #include "kv_i8.h"
 #include "qk_norm.h"
 
+#include <algorithm>
+
 namespace {
 
 struct AppendArgs {
@@ -185,12 +187,14 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a, PagedI8 p) {
 int launch_append(const char *name, bool fused, AppendArgs a, const PagedI8 &p, int64_t batch,
                   int64_t max_new, void *stream) {
     // a block is touched once by each of its heads' K and V waves; blocks
-    // behind the hint are reached by the loop
-    const int64_t hint = max_new < 1 ? 1 : max_new;
+    // behind the hint are reached by the loop, and so are those behind a limit
+    // that keeps many requests without a hint from a swarm of empty blocks
+    const int64_t hint = std::max<int64_t>(1, std::min(max_new, a.rows));
+    const int64_t most = std::max<int64_t>(64, (1 << 18) / batch);
     int64_t kvb = srq_cdiv((srq_cdiv(hint - 1, kI8Block) + 1) * 2 * p.H, 4);
     int64_t qb = fused ? hint : 0;
-    if (kvb > (1 << 20)) kvb = 1 << 20;
-    if (qb > (1 << 20)) qb = 1 << 20;
+    kvb = std::min(kvb, most);
+    qb = std::min(qb, most);
     a.kv_blocks = (int)kvb;
     const dim3 grid((unsigned)(kvb + qb), (unsigned)batch);
     if (fused)

@@ -90,6 +90,8 @@ def rtn_group_pack(w: torch.Tensor, groupsize: int, sym: bool = True, scales=Non
     s), codes clamp(round(W / s) + z, 0, 15).  Given scales (and zeros), as those
     that a weight was quantized with, only the codes are made.  Returns (packed
     u8 [N, K / 2], scales f16 [N, K / groupsize], zeros u8 or None)."""
+    if scales is not None and not sym and zeros is None:
+        raise ValueError("given scales of the asymmetric form come with zeros")
     n, k = w.shape
     g = w.float().view(n, k // groupsize, groupsize)
     if scales is None:

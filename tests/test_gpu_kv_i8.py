@@ -111,6 +111,35 @@ def test_append_ragged(page, hint):
     _append(c, k, v, _starts(new), hint)
 
 
+def test_many_uneven_requests_without_a_hint():
+    """Launches sized by all the rows for each of 6000 requests are cut down; one of
+    them has most of the rows, and any hint is taken."""
+    rng = np.random.default_rng(9)
+    new = [1] * 6000
+    new[17] = 5000
+    c = Cache(rng, new, 1, 16, L=1, layer=0)
+    k, v = _kv(rng, sum(new), 1)
+    q = rng.standard_normal((sum(new), 1, D)).astype(np.float16)
+    for hint in (None, 2 ** 62):
+        _append(c, k, v, _starts(new), hint)
+        c.assert_same()
+        got = _attend(c, q, _starts(new), hint)
+    first = c.scale[c.indices[c.indptr[:-1]], 0, 1, 0, 0].astype(np.float64)
+    rows = c.data[c.indices[c.indptr[:-1]], 0, 1, 0, 0] * first[:, None]
+    # one token: its own value, but for its weight's rounding and the result's
+    alone = np.array(new) == 1
+    at = _starts(new)[:-1]
+    assert (np.abs(got[at[alone], 0] - rows[alone])
+            <= 2.0 ** -10 * np.abs(rows[alone]) + 2.0 ** -25).all()
+    tail = Cache.__new__(Cache)                   # the long one's last 40 rows
+    tail.__dict__.update(c.__dict__)
+    tail.indptr, tail.last = c.indptr[17:19] - c.indptr[17], c.last[17:18]
+    tail.indices = c.indices[c.indptr[17]:c.indptr[18]]
+    end = at[17] + 5000
+    want, size = i8_ref.attention(q[end - 40:end], *tail.table(), np.array([0, 40]))
+    _close(got[end - 40:end], want, size, 5000)
+
+
 def test_append_values_at_the_ends():
     """Zero blocks, subnormal and largest values, and quotients on ties: x =
     (i + 0.5) s with s a power of two."""

@@ -38,6 +38,12 @@ def test_group_quantizer(sym):
     assert torch.equal(again[0], q) and torch.equal(again[1], s)
 
 
+def test_given_scales_come_with_their_zeros():
+    w = torch.randn(4, 64).half()
+    with pytest.raises(ValueError):
+        rtn_group_pack(w, 32, False, torch.ones(4, 2).half())
+
+
 def test_group_linear_on_the_host():
     lin = torch.nn.Linear(64, 8, dtype=torch.float16)
     mod = nn.GroupLinear4bit.from_float(lin, 32)
