@@ -1102,8 +1102,8 @@ def qkv_norm_rope_append_i8(kv_data, kv_scale, kv_indptr, kv_indices, last_page_
     q = torch.empty((rows, n_q_heads, 128), dtype=f16, device=qkv.device)
     _call_on(qkv, "srq_qkv_norm_rope_append_i8", _ptr(kv_data), _ptr(kv_scale), _ptr(kv_indptr),
              _ptr(kv_indices), _ptr(last_page_offset), *head, int(layer_idx), *tail, _ptr(qkv),
-             qkv.stride(0) if rows > 1 else cols, rows, _ptr(cos), _ptr(sin), cos.shape[0], n_q_heads,
-             _ptr(q_weight), _ptr(k_weight), 0.0 if eps is None else float(eps),
+             qkv.stride(0) if rows > 1 else cols, rows, _ptr(cos), _ptr(sin), cos.shape[0],
+             n_q_heads, _ptr(q_weight), _ptr(k_weight), 0.0 if eps is None else float(eps),
              0 if eps is None else 1, _ptr(new_indptr), hint, _ptr(q), _stream(kv_data))
     return q
 
@@ -1147,8 +1147,8 @@ def batch_attention_i8(o, q, kv_data, kv_scale, kv_indptr, kv_indices, last_page
         ws = torch.empty(n, dtype=torch.uint8, device=q.device)
     scale = 128 ** -0.5 if softmax_scale is None else float(softmax_scale)
     _call_on(q, "srq_batch_attention_i8", _ptr(o), _ptr(q), rows, Hq, _ptr(kv_data), _ptr(kv_scale),
-             _ptr(kv_indptr), _ptr(kv_indices), _ptr(last_page_offset), *head, int(layer_idx), *tail,
-             _ptr(q_indptr), hint, kv, scale, _ptr(ws), n, _stream(q))
+             _ptr(kv_indptr), _ptr(kv_indices), _ptr(last_page_offset), *head, int(layer_idx),
+             *tail, _ptr(q_indptr), hint, kv, scale, _ptr(ws), n, _stream(q))
     return o
 
 

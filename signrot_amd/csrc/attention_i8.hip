@@ -829,7 +829,7 @@ extern "C" int srq_batch_attention_i8(
     SRQ_CHECK_ARG(rows <= 0x7fffffff / n_q_heads, "batch_attention_i8: rows x heads >= 2^31");
     // (its products with a block's scale, 2^24 and 2^-100 stay normal numbers)
     SRQ_CHECK_ARG(sm_scale == 0.f || (fabsf(sm_scale) >= 0x1p-20f && fabsf(sm_scale) <= 0x1p60f),
-                  "batch_attention_i8: sm_scale=%g, neither 0 nor of magnitude 2^-20 to 2^60",
+                  "batch_attention_i8: sm_scale=%g is not a finite scale: 0, or 2^-20 to 2^60",
                   (double)sm_scale);
     if (batch == 0 || rows == 0) return SRQ_OK;
     SRQ_CHECK_ARG(o && q, "batch_attention_i8: null pointer");

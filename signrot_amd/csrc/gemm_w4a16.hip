@@ -71,6 +71,7 @@ enum { kWide, k64, k32, kAny };
 constexpr int W = 8;           // waves of a block
 constexpr int R = 2;           // blocks of 128 columns that a wave has in flight
 constexpr int kUnit = 4;       // blocks in a turn of the loop
+static_assert(R == 2 && kUnit % R == 0, "a turn refills its blocks in pairs");
 constexpr int kXS = 128 + 8;   // stride of x rows in LDS (halves)
 constexpr int kGroups = 32;    // scales of a row that a wave has in LDS at a time
 
