@@ -64,6 +64,12 @@ def test_batched_tables():
     _check(*_slots(_case(4, 9, 8, 2, 128, seed=3, cos_batch=4), 8, 2), 1e-5)
 
 
+@pytest.mark.parametrize("T", [512, 513])
+def test_tokens_with_many_heads(T):
+    """A block for every group of heads, and one for all of a token's."""
+    _check(*_slots(_case(1, T, 33, 8, 128, seed=T), 33, 8), 1e-6)
+
+
 @pytest.mark.parametrize("use", [(False, False), (True, False), (False, True)])
 def test_optional_weights(use):
     qkv, cos, sin, w = _case(2, 7, 8, 2, 128, seed=4)

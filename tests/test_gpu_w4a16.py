@@ -126,3 +126,37 @@ def test_refusals():
     base = torch.zeros(2 * 128 + 4, **f16)
     with pytest.raises(RuntimeError, match="aligned"):
         _CUDA.w4a16_linear(base[4:].view(2, 128), w, s)
+
+
+def test_stream_and_graph():
+    """A projection and the norms behind it, captured on another stream and replayed
+    with new inputs and other work between the replays: every replay is the eager
+    result bit for bit."""
+    rng = np.random.default_rng(9)
+    K, heads, D = 512, 6, 128
+    c, z = _weights(rng, heads * D, K, 64, True)
+    w, zt = torch.from_numpy(_pack(c)).to(DEV), torch.from_numpy(z).to(DEV)
+    s = torch.from_numpy(rng.uniform(0.005, 0.03, (heads * D, K // 64)).astype(np.float16)).to(DEV)
+    cos, sin = (torch.rand(1, 3, D, device=DEV).half() for _ in range(2))
+    x = torch.zeros(1, 3, K, dtype=torch.float16, device=DEV)
+
+    def run():
+        y = _CUDA.w4a16_linear(x, w, s, zt).view(1, 3, heads, D)
+        return _CUDA.qk_norm_rope(y[:, :, :4], y[:, :, 4:], cos, sin)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            got = run()
+    torch.cuda.current_stream().wait_stream(side)
+    for turn in range(4):
+        x.copy_(torch.from_numpy(rng.standard_normal((1, 3, K)).astype(np.float16)))
+        g.replay()
+        out = [t.clone() for t in got]
+        (torch.randn(1 << 20, device=DEV) * 2).sum()
+        want = run()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want)), turn
