@@ -10,13 +10,13 @@
 // bring a dword of each row to its place.  x passes through a wave's own piece of
 // LDS for the same reason, and scales through it 32 groups at a time.
 // Codes become exact fp16 integers c - z in two operations a pair (a mask that also
-// inserts the exponent of 1024, and an addition).  The products run on
+// inserts an exponent, and an addition).  The products run on
 // v_mfma_f32_16x16x32_f16 with the weights as the second operand: a lane's
 // accumulators then all belong to one output row, so its group scale is one
 // register, applied in fp32 to the group's sum, and the codes never meet a scale
 // in 16 bits.  The waves of a block split K and are joined through LDS.
 // M = 16, 8192 x 28672 with zero points, 124 MB: 37.3 us, 3.3 TB/s, bound by its
-// instructions (32 us with the weights in cache); M = 1 30 us, 4.1 TB/s; M = 1, 4096 x
+// instructions (32 us with the weights in cache); M = 1 29 us, 4.2 TB/s; M = 1, 4096 x
 // 4096 5 us, a launch and one load round trip.
 #include "common.h"
 
@@ -40,12 +40,18 @@ SRQ_DEV v4f mfma16(v8h a, v8h b, v4f c) {
 }
 
 // 8 codes of a dword (element e in bits 4 e ..) as fp16 c - zero, in the order
-// 0 4 1 5 2 6 3 7 of their places; zero2 holds -(1024 + zero) twice
+// 0 4 1 5 2 6 3 7 of their places; zero2 holds -(1024 + zero) twice.  A code is
+// masked out where it stands, in the lowest bits of a number from 1024 on or four
+// bits higher in one from 64 on, so that one shift serves all eight.
 SRQ_DEV v8h codes8(u32 w, v2h zero2) {
+    const v2h zero2s = zero2 + (v2h){960, 960};   // -(64 + zero)
     v2h d[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        d[i] = __builtin_bit_cast(v2h, ((w >> (4 * i)) & 0x000F000Fu) | 0x64006400u) + zero2;
+    for (int i = 0; i < 4; i += 2) {
+        const u32 x = w >> (4 * i);
+        d[i] = __builtin_bit_cast(v2h, (x & 0x000F000Fu) | 0x64006400u) + zero2;
+        d[i + 1] = __builtin_bit_cast(v2h, (x & 0x00F000F0u) | 0x54005400u) + zero2s;
+    }
     return (v8h){d[0][0], d[0][1], d[1][0], d[1][1], d[2][0], d[2][1], d[3][0], d[3][1]};
 }
 
