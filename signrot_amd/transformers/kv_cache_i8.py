@@ -26,17 +26,24 @@ from .kv_cache import _PageTable, _init_hf_cache, _pages_for
 
 class _LayerAttentionI8:
     """What update() returns after an append: q [B, T, Hq, 128] of the appended
-    tokens -> attention over this layer's cache, same shape."""
+    tokens -> attention over this layer's cache, same shape.  `live`: the rows of
+    [B T] that came in where the mask left some out, whose outputs are 0."""
 
-    def __init__(self, cache, layer_idx, tokens, starts):
+    def __init__(self, cache, layer_idx, tokens, starts, live=None):
         self.cache, self.layer_idx, self.tokens, self.starts = cache, layer_idx, tokens, starts
+        self.live = live
 
     def __call__(self, q):
         B, T, Hq, D = q.shape
         if T != self.tokens:
             raise ValueError(f"attention takes the {self.tokens} appended tokens, got {T}")
-        q = q.reshape(B * T, Hq, D).contiguous()
-        return self.cache._attend(q, self.layer_idx, T, self.starts).view(B, T, Hq, D)
+        q = q.reshape(B * T, Hq, D)
+        if self.live is None:
+            o = self.cache._attend(q.contiguous(), self.layer_idx, T, self.starts)
+        else:
+            o = torch.zeros(q.shape, dtype=q.dtype, device=q.device)
+            o[self.live] = self.cache._attend(q[self.live], self.layer_idx, T, self.starts)
+        return o.view(B, T, Hq, D)
 
 
 class MultiLayerPagedKVCache8Bit(Cache):
@@ -106,13 +113,33 @@ class MultiLayerPagedKVCache8Bit(Cache):
         """Row index of `tokens` rows per request, None for one each."""
         return None if tokens == 1 else self._table._row * tokens
 
+    def _check_mask(self, mask, tokens, layer_idx):
+        """The mask covers the new tokens, and behind the prefill those before them too
+        (the first layer counts the new ones)."""
+        B, first = self.batch_size, not self._filled[layer_idx]
+        want = tokens if first else self.length + (tokens if layer_idx == 0 else 0)
+        if mask.dim() != 2 or mask.shape[0] != B or mask.shape[1] < max(want, tokens) or \
+                (first and mask.shape[1] != want):
+            raise ValueError(f"attention_mask must be [{B}, {want}], got {tuple(mask.shape)}")
+
+    def _live_rows(self, mask, tokens):
+        """The rows of [B tokens] that the mask's last columns count as tokens (None
+        for all), and their index by request."""
+        live = mask[:, mask.shape[1] - tokens:] != 0
+        if bool(live.all()):
+            return None, self._starts(tokens)
+        starts = torch.zeros(self.batch_size + 1, device=self.device, dtype=torch.int32)
+        torch.cumsum(live.sum(dim=-1, dtype=torch.int32), dim=0, out=starts[1:])
+        return live.flatten().nonzero().flatten(), starts
+
     def update(self, key_states, value_states, layer_idx,
                cache_kwargs: Optional[Dict[str, Any]] = None):
         """Store K/V fp16 [B, T, H, 128] of one layer.  The first call for a layer
-        is its prefill (with an attention_mask only its 1-positions are stored)
-        and returns the inputs for the prefill attention; later calls append T
-        tokens per request and return the attention over the cache, a callable
-        that takes their queries [B, T, Hq, 128]."""
+        is its prefill and returns the inputs for the prefill attention; later calls
+        append T tokens per request and return the attention over the cache, a
+        callable that takes their queries [B, T, Hq, 128].  With an attention_mask (in
+        later calls the one of all tokens so far, its last T columns the new ones)
+        only its 1-positions are stored; a 0-position's attention is 0."""
         B, T, H, D = key_states.shape
         if H != self.num_heads:
             raise ValueError(f"update() takes the {self.num_heads} KV heads, got {H}")
@@ -122,15 +149,14 @@ class MultiLayerPagedKVCache8Bit(Cache):
         first = not self._filled[layer_idx]
         length = self.length
         try:
-            spec = self._step(T, layer_idx, mask)
             k, v = (t.reshape(B * T, H, D) for t in (key_states, value_states))
-            if first and mask is not None:
-                live = mask.flatten().nonzero().flatten()
+            live, starts = None, self._starts(T)
+            if mask is not None:
+                self._check_mask(mask, T, layer_idx)
+                live, starts = self._live_rows(mask, T)
+            spec = self._step(T, layer_idx, mask)
+            if live is not None:
                 k, v = k[live], v[live]
-                starts = torch.zeros(B + 1, device=self.device, dtype=torch.int32)
-                torch.cumsum(mask.sum(dim=-1, dtype=torch.int32), dim=0, out=starts[1:])
-            else:
-                starts = self._starts(T)
             _CUDA.append_kv_i8(**spec, layer_idx=layer_idx, k=k, v=v, new_indptr=starts, max_new=T)
         except BaseException:   # refused: no tokens came in
             self._undone(length, layer_idx)
@@ -138,7 +164,7 @@ class MultiLayerPagedKVCache8Bit(Cache):
         self._filled[layer_idx] = True
         if first:
             return key_states, value_states
-        return _LayerAttentionI8(self, layer_idx, T, starts)
+        return _LayerAttentionI8(self, layer_idx, T, starts, live)
 
     def update_qkv(self, qkv, cos, sin, layer_idx, num_q_heads, q_weight=None, k_weight=None,
                    eps=None, attention_mask=None):
@@ -148,12 +174,17 @@ class MultiLayerPagedKVCache8Bit(Cache):
         128]), k and v into the cache.  Returns q [B, T, Hq, 128], for attend().
         It may be a layer's first update too (of a prompt without padding: attend()
         then is the prefill attention, over the cache's values).  attention_mask: the
-        extended mask after a left-padded prefill, as for update()."""
+        extended mask after a left-padded prefill, as for update(), all of its last T
+        columns 1."""
         B, T = qkv.shape[:2]
         if B != self.batch_size:
             raise ValueError(f"batch {B} != the cache's {self.batch_size}")
         if attention_mask is not None and not self._filled[layer_idx]:
             raise ValueError("update_qkv() takes a prompt without padding")
+        if attention_mask is not None:
+            self._check_mask(attention_mask, T, layer_idx)
+            if self._live_rows(attention_mask, T)[0] is not None:
+                raise ValueError("update_qkv() takes new tokens without padding")
         if tuple(cos.shape) not in ((1, T, 128), (B, T, 128)) or cos.shape != sin.shape:
             raise ValueError(f"cos / sin must be [1 or {B}, {T}, 128]")
         rows = [t.reshape(T, 128) if B == 1 or (T == 1 and t.shape[0] == 1)

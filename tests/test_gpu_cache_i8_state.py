@@ -1,0 +1,51 @@
+"""MultiLayerPagedKVCache8Bit on the GPU where its state could go wrong: uneven pieces
+behind the prefill, refused calls, frozen index tensors (tests/test_host_cache_i8.py
+has the cases; here the launches themselves run)."""
+import pytest
+import torch
+
+from signrot_amd.transformers import MultiLayerPagedKVCache8Bit
+from tests import i8_ref
+from tests.gpu_util import DEV, to_np
+from tests.test_gpu_kv_cache_i8 import _gen, _rand, _state
+from tests.test_gpu_kv_i8 import _close
+
+pytestmark = pytest.mark.gpu
+D = 128
+
+
+@pytest.mark.parametrize("T", [1, 9, 40])
+def test_padding_of_a_later_piece_stays_out(T):
+    """Codes and scales of an uneven piece are those of the same tokens appended
+    request by request; its attention is that of 64 bits over them."""
+    B, H, Hq, g = 3, 2, 8, _gen(T)
+    cache = MultiLayerPagedKVCache8Bit(B, 64, 64, DEV, 1, H, D)
+    mask = torch.ones(B, 20, dtype=torch.int64, device=DEV)
+    mask[2, :3] = 0
+    k0, v0 = _rand(g, B, 20, H, D), _rand(g, B, 20, H, D)
+    cache.update(k0, v0, 0, {"attention_mask": mask})
+    new = torch.ones(B, T, dtype=torch.int64, device=DEV)
+    new[1, : max(1, T // 2)] = 0
+    if T > 1:
+        new[2, :1] = 0
+    mask = torch.cat([mask, new], 1)
+    k, v, q = _rand(g, B, T, H, D), _rand(g, B, T, H, D), _rand(g, B, T, Hq, D)
+    for t in (k, v, q):
+        t[new == 0] = float("nan")
+    got = cache.update(k, v, 0, {"attention_mask": mask})(q)
+    st = _state(cache, 0)
+    assert i8_ref.lengths(st[2], st[4], 64).tolist() == mask.sum(1).tolist()
+    starts = torch.cat([new.new_zeros(1), new.sum(1).cumsum(0)])
+    want, size = i8_ref.attention(to_np(q[new != 0]), *st, to_np(starts))
+    _close(to_np(got[new != 0]), want, size, 64)
+    assert (got[new == 0] == 0).all()
+    for b in range(B):
+        alone = MultiLayerPagedKVCache8Bit(1, 64, 64, DEV, 1, H, D)
+        first, live, n = mask[b, :20] != 0, new[b] != 0, int(mask[b].sum())
+        alone.update(k0[b: b + 1, first], v0[b: b + 1, first], 0)
+        if live.any():
+            alone.update(k[b: b + 1, live], v[b: b + 1, live], 0)
+        page = int(st[3][st[2][b]])
+        assert torch.equal(cache.pages[page, 0, :, :, :n], alone.pages[0, 0, :, :, :n])
+        assert torch.equal(cache.scales[page, 0, :, :, : -(-n // 16)],
+                           alone.scales[0, 0, :, :, : -(-n // 16)])

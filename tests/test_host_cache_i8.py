@@ -1,0 +1,143 @@
+"""MultiLayerPagedKVCache8Bit and the decode layer's use of it on the CPU: what goes
+into the pool, what the index tensors say and what is refused, with the plain append
+and attention (tests/i8_ref.py) in the place of the two launches."""
+import numpy as np
+import pytest
+import torch
+
+from signrot_amd import _CUDA
+from signrot_amd.transformers import MultiLayerPagedKVCache8Bit
+from tests import i8_ref
+
+D = 128
+
+
+def _np(t):
+    return None if t is None else t.numpy()
+
+
+@pytest.fixture(autouse=True)
+def plain_ops(monkeypatch):
+    """append_kv_i8, qkv_norm_rope_append_i8 (without a norm or a rotation) and
+    batch_attention_i8 on host tensors."""
+    def append(kv_data, kv_scale, kv_indptr, kv_indices, last_page_offset, layer_idx, k, v,
+               new_indptr=None, max_new=None):
+        if k.dtype != torch.float16:
+            raise RuntimeError("append_kv_i8: k must be fp16")
+        i8_ref.append(_np(kv_data), _np(kv_scale), _np(kv_indptr), _np(kv_indices),
+                      _np(last_page_offset), layer_idx, _np(k), _np(v), _np(new_indptr))
+
+    def qkv_append(kv_data, kv_scale, kv_indptr, kv_indices, last_page_offset, layer_idx, qkv, cos,
+                   sin, n_q_heads, q_weight=None, k_weight=None, eps=None, new_indptr=None,
+                   max_new=None):
+        H = kv_data.shape[3]
+        if qkv.shape[1] != (n_q_heads + 2 * H) * D:
+            raise RuntimeError("qkv_norm_rope_append_i8: columns")
+        q, k, v = qkv.view(len(qkv), -1, D).split((n_q_heads, H, H), dim=1)
+        append(kv_data, kv_scale, kv_indptr, kv_indices, last_page_offset, layer_idx,
+               k.contiguous(), v.contiguous(), new_indptr)
+        return q.contiguous()
+
+    def attend(o, q, kv_data, kv_scale, kv_indptr, kv_indices, last_page_offset, layer_idx,
+               q_indptr=None, max_q_len=None, max_kv_len=None, softmax_scale=None):
+        out, _ = i8_ref.attention(_np(q), _np(kv_data), _np(kv_scale), _np(kv_indptr),
+                                  _np(kv_indices), _np(last_page_offset), layer_idx, _np(q_indptr),
+                                  softmax_scale, _np(o))
+        return o.copy_(torch.from_numpy(out))
+
+    monkeypatch.setattr(_CUDA, "append_kv_i8", append)
+    monkeypatch.setattr(_CUDA, "qkv_norm_rope_append_i8", qkv_append)
+    monkeypatch.setattr(_CUDA, "batch_attention_i8", attend)
+
+
+def _cache(B, page=16, most=64, H=2, layers=1):
+    return MultiLayerPagedKVCache8Bit(B, page, most, "cpu", layers, H, D)
+
+
+def _rand(seed, *shape):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed)).half()
+
+
+def _held(cache, layer=0):
+    """The values of each request [2, H, len, D] and its length, from the index
+    tensors as they stand."""
+    t = cache.specs()
+    ptr, idx, last = (t[n].tolist() for n in ("kv_indptr", "kv_indices", "last_page_offset"))
+    out = []
+    for b in range(cache.batch_size):
+        pg = idx[ptr[b]: ptr[b + 1]]
+        n = (len(pg) - 1) * cache.page_size + last[b] if pg else 0
+        val = cache.pages[pg, layer].double().unflatten(3, (-1, 16)) * \
+            cache.scales[pg, layer].double()[..., None, None]
+        out.append(val.flatten(3, 4).permute(1, 2, 0, 3, 4).reshape(2, cache.num_heads, -1, D)
+                   [:, :, :n])
+    return out
+
+
+# ------------------------------------------------- masks behind the prefill
+
+@pytest.mark.parametrize("T", [1, 4])
+@pytest.mark.parametrize("masked_prompt", [False, True])
+def test_padding_of_a_later_piece_stays_out(T, masked_prompt):
+    """An uneven piece behind the prefill: the mask's zeros in its new columns are not
+    stored, nothing that was held before is written over, and the piece's queries see
+    what the same tokens, appended request by request, let them see."""
+    B, H, Hq = 3, 2, 4
+    cache = _cache(B)
+    mask = torch.ones(B, 8, dtype=torch.int64)
+    if masked_prompt:
+        mask[2, :3] = 0
+    k0, v0 = _rand(1, B, 8, H, D), _rand(2, B, 8, H, D)
+    cache.update(k0, v0, 0, {"attention_mask": mask} if masked_prompt else None)
+    before = _held(cache)
+    new = torch.ones(B, T, dtype=torch.int64)
+    new[1, : max(1, T // 2)] = 0
+    if T > 1:
+        new[2, :1] = 0
+    mask = torch.cat([mask, new], 1)
+    k, v, q = _rand(3, B, T, H, D), _rand(4, B, T, H, D), _rand(5, B, T, Hq, D)
+    bad = [t.clone() for t in (k, v, q)]
+    for t in bad:
+        t[new == 0] = float("nan")
+    got = cache.update(bad[0], bad[1], 0, {"attention_mask": mask})(bad[2])
+    held = _held(cache)
+    for b in range(B):
+        n, live = int(mask[b].sum()), new[b] != 0
+        assert held[b].shape[2] == n
+        alone = _cache(1)
+        first = mask[b, :8] != 0
+        alone.update(k0[b: b + 1, first], v0[b: b + 1, first], 0)
+        if live.any():
+            o = alone.update(k[b: b + 1, live], v[b: b + 1, live], 0)(q[b: b + 1, live])
+            assert torch.equal(got[b, live], o[0])
+        assert torch.equal(held[b], _held(alone)[0])
+        assert (got[b, ~live] == 0).all()
+        if not live.any():
+            assert torch.equal(held[b], before[b])
+
+
+def test_masks_that_do_not_fit_are_refused():
+    B, H = 2, 2
+    cache = _cache(B)
+    k = _rand(1, B, 8, H, D)
+    one = torch.ones(B, 20, dtype=torch.int64)
+    for m in (one[:, :7], one[:, :9], one[:1, :8], one[0, :8]):
+        with pytest.raises(ValueError):
+            cache.update(k, k, 0, {"attention_mask": m})
+    cache.update(k, k, 0, {"attention_mask": one[:, :8]})
+    before = _held(cache)
+    # of the new tokens alone, or of the held ones alone
+    for m in (one[:, :4], one[:, :8], one[:1, :12]):
+        with pytest.raises(ValueError):
+            cache.update(k[:, :4], k[:, :4], 0, {"attention_mask": m})
+    cos = torch.ones(1, 4, D, dtype=torch.float16)
+    qkv = _rand(2, B, 4, 8 * D)
+    pad = one[:, :12].clone()
+    pad[1, 8] = 0
+    for m in (one[:, :4], pad):
+        with pytest.raises(ValueError):
+            cache.update_qkv(qkv, cos, cos, 0, 4, attention_mask=m)
+    assert cache.length == 8
+    assert all(torch.equal(a, b) for a, b in zip(before, _held(cache)))
+    q = cache.update_qkv(qkv, cos, cos, 0, 4, attention_mask=one[:, :12])
+    assert q.shape == (B, 4, 4, D) and cache.length == 12
