@@ -149,6 +149,10 @@ class _PageTable:
         self.indices = torch.empty(capacity, device=self.device, dtype=torch.int32)
         self._written_for = -1
 
+    def unwritten(self):
+        """grow() has made a new indices tensor and nothing has filled it yet."""
+        return self._written_for < 0
+
     def set_pages(self, per_request: int):
         torch.mul(self._row, per_request, out=self.indptr)
         if per_request != self._written_for:

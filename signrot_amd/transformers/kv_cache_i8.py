@@ -77,6 +77,22 @@ class MultiLayerPagedKVCache8Bit(Cache):
         self._frozen = False
         self._spec = {}
         self._point_spec()
+        self._held = 0
+        self._set_table(0)
+
+    def _set_table(self, held):
+        """Index tensors of `held` tokens per request: one number, or int32 [B, 1].
+        They stay as they were where that is refused."""
+        was, self._held = self._held, held
+        try:
+            if isinstance(held, int):
+                self._table.set_uniform(held, self.page_size)
+            else:   # summed over its one column: the lengths themselves
+                self._table.set_from_mask(held, self.page_size)
+        except BaseException:
+            if self._held is not was:
+                self._set_table(was)
+            raise
 
     def _point_spec(self):
         self._spec.update(kv_data=self.pages, kv_scale=self.scales, kv_indptr=self._table.indptr,
@@ -92,9 +108,8 @@ class MultiLayerPagedKVCache8Bit(Cache):
         if need <= have:
             return
         total = max(need, 2 * have)
-        for name in ("pages", "scales"):
-            t = getattr(self, name)
-            setattr(self, name, torch.cat([t, t.new_empty((total - have, *t.shape[1:]))]))
+        self.pages, self.scales = (torch.cat([t, t.new_empty((total - have, *t.shape[1:]))])
+                                   for t in (self.pages, self.scales))
         self._table.grow(total)
         self._point_spec()
 
@@ -105,9 +120,11 @@ class MultiLayerPagedKVCache8Bit(Cache):
             self.length += tokens
         return self.get_cache_specs_for_flash_infer(mask)
 
-    def _undone(self, length, layer_idx):
-        if layer_idx == 0:
-            self.length = length
+    def _undone(self, length, held):
+        """After a refused call: length and index tensors as before it."""
+        self.length = length
+        if self._held is not held or self._table.unwritten():
+            self._set_table(held)
 
     def _starts(self, tokens):
         """Row index of `tokens` rows per request, None for one each."""
@@ -147,7 +164,7 @@ class MultiLayerPagedKVCache8Bit(Cache):
             raise ValueError(f"batch {B} != the cache's {self.batch_size}")
         mask = (cache_kwargs or {}).get("attention_mask")
         first = not self._filled[layer_idx]
-        length = self.length
+        length, held = self.length, self._held
         try:
             k, v = (t.reshape(B * T, H, D) for t in (key_states, value_states))
             live, starts = None, self._starts(T)
@@ -159,7 +176,7 @@ class MultiLayerPagedKVCache8Bit(Cache):
                 k, v = k[live], v[live]
             _CUDA.append_kv_i8(**spec, layer_idx=layer_idx, k=k, v=v, new_indptr=starts, max_new=T)
         except BaseException:   # refused: no tokens came in
-            self._undone(length, layer_idx)
+            self._undone(length, held)
             raise
         self._filled[layer_idx] = True
         if first:
@@ -189,7 +206,7 @@ class MultiLayerPagedKVCache8Bit(Cache):
             raise ValueError(f"cos / sin must be [1 or {B}, {T}, 128]")
         rows = [t.reshape(T, 128) if B == 1 or (T == 1 and t.shape[0] == 1)
                 else t.expand(B, T, 128).reshape(B * T, 128) for t in (cos, sin)]
-        length = self.length
+        length, held = self.length, self._held
         try:
             spec = self._step(T, layer_idx, attention_mask)
             q = _CUDA.qkv_norm_rope_append_i8(
@@ -197,7 +214,7 @@ class MultiLayerPagedKVCache8Bit(Cache):
                 sin=rows[1].contiguous(), n_q_heads=num_q_heads, q_weight=q_weight,
                 k_weight=k_weight, eps=eps, new_indptr=self._starts(T), max_new=T)
         except BaseException:
-            self._undone(length, layer_idx)
+            self._undone(length, held)
             raise
         self._filled[layer_idx] = True
         return q.view(B, T, num_q_heads, 128)
@@ -237,7 +254,7 @@ class MultiLayerPagedKVCache8Bit(Cache):
     def refresh_specs(self, length: Optional[int] = None):
         """Rewrite the index tensors in place for `length` tokens per request
         (default: the current length), before a replay of a captured step."""
-        self._table.set_uniform(self.length if length is None else length, self.page_size)
+        self._set_table(self.length if length is None else int(length))
         return self._spec
 
     def freeze_specs(self, frozen=True):
@@ -247,9 +264,9 @@ class MultiLayerPagedKVCache8Bit(Cache):
 
     def get_cache_specs_for_flash_infer(self, attention_mask):
         if attention_mask is not None:
-            self._table.set_from_mask(attention_mask, self.page_size)
+            self._set_table(attention_mask.sum(dim=-1, keepdim=True, dtype=torch.int32))
         elif not self._frozen:
-            self._table.set_uniform(self.length, self.page_size)
+            self._set_table(self.length)
         return self._spec
 
     def mark_prefilled(self, length: int):
@@ -258,6 +275,8 @@ class MultiLayerPagedKVCache8Bit(Cache):
         self._reserve(length)
         self.length = length
         self._filled = [True] * len(self._filled)
+        if not self._frozen:
+            self._set_table(length)
 
     def clone(self):
         """An independent copy: own pages, scales and index tensors, same state."""
@@ -273,6 +292,8 @@ class MultiLayerPagedKVCache8Bit(Cache):
     def reset(self):
         self.length = 0
         self._filled = [False] * len(self._filled)
+        if not self._frozen:
+            self._set_table(0)
 
     def get_seq_length(self, layer_idx: Optional[int] = 0) -> int:
         return self.length

@@ -49,3 +49,28 @@ def test_padding_of_a_later_piece_stays_out(T):
         assert torch.equal(cache.pages[page, 0, :, :, :n], alone.pages[0, 0, :, :, :n])
         assert torch.equal(cache.scales[page, 0, :, :, : -(-n // 16)],
                            alone.scales[0, 0, :, :, : -(-n // 16)])
+
+
+def test_index_tensors_after_refused_calls_and_resets():
+    B, H, g = 2, 2, _gen(3)
+    cache = MultiLayerPagedKVCache8Bit(B, 16, 32, DEV, 1, H, D)
+    k, q = _rand(g, B, 14, H, D), _rand(g, B, 1, 4, D)
+    cos = torch.ones(1, 9, D, dtype=torch.float16, device=DEV)
+    assert (cache.attend(q, 0) == 0).all()
+    cache.update(k, k, 0)
+    want, st = cache.attend(q, 0), _state(cache, 0)
+    many = torch.zeros(B, 300, H, D, device=DEV)
+    for call in (lambda: cache.update(k[:, :9].float(), k[:, :9].float(), 0),
+                 lambda: cache.update(many, many, 0),
+                 lambda: cache.update_qkv(_rand(g, B, 9, 7 * D), cos, cos, 0, 4),
+                 lambda: cache.refresh_specs(10 ** 6)):
+        with pytest.raises(RuntimeError):
+            call()
+        now = _state(cache, 0)
+        assert all((a[: len(b)] == b).all() for a, b in zip(now[2:5:2], st[2:5:2]))
+        assert torch.equal(cache.attend(q, 0), want)
+    copy = cache.clone()
+    cache.reset()
+    assert (cache.attend(q, 0) == 0).all()
+    copy.mark_prefilled(14)
+    assert torch.equal(copy.attend(q, 0), want)

@@ -141,3 +141,72 @@ def test_masks_that_do_not_fit_are_refused():
     assert all(torch.equal(a, b) for a, b in zip(before, _held(cache)))
     q = cache.update_qkv(qkv, cos, cos, 0, 4, attention_mask=one[:, :12])
     assert q.shape == (B, 4, 4, D) and cache.length == 12
+
+
+# ------------------------------------------ index tensors and the length agree
+
+def _unchanged(cache, call, error):
+    """A refused call leaves length, index tensors and what they show."""
+    length, before = cache.length, _held(cache)
+    q = _rand(90, cache.batch_size, 1, 4, D)
+    want = cache.attend(q, 0)
+    with pytest.raises(error):
+        call()
+    assert cache.length == length
+    got = _held(cache)
+    assert all(torch.equal(a, b) for a, b in zip(got, before))
+    assert torch.equal(cache.attend(q, 0), want)
+
+
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("masked", [False, True])
+def test_a_refused_update_leaves_the_index_tensors(page, masked):
+    B, H = 2, 2
+    cache = _cache(B, page)
+    k = _rand(1, B, 14, H, D)
+    mask = torch.ones(B, 14, dtype=torch.int64)
+    mask[1, :5] = 0
+    cache.update(k, k, 0, {"attention_mask": mask} if masked else None)
+    cos = torch.ones(1, 9, D, dtype=torch.float16)
+    kw = {}
+    if masked:
+        mask = torch.cat([mask, torch.ones(B, 9, dtype=torch.int64)], 1)
+        kw = {"attention_mask": mask}
+    refused = (RuntimeError, ValueError, NotImplementedError)
+    f = k[:, :9].float()
+    _unchanged(cache, lambda: cache.update(f, f, 0, kw), refused)
+    _unchanged(cache, lambda: cache.update_qkv(_rand(2, B, 9, 7 * D), cos, cos, 0, 4, **kw),
+               refused)
+    # a growth of the pool on the way
+    many = k[:, :1].float().expand(B, 300, H, D)
+    _unchanged(cache, lambda: cache.update(many, many, 0), refused)
+    if page == 16:   # requests that would need unlike numbers of pages
+        uneven = torch.ones(B, 23, dtype=torch.int64)
+        uneven[1, :20] = 0
+        _unchanged(cache, lambda: cache.update(k[:, :9], k[:, :9], 0,
+                                               {"attention_mask": uneven}), refused)
+    _unchanged(cache, lambda: cache.refresh_specs(10 ** 6), refused)
+    out = cache.update(k[:, :9], k[:, :9], 0, kw)
+    assert cache.length == 23 and callable(out)
+
+
+def test_the_index_tensors_follow_every_length():
+    """A new cache, one declared full and one reset, asked before their next update."""
+    B, q = 2, _rand(3, 2, 1, 4, D)
+    cache = _cache(B)
+    assert (cache.attend(q, 0) == 0).all()
+    k = _rand(4, B, 20, 2, D)
+    cache.update(k, k, 0)
+    want = cache.attend(q, 0)
+    other = _cache(B)
+    other.pages.copy_(cache.pages)
+    other.scales.copy_(cache.scales)
+    other.mark_prefilled(20)
+    assert torch.equal(other.attend(q, 0), want)
+    copy = cache.clone()
+    cache.reset()
+    assert (cache.attend(q, 0) == 0).all() and torch.equal(copy.attend(q, 0), want)
+    # frozen index tensors are the program's own
+    copy.freeze_specs(True)
+    copy.reset()
+    assert torch.equal(copy.attend(q, 0), want)
