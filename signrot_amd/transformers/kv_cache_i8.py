@@ -114,9 +114,12 @@ class MultiLayerPagedKVCache8Bit(Cache):
         self._point_spec()
 
     def _step(self, tokens, layer_idx, mask):
-        """Count the new tokens (with the first layer) and return the specs."""
+        """Count the new tokens (with the first layer) and return the specs.  Frozen
+        index tensors say themselves where the tokens go, within the pool that they
+        were made for: it keeps its place then, as a captured step needs."""
         if layer_idx == 0:
-            self._reserve(self.length + tokens)
+            if not self._frozen:
+                self._reserve(self.length + tokens)
             self.length += tokens
         return self.get_cache_specs_for_flash_infer(mask)
 
@@ -258,8 +261,8 @@ class MultiLayerPagedKVCache8Bit(Cache):
         return self._spec
 
     def freeze_specs(self, frozen=True):
-        """While frozen, update() uses the index tensors as they are, so it can be
-        captured in a graph."""
+        """While frozen, update() uses the index tensors as they are and the pool does
+        not grow, so it can be captured in a graph."""
         self._frozen = frozen
 
     def get_cache_specs_for_flash_infer(self, attention_mask):

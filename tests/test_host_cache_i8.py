@@ -210,3 +210,25 @@ def test_the_index_tensors_follow_every_length():
     copy.freeze_specs(True)
     copy.reset()
     assert torch.equal(copy.attend(q, 0), want)
+
+
+def test_a_frozen_step_keeps_the_pool():
+    """Passes over frozen index tensors (the warm-up of a captured step) write the same
+    slot each time; counted past the pool's end, they neither move nor lose it."""
+    B, q = 2, _rand(7, 2, 1, 4, D)
+    cache = _cache(B, most=32)
+    k = _rand(8, B, 31, 2, D)
+    cache.update(k, k, 0)
+    cache.refresh_specs(32)
+    cache.freeze_specs(True)
+    pool, tables = cache.pages, dict(cache.specs())
+    k1, v1 = _rand(9, B, 1, 2, D), _rand(10, B, 1, 2, D)
+    outs = [cache.update(k1, v1, 0)(q) for _ in range(4)]
+    assert all(torch.equal(o, outs[0]) for o in outs)
+    assert cache.pages is pool and all(t is cache.specs()[n] for n, t in tables.items())
+    # set free, it grows as ever
+    cache.freeze_specs(False)
+    cache.mark_prefilled(32)
+    assert torch.equal(cache.attend(q, 0), outs[0])
+    cache.update(k1, v1, 0)
+    assert cache.pages.shape[0] > pool.shape[0] and cache.length == 33
