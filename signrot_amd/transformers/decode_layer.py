@@ -24,8 +24,22 @@ from ..functional.hadamard import _inv_sqrt_f32, get_hadK, matmul_hadU_cuda
 from ..functional.quantization import rtn_weight_pack
 from ..nn.derived import derived
 from ..nn.normalization import RMSNorm
-from .kv_cache import qkv_prefill_of
+from .kv_cache import HFCacheAdapter, MultiLayerPagedKVCache4Bit, qkv_prefill_of
 from .kv_cache_i8 import MultiLayerPagedKVCache8Bit
+
+
+def _refuse_held(cache, layer_idx, tokens):
+    """A prefill's refusal of a layer that has its context, ahead of the update()
+    that would store its tokens behind it (an update() that is not the caches' own
+    is asked itself)."""
+    cache = cache.inner if isinstance(cache, HFCacheAdapter) else cache
+    own = getattr(getattr(cache, "update", None), "__func__", None)
+    if own not in (MultiLayerPagedKVCache4Bit.update, MultiLayerPagedKVCache8Bit.update) or \
+            not cache._filled[layer_idx]:
+        return
+    if isinstance(cache, MultiLayerPagedKVCache4Bit) and tokens != 1:
+        raise ValueError("after the prefill, update() appends one token per request")
+    raise RuntimeError("prefill: the cache already holds this layer's context")
 
 
 def rope_cos_sin(positions, head_dim, theta, device):
@@ -234,6 +248,7 @@ class W4A4LlamaDecodeLayer(torch.nn.Module):
         q, k = self._rope(q, k, cos, sin)
         keep("q_rope", q)
         keep("k_rope", k)
+        _refuse_held(cache, self.layer_idx, T)
         out = cache.update(k, v, self.layer_idx, {"attention_mask": attention_mask})
         if not isinstance(out, tuple):
             raise RuntimeError("prefill: the cache already holds this layer's context")
@@ -286,6 +301,7 @@ class W4A4LlamaDecodeLayer(torch.nn.Module):
             else:
                 q, k, v = (t.contiguous() for t in heads)
                 kernel.rope_qk(q, k, cos, sin)
+            _refuse_held(cache, self.layer_idx, T)
             out = cache.update(k, v, self.layer_idx, {"attention_mask": attention_mask})
             if not isinstance(out, tuple):
                 raise RuntimeError("prefill: the cache already holds this layer's context")

@@ -4,10 +4,12 @@ has the cases; here the launches themselves run)."""
 import pytest
 import torch
 
-from signrot_amd.transformers import MultiLayerPagedKVCache8Bit
+from signrot_amd.transformers import (HFCacheAdapter, MultiLayerPagedKVCache4Bit,
+                                      MultiLayerPagedKVCache8Bit)
+from signrot_amd.transformers import decode_layer as dl
 from tests import i8_ref
 from tests.gpu_util import DEV, to_np
-from tests.test_gpu_kv_cache_i8 import _gen, _rand, _state
+from tests.test_gpu_kv_cache_i8 import _cache, _gen, _layer, _rand, _state
 from tests.test_gpu_kv_i8 import _close
 
 pytestmark = pytest.mark.gpu
@@ -74,3 +76,28 @@ def test_index_tensors_after_refused_calls_and_resets():
     assert (cache.attend(q, 0) == 0).all()
     copy.mark_prefilled(14)
     assert torch.equal(copy.attend(q, 0), want)
+
+
+@pytest.mark.parametrize("qk_norm", [False, True])
+@pytest.mark.parametrize("cls", [MultiLayerPagedKVCache4Bit, MultiLayerPagedKVCache8Bit])
+@pytest.mark.parametrize("T", [1, 5])
+@pytest.mark.parametrize("wrap", [False, True])
+def test_a_refused_prefill_leaves_the_cache(qk_norm, cls, T, wrap):
+    """A prefill of a layer that has its context, fused and op by op: nothing is
+    stored or counted, and the next decode step is as without it."""
+    layer, B, g = _layer(qk_norm), 2, _gen(4)
+    h = _rand(g, B, 20, 1024)
+    cos, sin = dl.rope_cos_sin(range(20), D, 10000.0, DEV)
+    caches = [_cache(cls, B, 64) for _ in range(2)]
+    for c in caches:
+        c.pages.zero_()
+        layer.prefill(h.clone(), c, cos, sin)
+    c = HFCacheAdapter(caches[0]) if wrap else caches[0]
+    for trace in (None, {}):
+        with pytest.raises((RuntimeError, ValueError)):
+            layer.prefill(h[:, :T].clone(), c, cos[:, :T], sin[:, :T], trace=trace)
+        assert caches[0].length == 20
+    assert torch.equal(caches[0].pages[: B], caches[1].pages[: B])
+    cos, sin = dl.rope_cos_sin([20], D, 10000.0, DEV)
+    outs = [layer(h[:, :1].clone(), c, cos, sin) for c in caches]
+    assert torch.equal(*outs) and caches[0].length == 21
