@@ -87,12 +87,27 @@ def rtn_group_pack(w: torch.Tensor, groupsize: int, sym: bool = True, scales=Non
     of `groupsize` columns, on the grid that the kernels compute with (the fp16
     scales): symmetric, s = fp16(max|W| / 7), codes clamp(round(W / s), -8, 7);
     else over the range widened to 0, s = fp16((max - min) / 15), z = round(-min /
-    s), codes clamp(round(W / s) + z, 0, 15).  Given scales (and zeros), as those
-    that a weight was quantized with, only the codes are made.  Returns (packed
-    u8 [N, K / 2], scales f16 [N, K / groupsize], zeros u8 or None)."""
+    s), codes clamp(round(W / s) + z, 0, 15).  Given scales (and zeros) [N, K /
+    groupsize], as those that a weight was quantized with, only the codes are made;
+    scales are finite and not 0 in fp16, zeros whole numbers of 0 to 255 (0 when
+    sym).  Returns (packed u8 [N, K / 2], scales f16 [N, K / groupsize], zeros u8 or
+    None)."""
     if scales is not None and not sym and zeros is None:
         raise ValueError("given scales of the asymmetric form come with zeros")
+    if zeros is not None and scales is None:
+        raise ValueError("given zeros come with their scales")
     n, k = w.shape
+    if groupsize <= 0 or k % groupsize:
+        raise ValueError(f"groupsize={groupsize} must divide the {k} columns")
+    for t, name in ((scales, "scales"), (zeros, "zeros")):
+        if t is not None and tuple(t.shape) != (n, k // groupsize):
+            raise ValueError(f"{name} must be [{n}, {k // groupsize}], one for each group, got "
+                             f"{tuple(t.shape)}")
+    if zeros is not None and not bool(((zeros >= 0) & (zeros <= (0 if sym else 255))
+                                       & (zeros == zeros.to(torch.uint8))).all()):
+        raise ValueError("zeros must be 0 in the symmetric form, else whole numbers of 0 to 255")
+    if scales is not None and not bool((torch.isfinite(scales.half()) & (scales.half() != 0)).all()):
+        raise ValueError("scales must be finite and not 0 in fp16")
     g = w.float().view(n, k // groupsize, groupsize)
     if scales is None:
         lo, hi = g.amin(-1).clamp(max=0), g.amax(-1).clamp(min=0)

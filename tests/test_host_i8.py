@@ -62,3 +62,27 @@ def test_softmax_scales_that_leave_the_range_are_refused(sm):
     rc = _native.lib().srq_batch_attention_i8(
         64, 64, 1, 1, 64, 64, 64, 64, 64, 1, 1, 1, 1, 0, 1, 16, 128, None, 1, 16, sm, None, 0, None)
     assert rc != 0 and b"sm_scale" in _native.lib().srq_last_error()
+
+
+@pytest.mark.parametrize("sym", [True, False])
+def test_given_scales_have_one_for_each_group(sym):
+    """Scales and zeros of another shape, which would broadcast, zeros that a byte does
+    not hold and zeros without their scales are refused."""
+    lin = torch.nn.Linear(128, 6, dtype=torch.float16)
+    s, z = torch.full((6, 4), 0.01).half(), None if sym else torch.full((6, 4), 8.0)
+    ok = nn.GroupLinear4bit.from_float(lin, 32, sym, s, z)
+    assert ok.weight_scales.shape == (6, 4)
+    bad = [(s[:, :1], z), (s[:1], z), (s[:, :2], z), (s.flatten(), z), (s[:5], z),
+           (s.float() * 1e-7, z), (s.float() * 1e8, z), (s * float("nan"), z)]
+    if sym:
+        with_zeros = nn.GroupLinear4bit.from_float(lin, 32, sym, s, torch.zeros(6, 4))
+        assert torch.equal(with_zeros.weight, ok.weight) and with_zeros.weight_zeros is None
+        bad += [(s, torch.ones(6, 4)), (None, torch.zeros(6, 4))]
+    else:
+        bad += [(s, z[:, :1]), (s, z - 9), (s, z + 248), (s, z + 0.5), (None, z),
+                (s, torch.full((6, 4), float("nan")))]
+    for scales, zeros in bad:
+        with pytest.raises(ValueError):
+            nn.GroupLinear4bit.from_float(lin, 32, sym, scales, zeros)
+    with pytest.raises(ValueError):
+        rtn_group_pack(lin.weight.data, 48)
