@@ -106,7 +106,8 @@ def rtn_group_pack(w: torch.Tensor, groupsize: int, sym: bool = True, scales=Non
     if zeros is not None and not bool(((zeros >= 0) & (zeros <= (0 if sym else 255))
                                        & (zeros == zeros.to(torch.uint8))).all()):
         raise ValueError("zeros must be 0 in the symmetric form, else whole numbers of 0 to 255")
-    if scales is not None and not bool((torch.isfinite(scales.half()) & (scales.half() != 0)).all()):
+    if scales is not None and not bool((torch.isfinite(scales.half())
+                                        & (scales.half() != 0)).all()):
         raise ValueError("scales must be finite and not 0 in fp16")
     g = w.float().view(n, k // groupsize, groupsize)
     if scales is None:

@@ -211,7 +211,7 @@ class GroupLinear4bit(torch.nn.Module):
     def from_float(module: torch.nn.Linear, groupsize=128, sym=True, scales=None, zeros=None):
         """Round-to-nearest quantization of an fp16 Linear, or with given scales
         (and zeros) [out, in / groupsize] the codes of a weight that lies on their
-        grid."""
+        grid: after GPTQ by groups, its quantizer's group_scale and group_zero."""
         w = module.weight.data
         out = GroupLinear4bit(module.in_features, module.out_features, groupsize, sym,
                               module.bias is not None)

@@ -353,7 +353,12 @@ class WeightQuantizer:
     Asymmetric: scale = (max - min).clamp(1e-5) / maxq, zero =
     round(-min / scale), codes clamp(round(w / scale) + zero, 0, maxq).
     With mse, the range is shrunk by p = 1 - i / grid for i < maxshrink *
-    grid and the p with the least sum |w - q(w)|^norm is kept, per row."""
+    grid and the p with the least sum |w - q(w)|^norm is kept, per row.
+
+    scale and zero [rows, 1] are those of the last find_params; after GPTQ with
+    groups of columns, group_scale and group_zero [rows, groups] hold every group's
+    (None otherwise, and where act-order made the groups of columns that are not
+    neighbours)."""
 
     def __init__(self, bits=4, perchannel=True, sym=True, mse=False, norm=2.4, grid=100,
                  maxshrink=0.8, extend_zero=True, symmetric_grid=False):
@@ -362,6 +367,7 @@ class WeightQuantizer:
         self.extend_zero, self.symmetric_grid = extend_zero, symmetric_grid
         self.maxq = 2 ** (bits - 1) - 1 if sym else 2 ** bits - 1
         self.scale = self.zero = None
+        self.group_scale = self.group_zero = None
 
     def ready(self):
         return self.scale is not None
@@ -475,6 +481,7 @@ class GPTQ:
                 gq = copy.deepcopy(q)
                 gq.find_params(W[:, g0:g0 + groupsize])
                 groups.append(gq)
+        params = [(gq.scale, gq.zero) for gq in groups or ()]
         perm = None
         if actorder:
             perm = torch.argsort(torch.diagonal(H), descending=True)
@@ -502,6 +509,7 @@ class GPTQ:
                         # the current block have not received this block's
                         # error updates yet (gptq_utils.py:113-118)
                         q.find_params(W[:, col:col + groupsize])
+                        params.append((q.scale, q.zero))
                 w = W1[:, i]
                 d = Hb[i, i]
                 qc = q.quantize(w.unsqueeze(1)).flatten()
@@ -515,6 +523,9 @@ class GPTQ:
         if torch.isnan(Q).any():
             raise ValueError("GPTQ produced NaN weights")
         lin.weight.data = Q.reshape(lin.weight.shape).to(lin.weight.dtype)
+        q.group_scale = q.group_zero = None
+        if params and params[0][0] is not None and (static_groups or not actorder):
+            q.group_scale, q.group_zero = (torch.cat(t, 1) for t in zip(*params))
         self.quantizer = q
         return q
 
