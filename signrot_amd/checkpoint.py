@@ -129,8 +129,9 @@ def load_decode_layer(layer, ckpt, prefix):
     (e.g. "model.layers.0."): q/k/v and gate/up codes and scales are
     concatenated along the output dim (the layer's fused layout), o/down
     taken as stored, the SignRot down_proj sign copied.  The RMSNorms carry
-    no weight (SignRot folds them into the following linears).  `ckpt` is a
-    PackedCheckpoint (raw keys)."""
+    no weight (SignRot folds them into the following linears), but those of the
+    query and key heads of a layer with qk_norm do; a checkpoint has them
+    exactly if the layer does.  `ckpt` is a PackedCheckpoint (raw keys)."""
     def t(k):
         return ckpt.get_tensor(prefix + k)
 
@@ -138,7 +139,18 @@ def load_decode_layer(layer, ckpt, prefix):
         return ckpt.get_tensor(f"quantizer.{prefix}{name}.scale").reshape(-1).to(torch.float16)
 
     att, mlp = "self_attn.", "mlp."
+    norms = [prefix + att + n + ".weight" for n in ("q_norm", "k_norm")]
+    qk_norm = getattr(layer, "qk_norm", False)
+    if any((n in ckpt.keys()) != qk_norm for n in norms):
+        raise ValueError(f"the layer has {'' if qk_norm else 'no '}q/k norms, the checkpoint's "
+                         f"keys do not match: {', '.join(norms)}")
     with torch.no_grad():
+        if qk_norm:
+            for key, buf in zip(norms, (layer.q_norm, layer.k_norm)):
+                w = ckpt.get_tensor(key)
+                if w.shape != buf.shape:
+                    raise ValueError(f"{key} must be {tuple(buf.shape)}, got {tuple(w.shape)}")
+                buf.copy_(w)
         layer.w_qkv.copy_(torch.cat([t(att + p + ".weight") for p in ("q_proj", "k_proj",
                                                                         "v_proj")]))
         layer.s_qkv.copy_(torch.cat([scale(att + p) for p in ("q_proj", "k_proj", "v_proj")]))
@@ -158,7 +170,8 @@ def decode_layer_tensors(layer, prefix):
     codes and scales under the reference's checkpoint keys
     (realquant_utils.py:85-142 writes `<prefix>self_attn.q_proj.weight` u8
     [out, in/2] and `quantizer.<prefix>self_attn.q_proj.scale` fp16
-    [out, 1] per linear, plus `<prefix>mlp.down_proj.had_adj_sign`): the
+    [out, 1] per linear, plus `<prefix>mlp.down_proj.had_adj_sign`; with
+    qk_norm also `<prefix>self_attn.q_norm.weight` and `k_norm.weight`): the
     fused q/k/v and gate/up buffers are split back into their projections.
     Tensors are copied to the CPU."""
     hd = layer.head_dim
@@ -178,4 +191,7 @@ def decode_layer_tensors(layer, prefix):
         out[key + ".weight"] = w.detach().cpu().contiguous()
         out[f"quantizer.{key}.scale"] = s.detach().cpu().reshape(-1, 1).contiguous()
     out[mlp + "down_proj.had_adj_sign"] = layer.down_sign.detach().cpu().contiguous()
+    if getattr(layer, "qk_norm", False):
+        out[att + "q_norm.weight"] = layer.q_norm.detach().cpu().contiguous()
+        out[att + "k_norm.weight"] = layer.k_norm.detach().cpu().contiguous()
     return out
