@@ -715,7 +715,7 @@ int srq_qk_norm_rope(const void *q, const void *k, const void *cos, const void *
  * the new tokens.  Per block and head: scale = max(the block's scale if it holds
  * older tokens, fp32(max|new| * fp32(1 / 127))), new codes rne(x / scale), and older
  * codes c become rne(c * old scale / scale) where it grew, all as in exact
- * arithmetic.  A non-finite new value makes the block's scale NaN.  Rows of a
+ * arithmetic: each growth adds up to half a step of error to them.  A non-finite new value makes the block's scale NaN.  Rows of a
  * page behind the last token stay as they are.  A page that is written may belong
  * to one request only.  max_new >= the largest number of new tokens sizes the
  * launch (any value gives the same result). */

@@ -1043,8 +1043,9 @@ def append_kv_i8(kv_data, kv_scale, kv_indptr, kv_indices, last_page_offset, lay
     block of 16 tokens and head (page a multiple of 16).  Request b gets rows
     new_indptr[b] .. new_indptr[b + 1] (int32), or row b without an index; the
     page table counts them already.  A block that holds older tokens keeps the
-    larger of its scale and the new one, its codes requantized where it grew; a
-    non-finite value makes its block read as NaN.  k and v may be column slices
+    larger of its scale and the new one, its codes requantized where it grew (half
+    a step of error for a block that came at once, up to half a step more for each
+    growth); a non-finite value makes its block read as NaN.  k and v may be column slices
     (dense rows [H, 128]).  max_new: the largest number of new tokens, which sizes
     the launch.  Requests may share pages, but not the block that one of them
     appends to."""

@@ -8,8 +8,13 @@
 // magnitude over the wave and needs no LDS and no other wave.  With
 //   s = max(s_old, fp32(max|new| * fp32(1 / 127)))   s_old = 0 for a block without
 // older tokens, new codes are rne(x / s), and where s grew the older codes
-// follow, c -> rne(c s_old / s): they stay within one step of what was
-// appended first, instead of being clipped.  A NaN or an infinity among the
+// follow, c -> rne(c s_old / s), instead of being clipped.  Each growth rounds them
+// anew, by up to half a step of that time: a token is off by half a step when its
+// block came in one piece and by up to half a step more for every growth behind it,
+// 8 in the worst order of 16 single tokens.  Normal values one token at a time: 2.5
+// growths a block, its largest error 1.2 steps on average (2.4 in 400 blocks), its
+// rms error 25% above that of one piece; where one channel grows by 1% a token, codes
+// below 50 stand still and so grow with the scale, 6.5 steps.  A NaN or an infinity among the
 // new values makes the scale NaN: the block reads as NaN until it is started
 // anew.
 //

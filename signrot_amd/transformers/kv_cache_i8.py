@@ -4,8 +4,12 @@ attention 4 bits hurt and for models with query / key norms.
   pages  i8  [pages, n_layers, 2, num_heads, page_size, 128]      (K, V)
   scales f32 [pages, n_layers, 2, num_heads, page_size / 16]
 
-value = code * scale, one scale for each block of 16 tokens and head: 257 bytes a
-token and head for K and V together against the int4 cache's 136.  The page table
+value = code * scale, one scale for each block of 16 tokens and head: 256.5 bytes a
+token and head for K and V together against the int4 cache's 136.  Tokens that come
+one at a time are kept less exactly than a prompt's: each growth of the open block's
+scale rounds its older codes again (normal values: 25% more rms error than in one
+piece), so what the cache holds depends on how the tokens were cut into calls.  The
+page table
 is the int4 cache's (request b's page j is page j * B + b), and so are the protocol
 of update() and that of graph capture.  Differences:
   * update() takes any number of tokens after the prefill (a prompt's next piece,
