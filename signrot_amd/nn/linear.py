@@ -156,7 +156,8 @@ class GroupLinear4bit(torch.nn.Module):
 
     forward(tensor): up to `MAX_ROWS` tokens on the GPU go through w4a16_linear,
     which reads the packed weight once; more of them, an input that wants a
-    gradient or one on the host are a matrix product with the dequantized weight."""
+    gradient or carries a tangent, or one on the host are a matrix product with the
+    dequantized weight."""
 
     # us on one MI355X, w4a16_linear against dequantization and product: 512 rows
     # through 4096 x 4096 85 / 231, 8192 x 28672 902 / 3409, 28672 x 4096 611 / 1569
@@ -202,7 +203,8 @@ class GroupLinear4bit(torch.nn.Module):
 
     def forward(self, x):
         if (x.is_cuda and x.numel() <= self.MAX_ROWS * self.in_features
-                and not (x.requires_grad and torch.is_grad_enabled())):
+                and not (x.requires_grad and torch.is_grad_enabled())
+                and torch.autograd.forward_ad.unpack_dual(x).tangent is None):
             return kernel.w4a16_linear(x, self.weight, self.weight_scales, self.weight_zeros,
                                        self.bias)
         return torch.nn.functional.linear(x, self.dequantized(), self.bias)
