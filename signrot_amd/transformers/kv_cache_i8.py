@@ -246,6 +246,10 @@ class MultiLayerPagedKVCache8Bit(Cache):
         Hadamard (times scale) and the per-token quantizer.  qkv [B, (Hq + 2 H) 128]."""
         if not self._filled[layer_idx]:
             raise RuntimeError("update_qkv_decode_quant: the layer has no prefill yet")
+        if not 0 < num_q_heads <= 64 or num_q_heads & (num_q_heads - 1) or \
+                num_q_heads % self.num_heads:
+            raise RuntimeError(f"update_qkv_decode_quant: {num_q_heads} query heads must be a power "
+                               f"of two <= 64 and a multiple of the {self.num_heads} KV heads")
         B = qkv.shape[0]
         q = self.update_qkv(qkv.view(B, 1, -1), cos, sin, layer_idx, num_q_heads, q_weight,
                             k_weight, eps, attention_mask)

@@ -232,3 +232,20 @@ def test_a_frozen_step_keeps_the_pool():
     assert torch.equal(cache.attend(q, 0), outs[0])
     cache.update(k1, v1, 0)
     assert cache.pages.shape[0] > pool.shape[0] and cache.length == 33
+
+
+@pytest.mark.parametrize("heads,kv", [(6, 2), (3, 2), (128, 2), (2, 4)])
+def test_a_refused_decode_step_stores_nothing(heads, kv):
+    """Query heads that the attention or the head-axis rotation behind it does not
+    take are refused before the token goes into the cache."""
+    B = 2
+    cache = _cache(B, H=kv)
+    k = _rand(1, B, 5, kv, D)
+    cache.update(k, k, 0)
+    pages, scales, before = cache.pages.clone(), cache.scales.clone(), _held(cache)
+    cos = torch.ones(1, 1, D, dtype=torch.float16)
+    with pytest.raises(RuntimeError, match="heads"):
+        cache.update_qkv_decode_quant(_rand(2, B, (heads + 2 * kv) * D), cos, cos, 0, heads, 1.0)
+    assert cache.length == 5 and torch.equal(cache.pages, pages)
+    assert torch.equal(cache.scales.view(torch.int32), scales.view(torch.int32))
+    assert all(torch.equal(a, b) for a, b in zip(before, _held(cache)))
