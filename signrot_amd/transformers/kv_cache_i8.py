@@ -62,6 +62,9 @@ class MultiLayerPagedKVCache8Bit(Cache):
             raise ValueError("head_dim must be 128")
         if page_size <= 0 or page_size % _CUDA.I8_BLOCK:
             raise ValueError(f"page_size must be a multiple of {_CUDA.I8_BLOCK}")
+        if softmax_scale and not 2.0 ** -20 <= abs(softmax_scale) <= 2.0 ** 60:
+            raise ValueError(f"softmax_scale={softmax_scale} must be 0, or 2^-20 to 2^60 in "
+                             "magnitude")
         _init_hf_cache(self)
         self.batch_size = batch_size
         self.page_size = page_size

@@ -249,3 +249,12 @@ def test_a_refused_decode_step_stores_nothing(heads, kv):
     assert cache.length == 5 and torch.equal(cache.pages, pages)
     assert torch.equal(cache.scales.view(torch.int32), scales.view(torch.int32))
     assert all(torch.equal(a, b) for a, b in zip(before, _held(cache)))
+
+
+@pytest.mark.parametrize("sm", [float("nan"), float("inf"), 1e20, 1e-7, -1e-40])
+def test_softmax_scales_are_checked_when_the_cache_is_made(sm):
+    """And not by the attention, when the token is in the cache already."""
+    with pytest.raises(ValueError, match="softmax_scale"):
+        MultiLayerPagedKVCache8Bit(1, 16, 16, "cpu", 1, 1, D, softmax_scale=sm)
+    for ok in (None, 0.0, 2.0 ** -20, -0.125, 2.0 ** 60):
+        MultiLayerPagedKVCache8Bit(1, 16, 16, "cpu", 1, 1, D, softmax_scale=ok)
