@@ -1174,7 +1174,7 @@ def w4a16_linear(x, w, scales, zeros=None, bias=None):
     if x.shape[-1] != K or scales.shape[0] != N:
         raise RuntimeError(f"w4a16_linear: x {tuple(x.shape)} and scales {tuple(scales.shape)} do "
                            f"not fit weights of {N} x {K}")
-    if groups == 0 or K % groups or (K // groups) % 32:
+    if K == 0 or groups == 0 or K % groups or (K // groups) % 32:
         raise RuntimeError(f"w4a16_linear: {groups} groups of {K} columns: a group must be a "
                            "multiple of 32 columns")
     if zeros is not None and zeros.shape != scales.shape:

@@ -3,7 +3,7 @@ forward mode, and the form it takes at and behind MAX_ROWS."""
 import pytest
 import torch
 
-from signrot_amd import nn
+from signrot_amd import _CUDA, nn
 from tests.gpu_util import DEV
 
 pytestmark = pytest.mark.gpu
@@ -32,3 +32,11 @@ def test_forward_mode_tangents_are_kept():
         # an input without one, at the same level, has none to lose
         assert torch.equal(mod(x), mod(x.clone()))
     assert fw.unpack_dual(mod(x)).tangent is None
+
+
+def test_a_linear_without_columns_is_refused_by_name():
+    f16 = dict(dtype=torch.float16, device=DEV)
+    w = torch.zeros(16, 0, dtype=torch.uint8, device=DEV)
+    for groups in (0, 2):
+        with pytest.raises(RuntimeError, match="w4a16_linear"):
+            _CUDA.w4a16_linear(torch.zeros(2, 0, **f16), w, torch.ones(16, groups, **f16))
