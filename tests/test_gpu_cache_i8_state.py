@@ -4,6 +4,7 @@ has the cases; here the launches themselves run)."""
 import pytest
 import torch
 
+from signrot_amd.functional import kernel
 from signrot_amd.transformers import (HFCacheAdapter, MultiLayerPagedKVCache4Bit,
                                       MultiLayerPagedKVCache8Bit)
 from signrot_amd.transformers import decode_layer as dl
@@ -101,3 +102,28 @@ def test_a_refused_prefill_leaves_the_cache(qk_norm, cls, T, wrap):
     cos, sin = dl.rope_cos_sin([20], D, 10000.0, DEV)
     outs = [layer(h[:, :1].clone(), c, cos, sin) for c in caches]
     assert torch.equal(*outs) and caches[0].length == 21
+
+
+@pytest.mark.parametrize("page", [16, 32, 64])
+def test_update_qkv_stores_the_bits_of_the_two_calls(page):
+    """Codes of every held token and scales of every block that holds one, in pages of
+    one block and of several."""
+    B, H, Hq, g = 2, 2, 8, _gen(page)
+    caches = [MultiLayerPagedKVCache8Bit(B, page, 100, DEV, 1, H, D) for _ in range(2)]
+    w = [(1 + 0.2 * torch.randn(D, device=DEV, generator=g)).half() for _ in range(2)]
+    pos = 0
+    for T in (40, 1, 17, 1, 30):
+        qkv = _rand(g, B, T, (Hq + 2 * H) * D)
+        cos, sin = dl.rope_cos_sin(range(pos, pos + T), D, 10000.0, DEV)
+        caches[0].update_qkv(qkv, cos, sin, 0, Hq, *w, 1e-6)
+        heads = qkv.view(B, T, -1, D)
+        _, k = kernel.qk_norm_rope(heads[:, :, :Hq], heads[:, :, Hq: Hq + H], cos, sin, *w, 1e-6)
+        caches[1].update(k, heads[:, :, Hq + H:], 0)
+        pos += T
+        held = []
+        for c in caches:
+            pg = c.specs()["kv_indices"][: -(-pos // page) * B].view(B, -1).long()
+            codes = c.pages[pg, 0].permute(0, 2, 3, 1, 4, 5).reshape(B, 2, H, -1, D)
+            scales = c.scales[pg, 0].permute(0, 2, 3, 1, 4).reshape(B, 2, H, -1)
+            held.append((codes[:, :, :, :pos], scales[..., : -(-pos // 16)]))
+        assert all(torch.equal(a, b) for a, b in zip(*held)), T
