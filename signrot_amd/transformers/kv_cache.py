@@ -166,17 +166,22 @@ class _PageTable:
         self.set_pages(_pages_for(length, page_size))
 
     def set_from_mask(self, attention_mask, page_size: int):
-        """Per-request lengths from an HF attention_mask [B, T]; every request
-        must need the same number of pages (the shared page count is read on
-        the host)."""
-        lens = attention_mask.sum(dim=-1, dtype=torch.int32)
-        pages = (lens + page_size - 1) // page_size
+        """Per-request lengths from an HF attention_mask [B, T]."""
+        self.set_lengths(attention_mask.sum(dim=-1, dtype=torch.int32), page_size)
+
+    def set_lengths(self, lens, page_size: int, beside=None):
+        """Lengths int32 [B]; every request must need the same number of pages
+        (read on the host, in one transfer, and with them `beside`, another int32
+        [B], which is returned)."""
+        host = (lens if beside is None else torch.stack((lens, beside))).cpu().numpy()
+        pages = _pages_for(host if beside is None else host[0], page_size)
         lo, hi = int(pages.min()), int(pages.max())
         if lo != hi:
             raise NotImplementedError("Current implementation does not support the case where "
                                       "batches have different number of pages")
         self.last.copy_(torch.where(lens > 0, (lens - 1) % page_size + 1, 0))
         self.set_pages(lo)
+        return None if beside is None else host[1]
 
     def clone(self):
         t = _PageTable.__new__(_PageTable)

@@ -87,15 +87,15 @@ class MultiLayerPagedKVCache8Bit(Cache):
         self._held = 0
         self._set_table(0)
 
-    def _set_table(self, held):
-        """Index tensors of `held` tokens per request: one number, or int32 [B, 1].
-        They stay as they were where that is refused."""
+    def _set_table(self, held, beside=None):
+        """Index tensors of `held` tokens per request: one number, or int32 [B] (which
+        the host reads, and `beside` with them).  They stay as they were where that is
+        refused."""
         was, self._held = self._held, held
         try:
             if isinstance(held, int):
-                self._table.set_uniform(held, self.page_size)
-            else:   # summed over its one column: the lengths themselves
-                self._table.set_from_mask(held, self.page_size)
+                return self._table.set_uniform(held, self.page_size)
+            return self._table.set_lengths(held, self.page_size, beside)
         except BaseException:
             if self._held is not was:
                 self._set_table(was)
@@ -121,14 +121,19 @@ class MultiLayerPagedKVCache8Bit(Cache):
         self._point_spec()
 
     def _step(self, tokens, layer_idx, mask):
-        """Count the new tokens (with the first layer) and return the specs.  Frozen
-        index tensors say themselves where the tokens go, within the pool that they
-        were made for: it keeps its place then, as a captured step needs."""
+        """Count the new tokens (with the first layer), write the index tensors and
+        return whether the mask counts all of the new ones.  Frozen index tensors say
+        themselves where the tokens go, within the pool that they were made for: it
+        keeps its place then, as a captured step needs."""
         if layer_idx == 0:
             if not self._frozen:
                 self._reserve(self.length + tokens)
             self.length += tokens
-        return self.get_cache_specs_for_flash_infer(mask)
+        if mask is None:
+            self.get_cache_specs_for_flash_infer(None)
+            return True
+        new = mask[:, mask.shape[1] - tokens:].sum(dim=-1, dtype=torch.int32)
+        return bool((self._set_table(mask.sum(dim=-1, dtype=torch.int32), new) == tokens).all())
 
     def _undone(self, length, held):
         """After a refused call: length and index tensors as before it."""
@@ -150,11 +155,9 @@ class MultiLayerPagedKVCache8Bit(Cache):
             raise ValueError(f"attention_mask must be [{B}, {want}], got {tuple(mask.shape)}")
 
     def _live_rows(self, mask, tokens):
-        """The rows of [B tokens] that the mask's last columns count as tokens (None
-        for all), and their index by request."""
+        """The rows of [B tokens] that the mask's last columns count as tokens, and
+        their index by request."""
         live = mask[:, mask.shape[1] - tokens:] != 0
-        if bool(live.all()):
-            return None, self._starts(tokens)
         starts = torch.zeros(self.batch_size + 1, device=self.device, dtype=torch.int32)
         torch.cumsum(live.sum(dim=-1, dtype=torch.int32), dim=0, out=starts[1:])
         return live.flatten().nonzero().flatten(), starts
@@ -177,14 +180,14 @@ class MultiLayerPagedKVCache8Bit(Cache):
         length, held = self.length, self._held
         try:
             k, v = (t.reshape(B * T, H, D) for t in (key_states, value_states))
-            live, starts = None, self._starts(T)
             if mask is not None:
                 self._check_mask(mask, T, layer_idx)
+            if self._step(T, layer_idx, mask):
+                live, starts = None, self._starts(T)
+            else:
                 live, starts = self._live_rows(mask, T)
-            spec = self._step(T, layer_idx, mask)
-            if live is not None:
                 k, v = k[live], v[live]
-            _CUDA.append_kv_i8(**spec, layer_idx=layer_idx, k=k, v=v, new_indptr=starts, max_new=T)
+            _CUDA.append_kv_i8(**self._spec, layer_idx=layer_idx, k=k, v=v, new_indptr=starts, max_new=T)
         except BaseException:   # refused: no tokens came in
             self._undone(length, held)
             raise
@@ -210,17 +213,16 @@ class MultiLayerPagedKVCache8Bit(Cache):
             raise ValueError("update_qkv() takes a prompt without padding")
         if attention_mask is not None:
             self._check_mask(attention_mask, T, layer_idx)
-            if self._live_rows(attention_mask, T)[0] is not None:
-                raise ValueError("update_qkv() takes new tokens without padding")
         if tuple(cos.shape) not in ((1, T, 128), (B, T, 128)) or cos.shape != sin.shape:
             raise ValueError(f"cos / sin must be [1 or {B}, {T}, 128]")
         rows = [t.reshape(T, 128) if B == 1 or (T == 1 and t.shape[0] == 1)
                 else t.expand(B, T, 128).reshape(B * T, 128) for t in (cos, sin)]
         length, held = self.length, self._held
         try:
-            spec = self._step(T, layer_idx, attention_mask)
+            if not self._step(T, layer_idx, attention_mask):
+                raise ValueError("update_qkv() takes new tokens without padding")
             q = _CUDA.qkv_norm_rope_append_i8(
-                **spec, layer_idx=layer_idx, qkv=qkv.reshape(B * T, -1), cos=rows[0].contiguous(),
+                **self._spec, layer_idx=layer_idx, qkv=qkv.reshape(B * T, -1), cos=rows[0].contiguous(),
                 sin=rows[1].contiguous(), n_q_heads=num_q_heads, q_weight=q_weight,
                 k_weight=k_weight, eps=eps, new_indptr=self._starts(T), max_new=T)
         except BaseException:
@@ -278,7 +280,7 @@ class MultiLayerPagedKVCache8Bit(Cache):
 
     def get_cache_specs_for_flash_infer(self, attention_mask):
         if attention_mask is not None:
-            self._set_table(attention_mask.sum(dim=-1, keepdim=True, dtype=torch.int32))
+            self._set_table(attention_mask.sum(dim=-1, dtype=torch.int32))
         elif not self._frozen:
             self._set_table(self.length)
         return self._spec
