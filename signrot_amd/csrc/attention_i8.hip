@@ -20,9 +20,14 @@
 // the code itself, exactly.  Scales never touch the codes: K's multiplies the
 // scores of its block of 16 tokens, and V's goes into the exponent,
 //   p' = exp2(s ks c + log2 vs - m),   O = sum p' code,   l = sum p' / vs,
-// so out = O / l with codes as integers throughout.  p' is rounded to fp16 for
-// the product; m (the running maximum of the exponent) moves only when a score
-// exceeds it by more than 8, so p' <= 2^8.
+// so out = O / l with codes as integers throughout.  m (the running maximum of
+// the exponent) moves only when a score exceeds it by more than 8, so p' <= 2^8.
+// p' is rounded to fp16 for the second product, the one rounding to 16 bits before
+// the output's: 2.4e-4 to 2.9e-4 from 64 bits where the output's alone leaves
+// 2.1e-4.  The rest of p' as a second fp16 operand would leave 2.1e-4 too; it
+// doubles that product, 45.2 -> 46.4 us for the decode batch below and 181 -> 233 us
+// for pieces of a prompt, and was not taken.  (Scores are summed over codes + 128,
+// whose part 128 sum(q) is taken out in fp32: far below either.)
 //
 // The waves of a block take 32-token tiles in turn and are joined through LDS;
 // a request is split over blocks (chunks) when there are few, whose partial
@@ -410,8 +415,8 @@ __global__ __launch_bounds__(kWaves * 64, 2) void attn_i8_kernel(AttnI8Args a, P
 // scales reach the scores as above, and P^T is the second product's operand
 // straight from registers.  V's operand comes from the transposing LDS read.
 // 3125 to 5000 cached and 320 to 512 new tokens of 4 requests, 32 / 8 heads, 120
-// GFLOP: 180 us, 0.66 PFLOP/s, bound by the instructions of a wave (2250 of its 4760
-// cycles a tile issue one) and by uneven requests.
+// GFLOP: 180 us, 0.66 PFLOP/s, bound by the instructions of a wave (535 a tile: 2290
+// of its 4750 cycles issue one, 1440 wait to) and by uneven requests.
 constexpr int KT = 64;
 constexpr int kRowsBlock = 32 * kWaves;
 constexpr int KS = kI8D + 8;     // row strides in halves: 16-byte reads of K and the

@@ -25,9 +25,9 @@
 // without being a tie.
 //
 // A wave's chain of dependent loads bounds it (row index, table, block, scale), and
-// with many tokens HBM: 6500 tokens of 8 heads, 40 MB, 12.8 us, 3.1 TB/s; one token
-// for each of 32 requests 4.5 us, of 16 with norm and rotation 5.8; 2048 tokens
-// with them and 32 query heads, 47 MB, 13.0 us, 3.6 TB/s.
+// with many tokens HBM: 6500 tokens of 8 heads, 40 MB, 12.6 us, 3.2 TB/s; one token
+// for each of 32 requests 4.5 us, of 16 with norm and rotation 5.6; 2048 tokens
+// with them and 32 query heads, 49 MB, 13.6 us, 3.6 TB/s.
 #include "kv_i8.h"
 #include "qk_norm.h"
 

@@ -159,8 +159,9 @@ class GroupLinear4bit(torch.nn.Module):
     gradient or carries a tangent, or one on the host are a matrix product with the
     dequantized weight."""
 
-    # us on one MI355X, w4a16_linear against dequantization and product: 512 rows
-    # through 4096 x 4096 85 / 231, 8192 x 28672 902 / 3409, 28672 x 4096 611 / 1569
+    # us on one MI355X, w4a16_linear against dequantization and product, 512 / 1024 /
+    # 2048 rows: 4096 x 4096 95 : 242, 179 : 247, 314 : 276; 8192 x 28672 907 : 3424, 1700 :
+    # 3476, 3359 : 3770; 28672 x 4096 609 : 1586, 1181 : 1658, 2352 : 1819
     MAX_ROWS = 1024
 
     weight: torch.Tensor

@@ -9,9 +9,8 @@ token and head for K and V together against the int4 cache's 136.  Tokens that c
 one at a time are kept less exactly than a prompt's: each growth of the open block's
 scale rounds its older codes again (normal values: 25% more rms error than in one
 piece), so what the cache holds depends on how the tokens were cut into calls.  The
-page table
-is the int4 cache's (request b's page j is page j * B + b), and so are the protocol
-of update() and that of graph capture.  Differences:
+page table is the int4 cache's (request b's page j is page j * B + b), and so are the
+protocol of update() and that of graph capture.  Differences:
   * update() takes any number of tokens after the prefill (a prompt's next piece,
     tokens to be verified), and its attention as many queries, causally.
   * update_qkv() is update() from the q/k/v projection output with the q/k norms
