@@ -385,6 +385,8 @@ class MultiLayerPagedKVCache4Bit(Cache):
             raise ValueError(f"update() takes the {self.num_heads} KV heads, got {H}")
         if B != self.batch_size:
             raise ValueError(f"batch {B} != the cache's {self.batch_size}")
+        if self._filled[layer_idx] and T != 1:
+            raise ValueError("after the prefill, update() appends one token per request")
         mask = (cache_kwargs or {}).get("attention_mask")
         kq, kp, vq, vp = self._quantize(key_states, value_states)
         if layer_idx == 0:
@@ -406,8 +408,6 @@ class MultiLayerPagedKVCache4Bit(Cache):
             init_kv_i4(**spec, k=kq.contiguous(), v=vq.contiguous(), k_param=kp.contiguous(),
                        v_param=vp.contiguous(), seqlen_indptr=starts, layer_idx=layer_idx)
             return key_states, value_states
-        if T != 1:
-            raise ValueError("after the prefill, update() appends one token per request")
         append_kv_i4(**spec, k=kq.view(B, H, D // 2), v=vq.view(B, H, D // 2),
                      k_param=kp.view(B, H, 2), v_param=vp.view(B, H, 2), layer_idx=layer_idx)
         return _LayerAttention(self._decoder, spec, layer_idx)
