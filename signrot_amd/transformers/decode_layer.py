@@ -32,7 +32,7 @@ def _refuse_held(cache, layer_idx, tokens):
     """A prefill's refusal of a layer that has its context, ahead of the update()
     that would store its tokens behind it (an update() that is not the caches' own
     is asked itself)."""
-    cache = cache.inner if isinstance(cache, HFCacheAdapter) else cache
+    cache = cache.inner if type(cache) is HFCacheAdapter else cache
     own = getattr(getattr(cache, "update", None), "__func__", None)
     if own not in (MultiLayerPagedKVCache4Bit.update, MultiLayerPagedKVCache8Bit.update) or \
             not cache._filled[layer_idx]:

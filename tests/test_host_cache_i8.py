@@ -258,3 +258,31 @@ def test_softmax_scales_are_checked_when_the_cache_is_made(sm):
         MultiLayerPagedKVCache8Bit(1, 16, 16, "cpu", 1, 1, D, softmax_scale=sm)
     for ok in (None, 0.0, 2.0 ** -20, -0.125, 2.0 ** 60):
         MultiLayerPagedKVCache8Bit(1, 16, 16, "cpu", 1, 1, D, softmax_scale=ok)
+
+
+def test_who_refuses_a_second_prefill():
+    """The layer for the caches' own update(), also behind the adapter; an update() that
+    a program has put in place is asked itself."""
+    from signrot_amd.transformers import HFCacheAdapter
+    from signrot_amd.transformers.decode_layer import _refuse_held
+
+    class Rewinds(HFCacheAdapter):
+        def update(self, *args):
+            self.inner.reset()
+            return super().update(*args)
+
+    class Own(MultiLayerPagedKVCache8Bit):
+        def update(self, *args):
+            return super().update(*args)
+
+    cache, own = _cache(1), Own(1, 16, 64, "cpu", 1, 2, D)
+    for c in (cache, HFCacheAdapter(cache), own):
+        _refuse_held(c, 0, 4)
+    k = _rand(1, 1, 4, 2, D)
+    for c in (cache, own):
+        c.update(k, k, 0)
+    for c in (cache, HFCacheAdapter(cache)):
+        with pytest.raises(RuntimeError, match="already holds"):
+            _refuse_held(c, 0, 4)
+    for c in (own, Rewinds(cache), object()):
+        _refuse_held(c, 0, 4)
