@@ -172,16 +172,16 @@ class _PageTable:
     def set_lengths(self, lens, page_size: int, beside=None):
         """Lengths int32 [B]; every request must need the same number of pages
         (read on the host, in one transfer, and with them `beside`, another int32
-        [B], which is returned)."""
-        host = (lens if beside is None else torch.stack((lens, beside))).cpu().numpy()
-        pages = _pages_for(host if beside is None else host[0], page_size)
+        [B]).  Returns what the host has read, [1 or 2, B]."""
+        host = torch.stack((lens,) if beside is None else (lens, beside)).cpu().numpy()
+        pages = _pages_for(host[0], page_size)
         lo, hi = int(pages.min()), int(pages.max())
         if lo != hi:
             raise NotImplementedError("Current implementation does not support the case where "
                                       "batches have different number of pages")
         self.last.copy_(torch.where(lens > 0, (lens - 1) % page_size + 1, 0))
         self.set_pages(lo)
-        return None if beside is None else host[1]
+        return host
 
     def clone(self):
         t = _PageTable.__new__(_PageTable)

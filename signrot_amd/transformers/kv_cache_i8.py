@@ -88,13 +88,16 @@ class MultiLayerPagedKVCache8Bit(Cache):
 
     def _set_table(self, held, beside=None):
         """Index tensors of `held` tokens per request: one number, or int32 [B] (which
-        the host reads, and `beside` with them).  They stay as they were where that is
-        refused."""
+        the host reads and returns, and `beside` with them).  They stay as they were
+        where that is refused."""
         was, self._held = self._held, held
         try:
             if isinstance(held, int):
                 return self._table.set_uniform(held, self.page_size)
-            return self._table.set_lengths(held, self.page_size, beside)
+            host = self._table.set_lengths(held, self.page_size, beside)
+            if (host[0] == self.length).all():   # no padding: as without a mask
+                self._held = self.length
+            return host
         except BaseException:
             if self._held is not was:
                 self._set_table(was)
@@ -124,6 +127,8 @@ class MultiLayerPagedKVCache8Bit(Cache):
         return whether the mask counts all of the new ones.  Frozen index tensors say
         themselves where the tokens go, within the pool that they were made for: it
         keeps its place then, as a captured step needs."""
+        if mask is None and not self._frozen and self.length and not isinstance(self._held, int):
+            raise ValueError("the cache holds padded requests: their attention_mask is needed")
         if layer_idx == 0:
             if not self._frozen:
                 self._reserve(self.length + tokens)
@@ -132,7 +137,7 @@ class MultiLayerPagedKVCache8Bit(Cache):
             self.get_cache_specs_for_flash_infer(None)
             return True
         new = mask[:, mask.shape[1] - tokens:].sum(dim=-1, dtype=torch.int32)
-        return bool((self._set_table(mask.sum(dim=-1, dtype=torch.int32), new) == tokens).all())
+        return bool((self._set_table(mask.sum(dim=-1, dtype=torch.int32), new)[1] == tokens).all())
 
     def _undone(self, length, held):
         """After a refused call: length and index tensors as before it."""
@@ -168,7 +173,8 @@ class MultiLayerPagedKVCache8Bit(Cache):
         append T tokens per request and return the attention over the cache, a
         callable that takes their queries [B, T, Hq, 128].  With an attention_mask (in
         later calls the one of all tokens so far, its last T columns the new ones)
-        only its 1-positions are stored; a 0-position's attention is 0."""
+        only its 1-positions are stored; a 0-position's attention is 0.  Padded requests
+        go on with their mask."""
         B, T, H, D = key_states.shape
         if H != self.num_heads:
             raise ValueError(f"update() takes the {self.num_heads} KV heads, got {H}")
@@ -186,7 +192,8 @@ class MultiLayerPagedKVCache8Bit(Cache):
             else:
                 live, starts = self._live_rows(mask, T)
                 k, v = k[live], v[live]
-            _CUDA.append_kv_i8(**self._spec, layer_idx=layer_idx, k=k, v=v, new_indptr=starts, max_new=T)
+            _CUDA.append_kv_i8(**self._spec, layer_idx=layer_idx, k=k, v=v, new_indptr=starts,
+                               max_new=T)
         except BaseException:   # refused: no tokens came in
             self._undone(length, held)
             raise
@@ -221,9 +228,10 @@ class MultiLayerPagedKVCache8Bit(Cache):
             if not self._step(T, layer_idx, attention_mask):
                 raise ValueError("update_qkv() takes new tokens without padding")
             q = _CUDA.qkv_norm_rope_append_i8(
-                **self._spec, layer_idx=layer_idx, qkv=qkv.reshape(B * T, -1), cos=rows[0].contiguous(),
-                sin=rows[1].contiguous(), n_q_heads=num_q_heads, q_weight=q_weight,
-                k_weight=k_weight, eps=eps, new_indptr=self._starts(T), max_new=T)
+                **self._spec, layer_idx=layer_idx, qkv=qkv.reshape(B * T, -1),
+                cos=rows[0].contiguous(), sin=rows[1].contiguous(), n_q_heads=num_q_heads,
+                q_weight=q_weight, k_weight=k_weight, eps=eps, new_indptr=self._starts(T),
+                max_new=T)
         except BaseException:
             self._undone(length, held)
             raise
@@ -252,8 +260,8 @@ class MultiLayerPagedKVCache8Bit(Cache):
             raise RuntimeError("update_qkv_decode_quant: the layer has no prefill yet")
         if not 0 < num_q_heads <= 64 or num_q_heads & (num_q_heads - 1) or \
                 num_q_heads % self.num_heads:
-            raise RuntimeError(f"update_qkv_decode_quant: {num_q_heads} query heads must be a power "
-                               f"of two <= 64 and a multiple of the {self.num_heads} KV heads")
+            raise RuntimeError(f"update_qkv_decode_quant: {num_q_heads} query heads must be a "
+                               f"power of two <= 64, a multiple of the {self.num_heads} KV heads")
         B = qkv.shape[0]
         q = self.update_qkv(qkv.view(B, 1, -1), cos, sin, layer_idx, num_q_heads, q_weight,
                             k_weight, eps, attention_mask)

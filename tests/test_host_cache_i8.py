@@ -286,3 +286,40 @@ def test_who_refuses_a_second_prefill():
             _refuse_held(c, 0, 4)
     for c in (own, Rewinds(cache), object()):
         _refuse_held(c, 0, 4)
+
+
+@pytest.mark.parametrize("pads", [(0, 5), (3, 3)])
+def test_padded_requests_go_on_with_their_mask(pads):
+    """Without it every request would count as long as the padded prompt, and what lies
+    behind the shorter ones is nothing that was stored; a mask of ones may be left out."""
+    B = 2
+    k, q = _rand(1, B, 14, 2, D), _rand(2, B, 1, 4, D)
+    cos = torch.ones(1, 1, D, dtype=torch.float16)
+    mask = torch.ones(B, 14, dtype=torch.int64)
+    whole = _cache(B, layers=2)
+    for layer in range(2):
+        whole.update(k, k, layer, {"attention_mask": mask})
+    plain = _cache(B, layers=2)
+    for layer in range(2):
+        plain.update(k, k, layer)
+    outs = [c.update(k[:, :1], k[:, :1], 0)(q) for c in (whole, plain)]
+    assert torch.equal(*outs)
+    for b, n in enumerate(pads):
+        mask[b, :n] = 0
+    cache = _cache(B, layers=2)
+    cache.update(k, k, 0, {"attention_mask": mask})
+    refused = (ValueError,)
+    _unchanged(cache, lambda: cache.update(k, k, 1), refused)
+    cache.update(k, k, 1, {"attention_mask": mask})
+    _unchanged(cache, lambda: cache.update(k[:, :1], k[:, :1], 0), refused)
+    _unchanged(cache, lambda: cache.update_qkv(_rand(3, B, 1, 8 * D), cos, cos, 0, 4), refused)
+    longer = torch.cat([mask, torch.ones(B, 1, dtype=torch.int64)], 1)
+    cache.update(k[:, :1], k[:, :1], 0, {"attention_mask": longer})
+    assert [h.shape[2] for h in _held(cache)] == [15 - n for n in pads]
+    # its own index tensors while frozen, and a fresh start after reset
+    cache.freeze_specs(True)
+    cache.update(k[:, :1], k[:, :1], 1)
+    cache.reset()
+    cache.freeze_specs(False)
+    cache.update(k, k, 0)
+    assert [h.shape[2] for h in _held(cache)] == [14, 14]
