@@ -770,6 +770,54 @@ int srq_w4a16_linear(const void *x, const void *w, const void *scales, const voi
                      const void *bias, int64_t M, int64_t N, int64_t K, int64_t group, void *out,
                      void *stream);
 
+/* Rows to int8 codes with one fp32 scale each, behind the residual's addition and an
+ * RMSNorm:
+ *   h = fp16(x + residual)   (h = x with residual NULL), stored to sum unless NULL
+ *   y = h / sqrt(sum h^2 / mean_dim + eps) * weight      (weight NULL: 1)
+ *   scale = fp32(clip_ratio max|y| / 127),  q = clamp(rne(y / scale), -127, 127)
+ * codes and scales those of 64-bit arithmetic; norm (or NULL) receives fp16(y).  x,
+ * residual f16 [rows, cols] with row strides in elements, weight f16 [cols], sum and
+ * norm f16 [rows, cols], q i8 [rows, cols], scale f32 [rows], all dense.  sum may be x
+ * or residual.  A row of zeros has scale 0 and codes 0; one that holds a NaN or an
+ * infinity has scale NaN and codes 0.  0 < clip_ratio <= 1.  No counterpart in the
+ * reference, whose activations have 4 bits (fused.cu:68-138, 278-309).
+ * srq_sym_quant_dynamic_i8 is the same without addition and norm (y = x). */
+int srq_rmsnorm_quant_i8(const void *x, int64_t x_stride, const void *residual,
+                         int64_t res_stride, const void *weight, int64_t rows, int64_t cols,
+                         double eps, int64_t mean_dim, double clip_ratio, void *sum, void *norm,
+                         void *q, void *scale, void *stream);
+int srq_sym_quant_dynamic_i8(const void *x, int64_t x_stride, int64_t rows, int64_t cols,
+                             double clip_ratio, void *q, void *scale, void *stream);
+
+/* int8 rows through packed int4 weights with a scale per output channel:
+ *   out[m, n] = fp16(sum_k a[m, k] w[n, k] * a_scale[m] * w_scale[n] (+ bias[n])
+ *                    (+ residual[m, n]))
+ * the sum exact, the rest fp32 with one rounding.  a i8 [M, K], a_scale f32 [M], w u8
+ * [N, K / 2] (srq_w4a4_linear's layout), w_scale f16 [N], bias f16 [N] or NULL,
+ * residual f16 [M, N] or NULL (may be out), out f16 [M, N].  K is a multiple of 32
+ * below 131072.  ws: at least the bytes that ..._workspace gives, 16-byte aligned (0:
+ * any, or none). */
+int srq_w4a8_linear(const void *a, const void *a_scale, const void *w, const void *w_scale,
+                    const void *bias, const void *residual, int64_t M, int64_t N, int64_t K,
+                    void *out, void *ws, int64_t ws_bytes, void *stream);
+int srq_w4a8_linear_workspace(int64_t M, int64_t N, int64_t K, int64_t *bytes);
+
+/* The low-rank adapters of a batch's tokens beside a projection that they share:
+ *   out[m, n] = fp16(y[m, n] + scaling[i] sum_j (sum_k x[m, k] A[i, s r + j, k]) B[i, n, j])
+ * with i = ids[m] and s the column slice of n: slice_cols[0 .. slices) (on the host)
+ * divide the N columns, each slice with r rows of A of its own.  x f16 [M, K], y and out
+ * f16 [M, N] (row strides in elements; out may be y), lora_a f16 [adapters, slices r, K],
+ * lora_b f16 [adapters, N, r], ids int32 [M], scaling f32 [adapters] or NULL (1).  A token
+ * whose id lies outside [0, adapters) keeps y.  Sums in fp32, one rounding.  r is a
+ * multiple of 8 up to 256, K one of 8, at most 8 slices; x (rows too) and the adapters
+ * are 16-byte aligned.  ws: the bytes of srq_lora_workspace, 16-byte aligned. */
+int srq_lora_add(const void *y, int64_t y_stride, const void *x, int64_t x_stride,
+                 const void *lora_a, const void *lora_b, const int32_t *ids, const float *scaling,
+                 int64_t M, int64_t K, int64_t adapters, int64_t rank, int64_t slices,
+                 const int64_t *slice_cols, void *out, int64_t out_stride, void *ws,
+                 int64_t ws_bytes, void *stream);
+int srq_lora_workspace(int64_t M, int64_t K, int64_t rank, int64_t slices, int64_t *bytes);
+
 #ifdef __cplusplus
 }
 #endif

@@ -29,6 +29,9 @@ Added ops for models and formats that the reference does not serve:
   qk_norm_rope, append_kv_i8, qkv_norm_rope_append_i8, batch_attention_i8: q/k
   norms, and a paged int8 KV cache with a scale per block of 16 tokens and head
   w4a16_linear: fp16 activations through 4-bit weights with group scales
+  rmsnorm_quant_i8, sym_quant_dynamic_i8, w4a8_linear: 8-bit activations through
+  the int4 weights of w4a4_linear
+  lora_add: the low-rank adapters of a batch's requests beside a shared projection
 """
 import ctypes
 import functools
@@ -1185,6 +1188,179 @@ def w4a16_linear(x, w, scales, zeros=None, bias=None):
     out = torch.empty((*x.shape[:-1], N), dtype=f16, device=x.device)
     _call_on(x, "srq_w4a16_linear", _ptr(x), _ptr(w), _ptr(scales), _ptr(zeros), _ptr(bias), M, N,
              K, K // groups, _ptr(out), _stream(x))
+    return out
+
+
+def _row_view(name, t, tname, n):
+    """Rows and their stride of t [..., n], dense in its last dim and evenly spaced
+    in the others."""
+    if t.dim() < 1 or t.shape[-1] != n:
+        raise RuntimeError(f"{name}: '{tname}' must be [..., {n}], got {tuple(t.shape)}")
+    rows = t.numel() // n if n else 0
+    if rows == 0:
+        return 0, n
+    if n > 1 and t.stride(-1) != 1:
+        raise RuntimeError(f"{name}: '{tname}' must be dense in its last dimension")
+    step, want = n, None   # rows next to each other unless there are two
+    for size, stride in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+        if size == 1:
+            continue
+        if want is None:
+            step = stride
+        elif stride != want:
+            raise RuntimeError(f"{name}: the rows of '{tname}' must be evenly spaced")
+        want = stride * size
+    return rows, step
+
+
+# ------------------------------------------------------- 8-bit activations
+
+def rmsnorm_quant_i8(x, eps, mean_dim=None, residual=None, weight=None, clip_ratio=1.0,
+                     return_norm=False, out=None):
+    """The residual's addition, RMSNorm and int8 quantization in one launch:
+    h = fp16(x + residual), y = h / sqrt(sum h^2 / mean_dim + eps) * weight, scale =
+    fp32(clip_ratio max|y| / 127), q = clamp(rne(y / scale), -127, 127), codes and
+    scales as in 64-bit arithmetic.  Returns (q i8 [..., n], scale f32 [..., 1]), then h
+    where a residual is given (written to `out`, which may be x or residual), then with
+    return_norm fp16 y.  x and residual fp16 [..., n] of any length, rows evenly spaced;
+    weight fp16 [n] or None; mean_dim None is n.  A row with a NaN or an infinity has
+    scale NaN and codes 0."""
+    res = _host.rmsnorm_quant_i8(x, eps, mean_dim, residual, weight, clip_ratio, return_norm, out)
+    if res is not None:
+        return res
+    name, f16 = "rmsnorm_quant_i8", torch.float16
+    _check(name, [(x, "x"), (residual, "residual")], [f16, f16], contiguous=False)
+    _check(name, [(weight, "weight"), (out, "out")], [f16, f16])
+    _check(name, [(x, "x"), (weight, "weight"), (out, "out")], contiguous=False)
+    if x.dim() < 1:
+        raise RuntimeError(f"{name}: x must be [..., n]")
+    n = x.shape[-1]
+    rows, xs = _row_view(name, x, "x", n)
+    rs = 0
+    if residual is not None:
+        if residual.shape != x.shape:
+            raise RuntimeError(f"{name}: residual must have x's shape {tuple(x.shape)}")
+        rs = _row_view(name, residual, "residual", n)[1]
+    if weight is not None and (weight.dim() != 1 or weight.shape[0] != n):
+        raise RuntimeError(f"{name}: weight must be [{n}]")
+    if out is not None and (residual is None or out.shape != x.shape):
+        raise RuntimeError(f"{name}: out takes the sum with a residual, of x's shape")
+    q = torch.empty(x.shape, dtype=torch.int8, device=x.device)
+    scale = torch.empty((*x.shape[:-1], 1), dtype=torch.float32, device=x.device)
+    h = out
+    if residual is not None and out is None:
+        h = torch.empty(x.shape, dtype=f16, device=x.device)
+    y = torch.empty(x.shape, dtype=f16, device=x.device) if return_norm else None
+    _call_on(x, "srq_rmsnorm_quant_i8", _ptr(x), xs, _ptr(residual), rs, _ptr(weight), rows, n,
+             float(eps), n if mean_dim is None else int(mean_dim), float(clip_ratio), _ptr(h),
+             _ptr(y), _ptr(q), _ptr(scale), _stream(x))
+    return (q, scale) + ((h,) if residual is not None else ()) + ((y,) if return_norm else ())
+
+
+def sym_quant_dynamic_i8(x, clip_ratio=1.0):
+    """Per-row int8 codes and fp32 scales of fp16 x [..., n] (rows evenly spaced): (q i8
+    [..., n], scale f32 [..., 1]); scale = fp32(clip_ratio max|x| / 127), q = clamp(rne(x /
+    scale), -127, 127), as in exact arithmetic."""
+    res = _host.sym_quant_dynamic_i8(x, clip_ratio)
+    if res is not None:
+        return res
+    name = "sym_quant_dynamic_i8"
+    _check(name, [(x, "x")], [torch.float16], contiguous=False)
+    if x.dim() < 1:
+        raise RuntimeError(f"{name}: x must be [..., n]")
+    n = x.shape[-1]
+    rows, xs = _row_view(name, x, "x", n)
+    q = torch.empty(x.shape, dtype=torch.int8, device=x.device)
+    scale = torch.empty((*x.shape[:-1], 1), dtype=torch.float32, device=x.device)
+    _call_on(x, "srq_sym_quant_dynamic_i8", _ptr(x), xs, rows, n, float(clip_ratio), _ptr(q),
+             _ptr(scale), _stream(x))
+    return q, scale
+
+
+def w4a8_linear(A, a_scale, B, b_scale, bias=None, residual=None, out=None):
+    """int8 rows A [..., K] (scales fp32, one a row) through packed int4 weights B u8
+    [N, K/2] with scales fp16 [N]: out f16 [..., N] = A B^T a_scale b_scale (+ bias) (+
+    residual), the product exact in int32, the rest in fp32 with one rounding.  `out` may
+    be `residual`.  K a multiple of 32 below 131072."""
+    res = _host.w4a8_linear(A, a_scale, B, b_scale, bias, residual, out)
+    if res is not None:
+        return res
+    name, f16 = "w4a8_linear", torch.float16
+    _check(name, [(A, "A"), (a_scale, "a_scale"), (B, "B"), (b_scale, "b_scale"), (bias, "bias"),
+                  (residual, "residual"), (out, "out")],
+           [torch.int8, torch.float32, torch.uint8, f16, f16, f16, f16])
+    if A.dim() < 1 or B.dim() != 2 or A.shape[-1] != 2 * B.shape[1]:
+        raise RuntimeError(f"{name}: expected A [..., K] and B [N, K/2], got {tuple(A.shape)} and "
+                           f"{tuple(B.shape)}")
+    N, K = B.shape[0], B.shape[1] * 2
+    M = A.numel() // K if K else 0
+    shape = (*A.shape[:-1], N)
+    if a_scale.numel() != M or b_scale.numel() != N:
+        raise RuntimeError(f"{name}: a_scale must have a value a row and b_scale N")
+    if bias is not None and bias.numel() != N:
+        raise RuntimeError(f"{name}: bias must have N elements")
+    for t, tname in ((residual, "residual"), (out, "out")):
+        if t is not None and tuple(t.shape) != shape:
+            raise RuntimeError(f"{name}: {tname} must be {shape}, got {tuple(t.shape)}")
+    if out is None:
+        out = torch.empty(shape, dtype=f16, device=A.device)
+    wb = ctypes.c_int64()
+    _call("srq_w4a8_linear_workspace", M, N, K, ctypes.byref(wb))
+    ws = torch.empty(wb.value, dtype=torch.uint8, device=A.device) if wb.value else None
+    _call_on(A, "srq_w4a8_linear", _ptr(A), _ptr(a_scale), _ptr(B), _ptr(b_scale), _ptr(bias),
+             _ptr(residual), M, N, K, _ptr(out), _ptr(ws), wb.value, _stream(A))
+    return out
+
+
+# ------------------------------------------------------- low-rank adapters
+
+def lora_add(y, x, lora_a, lora_b, ids, scaling=None, slices=None, out=None):
+    """The low-rank adapters of a batch's tokens beside a projection that they share: out
+    = y + scaling[i] (x A_i^T) B_i^T for each token's own i = ids[token].  y fp16 [..., N]
+    is the projection's output for x fp16 [..., K]; lora_a fp16 [adapters, S r, K], lora_b
+    fp16 [adapters, N, r], ids int32 [tokens], scaling fp32 [adapters] (None: 1).  slices
+    (None: one) are the widths of the column slices of a projection that is several in
+    one: slice s meets the s-th r rows of A.  A token whose id lies outside [0, adapters)
+    keeps y.  fp32 sums, one rounding.  Returns out (dense and new, or given: `out` may be
+    y).  Rows of y, x and out are evenly spaced; r is a multiple of 8 up to 256, K one of 8.
+    Made for tokens of a request that stand together; any order is correct."""
+    res = _host.lora_add(y, x, lora_a, lora_b, ids, scaling, slices, out)
+    if res is not None:
+        return res
+    name, f16 = "lora_add", torch.float16
+    _check(name, [(y, "y"), (x, "x"), (out, "out")], [f16] * 3, contiguous=False)
+    _check(name, [(lora_a, "lora_a"), (lora_b, "lora_b"), (ids, "ids"), (scaling, "scaling")],
+           [f16, f16, torch.int32, torch.float32])
+    _check(name, [(y, "y"), (lora_a, "lora_a"), (ids, "ids")], contiguous=False)
+    if lora_a.dim() != 3 or lora_b.dim() != 3 or lora_a.shape[0] != lora_b.shape[0]:
+        raise RuntimeError(f"{name}: expected lora_a [adapters, S r, K] and lora_b [adapters, N, r]")
+    L, R, K = lora_a.shape
+    N, r = lora_b.shape[1:]
+    widths = (N,) if slices is None else tuple(int(v) for v in slices)
+    if sum(widths) != N or R != len(widths) * r:
+        raise RuntimeError(f"{name}: {len(widths)} slices {widths} of rank {r} do not fit lora_a "
+                           f"{tuple(lora_a.shape)} and lora_b {tuple(lora_b.shape)}")
+    if x.dim() < 1 or y.shape[:-1] != x.shape[:-1]:
+        raise RuntimeError(f"{name}: y and x must have the same tokens, got {tuple(y.shape)} and "
+                           f"{tuple(x.shape)}")
+    M, xs = _row_view(name, x, "x", K)
+    rows, ys = _row_view(name, y, "y", N)
+    if ids.dim() != 1 or ids.numel() != rows:
+        raise RuntimeError(f"{name}: ids must be [{rows}], one a token")
+    if scaling is not None and (scaling.dim() != 1 or scaling.numel() != L):
+        raise RuntimeError(f"{name}: scaling must be [{L}]")
+    if out is None:
+        out = torch.empty(y.shape, dtype=f16, device=y.device)
+    elif out.shape != y.shape:
+        raise RuntimeError(f"{name}: out must have y's shape {tuple(y.shape)}")
+    os = _row_view(name, out, "out", N)[1]
+    cols = (ctypes.c_int64 * len(widths))(*widths)
+    wb = ctypes.c_int64()
+    _call("srq_lora_workspace", M, K, r, len(widths), ctypes.byref(wb))
+    ws = torch.empty(wb.value, dtype=torch.uint8, device=y.device)
+    _call_on(y, "srq_lora_add", _ptr(y), ys, _ptr(x), xs, _ptr(lora_a), _ptr(lora_b), _ptr(ids),
+             _ptr(scaling), M, K, L, r, len(widths), cols, _ptr(out), os, _ptr(ws), wb.value,
+             _stream(y))
     return out
 
 

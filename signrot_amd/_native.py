@@ -15,6 +15,7 @@ HOST_PATH = LIB_PATH.with_name("srq_host.so")
 _i64 = ctypes.c_int64
 _i32 = ctypes.c_int
 _f32 = ctypes.c_float
+_f64 = ctypes.c_double
 _p = ctypes.c_void_p
 
 # name -> argtypes (restype is int for all compute entry points)
@@ -98,6 +99,14 @@ SIGNATURES = {
                                _i64, _i64, _i64, _i64, _p, _i64, _i64, _f32, _p, _i64, _p],
     "srq_batch_attention_i8_workspace": [_i64, _i64, _i64, _i64, _i64, _i64, _p],
     "srq_w4a16_linear": [_p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _p, _p],
+    "srq_rmsnorm_quant_i8": [_p, _i64, _p, _i64, _p, _i64, _i64, _f64, _i64, _f64, _p, _p, _p, _p,
+                             _p],
+    "srq_sym_quant_dynamic_i8": [_p, _i64, _i64, _i64, _f64, _p, _p, _p],
+    "srq_w4a8_linear": [_p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _p, _p, _i64, _p],
+    "srq_w4a8_linear_workspace": [_i64, _i64, _i64, _p],
+    "srq_lora_add": [_p, _i64, _p, _i64, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _p, _p,
+                     _i64, _p, _i64, _p],
+    "srq_lora_workspace": [_i64, _i64, _i64, _i64, _p],
 }
 
 

@@ -1,0 +1,516 @@
+// int8 rows through 4-bit weights with a scale per output channel:
+//   out[m, n] = fp16(sum_k a[m, k] w[n, k] * sa[m] * sb[n] (+ bias[n]) (+ residual[m, n]))
+// a int8 [M, K], w packed signed int4 [N, K / 2] (element 2 j in the low nibble of byte
+// j), the sum exact in int32, the rest in fp32 with one rounding.
+// The products run on the int8 matrix instructions; a nibble becomes 16 times its code
+// by a mask (hence the shift by 4 behind the sums), and a dword of eight codes two
+// dwords in order by a shift, two masks and two byte permutes, beside which the int8
+// rows need nothing: they go from memory through LDS into the instructions as they are.
+// Both operands reach LDS by direct loads of 16 bytes a lane, whole cache lines of a
+// row, with the 16-byte chunks of a row exchanged by its number so that the reads in
+// operand order hit all banks.
+#include "common.h"
+
+namespace {
+
+constexpr uint32_t kOob = 0xFFFFFFF0u;
+constexpr int64_t kMaxK = 131071;   // 2^14 K < 2^31: the sums of 16 times the codes
+
+struct A8Args {
+    const int8_t *a;        // [M, K]
+    const float *sa;        // [M]
+    const uint8_t *w;       // [N, K / 2]
+    const f16 *sb;          // [N]
+    const f16 *bias;        // [N] or null
+    const f16 *res;         // [M, N] or null (may be out)
+    f16 *out;               // [M, N]
+    int32_t *part;          // split over K: [splits, M, N]
+    int64_t M, N, K;
+    int64_t kc;             // codes of a split (a multiple of 128), 0: not split
+};
+
+SRQ_DEV v4i mfma16x64(v4i a, v4i b, v4i c) {
+    return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0);
+}
+
+SRQ_DEV v16i mfma32x32(v4i a, v4i b, v16i c) {
+    return __builtin_amdgcn_mfma_i32_32x32x32_i8(a, b, c, 0, 0, 0);
+}
+
+// 8 codes of a dword as 16 times their values, bytes in order
+SRQ_DEV void codes8(u32 w, int &lo, int &hi) {
+    const u32 l = w << 4;
+    lo = (int)(__builtin_amdgcn_perm(w, l, 0x05010400u) & 0xF0F0F0F0u);
+    hi = (int)(__builtin_amdgcn_perm(w, l, 0x07030602u) & 0xF0F0F0F0u);
+}
+
+SRQ_DEV v4i codes16(u32 w0, u32 w1) {
+    v4i r;
+    int x, y;
+    codes8(w0, x, y);
+    r[0] = x;
+    r[1] = y;
+    codes8(w1, x, y);
+    r[2] = x;
+    r[3] = y;
+    return r;
+}
+
+SRQ_DEV float dequant(int acc16, float sa, float sb) { return (float)(acc16 >> 4) * sa * sb; }
+
+// A value that is the same in all lanes, in scalar registers (divisions and 64-bit
+// comparisons run on the vector unit, and a buffer's descriptor must be scalar).
+SRQ_DEV uint32_t uni(uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); }
+
+SRQ_DEV uint32_t rows_bytes(int64_t rows, int64_t most, int64_t stride) {
+    return uni((uint32_t)((rows < most ? rows : most) * stride));
+}
+
+SRQ_DEV uint32_t lds_addr(const void *p) {
+    return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void *)p;
+}
+
+// At most `ahead` groups of PER loads of this wave are still in flight (ahead < 8; the
+// counter goes to 63, and a smaller count waits for more).
+template <int PER>
+SRQ_DEV void wait_ahead(int ahead) {
+    switch (ahead) {
+    case 0: asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); break;
+    case 1: asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PER) : "memory"); break;
+    case 2: asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * PER) : "memory"); break;
+    case 3: asm volatile("s_waitcnt vmcnt(%0)" ::"n"(3 * PER) : "memory"); break;
+    case 4: asm volatile("s_waitcnt vmcnt(%0)" ::"n"(4 * PER < 64 ? 4 * PER : 63) : "memory"); break;
+    case 5: asm volatile("s_waitcnt vmcnt(%0)" ::"n"(5 * PER < 64 ? 5 * PER : 63) : "memory"); break;
+    case 6: asm volatile("s_waitcnt vmcnt(%0)" ::"n"(6 * PER < 64 ? 6 * PER : 63) : "memory"); break;
+    default: asm volatile("s_waitcnt vmcnt(%0)" ::"n"(7 * PER < 64 ? 7 * PER : 63) : "memory"); break;
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Up to 32 rows: the weights' bytes bound it.  A block of 8 waves takes 16 NT columns,
+// each wave an eighth of K in units of 128 codes, which it streams through its own ring
+// of S stages in LDS (AR activation rows of 128 bytes, then 16 NT weight rows of 64)
+// without a barrier; the waves' int32 sums are joined through LDS at the end.
+constexpr int W = 8;
+
+template <int AR, int NT, int S>
+__global__ __launch_bounds__(W * 64) void w4a8_stream_kernel(A8Args a) {
+    constexpr int MT = AR == 32 ? 2 : 1;
+    constexpr int kStage = AR * 128 + NT * 1024;
+    constexpr int PER = AR / 8 + NT;
+    constexpr int kPart = W * 16 * MT * 16 * NT * 4;
+    constexpr int kRing = W * S * kStage;
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[kRing > kPart ? kRing : kPart];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int64_t n0 = (int64_t)blockIdx.x * 16 * NT;
+    const int64_t KB = a.K / 2;
+    const int units = (int)((a.K + 127) / 128), per = (units + W - 1) / W;
+    const int u0 = wave * per, cnt = max(0, min(per, units - u0));
+    const __amdgpu_buffer_rsrc_t ar = make_rsrc(a.a, a.M * a.K);
+    const __amdgpu_buffer_rsrc_t br = make_rsrc(a.w + n0 * KB, rows_bytes(a.N - n0, 16 * NT, KB));
+    uint8_t *ring = smem + wave * S * kStage;
+    const uint32_t ring0 = lds_addr(ring);
+
+    // rows past M stay as LDS has them and columns past N read zeros: neither is stored.
+    // A chunk past K reads zeros on the weights' side, which cancels the other.
+    uint32_t aoff[AR / 8], boff[NT];
+    int bk;
+#pragma unroll
+    for (int i = 0; i < AR / 8; ++i) {
+        const int r = 8 * i + (lane >> 3);
+        aoff[i] = r < a.M ? (uint32_t)(r * a.K) + 16 * ((lane & 7) ^ (r & 7)) : kOob;
+    }
+    bk = 16 * ((lane & 3) ^ ((lane >> 4) & 3));
+#pragma unroll
+    for (int t = 0; t < NT; ++t) boff[t] = (uint32_t)((16 * t + (lane >> 2)) * KB) + bk;
+    auto issue = [&](int u, int slot) __attribute__((always_inline)) {
+        const uint32_t dst = ring0 + slot * kStage;
+        const uint32_t ka = (uint32_t)(u0 + u) * 128u, kb = ka / 2;
+#pragma unroll
+        for (int i = 0; i < AR / 8; ++i)
+            dma16(ar, aoff[i] == kOob ? kOob : aoff[i] + ka, dst + i * 1024);
+        const bool in = kb + bk < KB;
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+            dma16(br, in ? boff[t] + kb : kOob, dst + AR * 128 + t * 1024);
+    };
+
+    v4i acc[MT][NT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) acc[i][t] = (v4i){0, 0, 0, 0};
+    const int m = lane & 15, g = lane >> 4;
+    const int mr = AR == 8 ? m & 7 : m;   // with 8 rows staged the upper 8 results are not stored
+#pragma unroll
+    for (int p = 0; p < S - 1; ++p)
+        if (p < cnt) issue(p, p);
+    int slot = 0, free = S - 1;
+    for (int u = 0; u < cnt; ++u) {
+        // the reads of the stage that is filled next have returned
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        if (u + S - 1 < cnt) issue(u + S - 1, free);
+        wait_ahead<PER>(min(S - 1, cnt - 1 - u));
+        const uint8_t *st = ring + slot * kStage;
+        v4i av[MT][2];
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                av[i][h] = *reinterpret_cast<const v4i *>(
+                    st + (16 * i + mr) * 128 + 16 * ((2 * g + h) ^ (mr & 7)));
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const v4i w = *reinterpret_cast<const v4i *>(
+                st + AR * 128 + t * 1024 + m * 64 + 16 * (g ^ ((m >> 2) & 3)));
+            const v4i b0 = codes16((u32)w[0], (u32)w[1]), b1 = codes16((u32)w[2], (u32)w[3]);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                acc[i][t] = mfma16x64(av[i][0], b0, acc[i][t]);
+                acc[i][t] = mfma16x64(av[i][1], b1, acc[i][t]);
+            }
+        }
+        slot = slot == S - 1 ? 0 : slot + 1;
+        free = free == S - 1 ? 0 : free + 1;
+    }
+    __syncthreads();   // the rings are free (every load has been waited for)
+    int *part = reinterpret_cast<int *>(smem);
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                part[((wave * MT + i) * 16 + 4 * g + e) * (16 * NT) + 16 * t + m] = acc[i][t][e];
+    __syncthreads();
+    for (int i = threadIdx.x; i < 16 * MT * 16 * NT; i += W * 64) {
+        const int om = i / (16 * NT), on = i % (16 * NT);
+        const int64_t n = n0 + on;
+        if (om >= a.M || n >= a.N) continue;
+        int sum = 0;
+#pragma unroll
+        for (int w = 0; w < W; ++w) sum += part[w * (16 * MT * 16 * NT) + i];
+        float v = dequant(sum, a.sa[om], (float)a.sb[n]);
+        if (a.bias) v += (float)a.bias[n];
+        if (a.res) v += (float)a.res[om * a.N + n];
+        a.out[om * a.N + n] = f16_rn(v);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// More rows: tiles of BM x BN, WM x WN waves with (BM / WM) x (BN / WN) each in blocks
+// of v_mfma_i32_32x32x32_i8, K in steps of 128 codes through a ring of NSTG stages
+// (BM rows of 128 bytes, then BN rows of 64) that every wave fills with its share of
+// loads.  One barrier a step: behind it step s has landed for all and step s - 1, whose
+// stage is filled next, has been read by all.
+struct __attribute__((packed, aligned(2))) U8h { v8h v; };
+
+template <int BM, int BN, int WM, int WN, int NSTG>
+__global__ __launch_bounds__(64 * WM * WN) void w4a8_tile_kernel(A8Args a) {
+    constexpr int NW = WM * WN, FM = BM / WM / 32, FN = BN / WN / 32;
+    static_assert(FM * WM * 32 == BM && FN * WN * 32 == BN, "tile");
+    constexpr int kStage = BM * 128 + BN * 64;
+    constexpr int PA = BM / 8 / NW, PB = BN / 16 / NW, PER = PA + PB;
+    static_assert(PA * NW * 8 == BM && PB * NW * 16 == BN, "loads of a stage");
+    static_assert(NSTG >= 2 && NSTG <= 8 && (NSTG - 2) * PER <= 63, "loads in flight");
+    constexpr int kTileW = 32 * FN + 8;                 // row stride of a wave's output rows
+    constexpr int kRing = NSTG * kStage;
+    static_assert(NW * 32 * kTileW * 2 <= kRing, "output rows");
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[kRing];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+
+    // Block b runs on XCD b % 8: each XCD takes a run of tiles, rows fastest, so that
+    // the blocks which share its L2 read the same few weight panels.
+    const uint32_t tiles_m = (uint32_t)srq_cdiv(a.M, BM), total = gridDim.x;
+    const uint32_t x = blockIdx.x % 8, per = total / 8, rem = total % 8;
+    const uint32_t idx = x * per + min(x, rem) + blockIdx.x / 8;
+    const uint32_t tn = uni(idx / tiles_m);
+    const int64_t m0 = (int64_t)(idx - tn * tiles_m) * BM, n0 = (int64_t)tn * BN;
+
+    const int64_t KB = a.K / 2;
+    const int64_t k_lo = a.kc ? (int64_t)blockIdx.y * a.kc : 0;
+    const int64_t k_hi = a.kc ? min(a.K, k_lo + a.kc) : a.K;
+    const int steps = (int)((k_hi - k_lo + 127) / 128);
+    // addresses behind a tile's last row are out of the buffer's range and read zeros
+    const __amdgpu_buffer_rsrc_t ar = make_rsrc(a.a + m0 * a.K, rows_bytes(a.M - m0, BM, a.K));
+    const __amdgpu_buffer_rsrc_t br = make_rsrc(a.w + n0 * KB, rows_bytes(a.N - n0, BN, KB));
+    const uint32_t ring0 = lds_addr(smem);
+
+    uint32_t aoff[PA], boff[PB];
+#pragma unroll
+    for (int q = 0; q < PA; ++q) {
+        const int r = 8 * (q * NW + wave) + (lane >> 3);
+        aoff[q] = (uint32_t)(r * a.K + k_lo) + 16 * ((lane & 7) ^ (r & 7));
+    }
+    const int bk = 16 * ((lane & 3) ^ ((lane >> 4) & 3));
+#pragma unroll
+    for (int q = 0; q < PB; ++q)
+        boff[q] = (uint32_t)((16 * (q * NW + wave) + (lane >> 2)) * KB + k_lo / 2) + bk;
+    auto issue = [&](int s) __attribute__((always_inline)) {
+        const uint32_t dst = ring0 + (s % NSTG) * kStage + wave * 1024;
+#pragma unroll
+        for (int q = 0; q < PA; ++q) dma16(ar, aoff[q] + 128u * s, dst + q * NW * 1024);
+        // past K: zero weights cancel whatever the rows hold there
+        const bool in = k_lo / 2 + 64 * (int64_t)s + bk < KB;
+#pragma unroll
+        for (int q = 0; q < PB; ++q)
+            dma16(br, in ? boff[q] + 64u * s : kOob, dst + BM * 128 + q * NW * 1024);
+    };
+#pragma unroll
+    for (int p = 0; p < NSTG - 1; ++p)
+        if (p < steps) issue(p);
+
+    const int wm = wave / WN, wn = wave % WN;
+    const int rr = lane & 31, g = lane >> 5;
+    v16i acc[FM][FN];
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) acc[i][j] = (v16i){};
+    for (int s = 0; s < steps; ++s) {
+        wait_ahead<PER>(min(NSTG - 2, steps - 1 - s));
+        // this wave's reads of step s - 1 have returned
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        if (s + NSTG - 1 < steps) issue(s + NSTG - 1);
+        const uint8_t *sa = smem + (s % NSTG) * kStage, *sb = sa + BM * 128;
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+            v4i wv[FN];
+#pragma unroll
+            for (int j = 0; j < FN; ++j) {
+                const int r = wn * (FN * 32) + j * 32 + rr;
+                wv[j] = *reinterpret_cast<const v4i *>(sb + r * 64 + 16 * ((2 * p + g) ^ ((r >> 2) & 3)));
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                v4i av[FM];
+#pragma unroll
+                for (int i = 0; i < FM; ++i) {
+                    const int r = wm * (FM * 32) + i * 32 + rr;
+                    av[i] = *reinterpret_cast<const v4i *>(sa + r * 128 +
+                                                           16 * ((4 * p + 2 * g + h) ^ (r & 7)));
+                }
+#pragma unroll
+                for (int j = 0; j < FN; ++j) {
+                    const v4i b = codes16((u32)wv[j][2 * h], (u32)wv[j][2 * h + 1]);
+#pragma unroll
+                    for (int i = 0; i < FM; ++i) acc[i][j] = mfma32x32(av[i], b, acc[i][j]);
+                }
+            }
+        }
+    }
+
+    const int64_t mw = m0 + wm * (FM * 32), nw = n0 + wn * (FN * 32);
+    if (a.kc) {
+        int32_t *part = a.part + (int64_t)blockIdx.y * a.M * a.N;
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) {
+                const int64_t m = mw + i * 32 + 8 * (v / 4) + 4 * g + v % 4;
+#pragma unroll
+                for (int j = 0; j < FN; ++j) {
+                    const int64_t n = nw + j * 32 + rr;
+                    if (m < a.M && n < a.N) part[m * a.N + n] = acc[i][j][v];
+                }
+            }
+        return;
+    }
+    // 32 rows of the wave at a time through its own piece of LDS, so that they leave in
+    // 16 bytes a lane
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    f16 *tile = reinterpret_cast<f16 *>(smem) + wave * 32 * kTileW;
+    float sbv[FN], bv[FN];
+#pragma unroll
+    for (int j = 0; j < FN; ++j) {
+        const int64_t n = nw + j * 32 + rr;
+        sbv[j] = n < a.N ? (float)a.sb[n] : 0.f;
+        bv[j] = a.bias && n < a.N ? (float)a.bias[n] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+            const int lr = 8 * (v / 4) + 4 * g + v % 4;
+            const int64_t m = mw + i * 32 + lr;
+            const float sa = m < a.M ? a.sa[m] : 0.f;
+#pragma unroll
+            for (int j = 0; j < FN; ++j) {
+                const int64_t n = nw + j * 32 + rr;
+                float o = dequant(acc[i][j][v], sa, sbv[j]) + bv[j];
+                if (a.res && m < a.M && n < a.N) o += (float)a.res[m * a.N + n];
+                tile[lr * kTileW + j * 32 + rr] = f16_rn(o);
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        constexpr int LPR = 4 * FN, RPI = 64 / LPR;   // lanes a row, rows an instruction
+#pragma unroll
+        for (int r0 = 0; r0 < 32; r0 += RPI) {
+            const int lr = r0 + lane / LPR, c = 8 * (lane % LPR);
+            const int64_t m = mw + i * 32 + lr, n = nw + c;
+            if (m >= a.M || n >= a.N) continue;
+            const v8h o = *reinterpret_cast<const v8h *>(tile + lr * kTileW + c);
+            f16 *dst = a.out + m * a.N + n;
+            if (n + 8 <= a.N) {
+                reinterpret_cast<U8h *>(dst)->v = o;
+            } else {
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    if (n + k < a.N) dst[k] = o[k];
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    }
+}
+
+// The splits' int32 sums, joined, and the epilogue: 4 columns a thread.
+__global__ __launch_bounds__(256) void w4a8_join_kernel(A8Args a, int splits) {
+    const int64_t mn = a.M * a.N;
+    const int64_t i = 4 * ((int64_t)blockIdx.x * 256 + threadIdx.x);
+    if (i >= mn) return;
+    const int cnt = (int)min((int64_t)4, mn - i);
+    int sum[4] = {0, 0, 0, 0};
+    for (int s = 0; s < splits; ++s) {
+        const int32_t *p = a.part + s * mn + i;
+        if (cnt == 4) {
+            struct __attribute__((packed, aligned(4))) U4i { v4i v; };
+            const v4i v = reinterpret_cast<const U4i *>(p)->v;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) sum[k] += v[k];
+        } else {
+            for (int k = 0; k < cnt; ++k) sum[k] += p[k];
+        }
+    }
+    int64_t m = i / a.N, n = i % a.N;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        if (k >= cnt) break;
+        float v = dequant(sum[k], a.sa[m], (float)a.sb[n]);
+        if (a.bias) v += (float)a.bias[n];
+        if (a.res) v += (float)a.res[i + k];
+        a.out[i + k] = f16_rn(v);
+        if (++n == a.N) {
+            n = 0;
+            ++m;
+        }
+    }
+}
+
+// How a product runs, by its sizes alone.
+struct Plan {
+    int kind;        // 0: stream, else a tile form
+    int splits;      // over K (tile forms)
+    int64_t kc;
+};
+enum { kStream, k64x64, k128x64, k128x128, k256x256 };
+
+void split(Plan &p, int64_t tiles, int64_t K) {
+    const int64_t steps = srq_cdiv(K, 128);
+    int64_t s = 256 / (tiles > 0 ? tiles : 1);
+    if (s > steps / 8) s = steps / 8;   // at least 8 steps a split
+    if (s > 16) s = 16;
+    if (s < 2) return;
+    const int64_t per = srq_cdiv(steps, s);
+    p.kc = per * 128;
+    p.splits = (int)srq_cdiv(steps, per);
+    if (p.splits < 2) p = Plan{p.kind, 1, 0};
+}
+
+Plan plan_of(int64_t M, int64_t N, int64_t K) {
+    Plan p{kStream, 1, 0};
+    if (M <= 32) return p;
+    if (M > 512 && srq_cdiv(M, 256) * srq_cdiv(N, 256) >= 200) {
+        p.kind = k256x256;
+        return p;
+    }
+    if (M <= 64) {
+        p.kind = k64x64;
+        split(p, srq_cdiv(M, 64) * srq_cdiv(N, 64), K);
+        return p;
+    }
+    const int64_t t128 = srq_cdiv(M, 128) * srq_cdiv(N, 128);
+    if (t128 >= 200) {
+        p.kind = k128x128;
+        return p;
+    }
+    p.kind = k128x64;
+    split(p, srq_cdiv(M, 128) * srq_cdiv(N, 64), K);
+    return p;
+}
+
+template <int BM, int BN, int WM, int WN, int NSTG>
+void launch_tile(const A8Args &a, int splits, hipStream_t st) {
+    const dim3 grid((unsigned)(srq_cdiv(a.M, BM) * srq_cdiv(a.N, BN)), (unsigned)splits);
+    w4a8_tile_kernel<BM, BN, WM, WN, NSTG><<<grid, 64 * WM * WN, 0, st>>>(a);
+}
+
+template <int AR>
+void launch_stream(const A8Args &a, hipStream_t st) {
+    const int64_t cb = srq_cdiv(a.N, 16);
+    if (cb <= 256)
+        w4a8_stream_kernel<AR, 1, AR == 32 ? 3 : 6><<<(unsigned)cb, W * 64, 0, st>>>(a);
+    else
+        w4a8_stream_kernel<AR, 2, AR == 32 ? 3 : 4>
+            <<<(unsigned)srq_cdiv(cb, 2), W * 64, 0, st>>>(a);
+}
+
+}  // namespace
+
+extern "C" int srq_w4a8_linear_workspace(int64_t M, int64_t N, int64_t K, int64_t *bytes) {
+    SRQ_CHECK_ARG(bytes, "w4a8_linear: null pointer");
+    *bytes = 0;
+    if (M <= 0 || N <= 0 || K <= 0) return SRQ_OK;
+    const Plan p = plan_of(M, N, K);
+    if (p.kc) *bytes = 4 * p.splits * M * N;
+    return SRQ_OK;
+}
+
+extern "C" int srq_w4a8_linear(const void *a, const void *a_scale, const void *w,
+                               const void *w_scale, const void *bias, const void *residual,
+                               int64_t M, int64_t N, int64_t K, void *out, void *ws,
+                               int64_t ws_bytes, void *stream) {
+    SRQ_CHECK_ARG(M >= 0 && N >= 0 && K >= 0, "w4a8_linear: negative size");
+    SRQ_CHECK_ARG(K > 0 && K % 32 == 0, "w4a8_linear: K=%lld must be a positive multiple of 32",
+                  (long long)K);
+    SRQ_CHECK_ARG(K <= kMaxK, "w4a8_linear: K=%lld must be below 131072", (long long)K);
+    SRQ_CHECK_ARG(M <= (int64_t)1 << 31 && N <= (int64_t)1 << 31 &&
+                      srq_cdiv(M, 64) * srq_cdiv(N, 64) <= 0x7FFFFFFF / 4,
+                  "w4a8_linear: shape out of range");
+    if (M == 0 || N == 0) return SRQ_OK;
+    SRQ_CHECK_ARG(a && a_scale && w && w_scale && out, "w4a8_linear: null pointer");
+    SRQ_CHECK_ARG(srq_aligned(a, 16) && srq_aligned(w, 16),
+                  "w4a8_linear: the codes must be 16-byte aligned");
+    Plan p = plan_of(M, N, K);
+    if (p.kc)
+        SRQ_CHECK_ARG(ws && srq_aligned(ws, 16) && ws_bytes >= 4 * p.splits * M * N,
+                      "w4a8_linear: the workspace is missing or too small");
+    A8Args q{(const int8_t *)a, (const float *)a_scale, (const uint8_t *)w, (const f16 *)w_scale,
+             (const f16 *)bias, (const f16 *)residual, (f16 *)out, (int32_t *)ws, M, N, K, p.kc};
+    hipStream_t st = (hipStream_t)stream;
+    switch (p.kind) {
+    case kStream:
+        M <= 8 ? launch_stream<8>(q, st) : M <= 16 ? launch_stream<16>(q, st)
+                                                   : launch_stream<32>(q, st);
+        break;
+    case k64x64: launch_tile<64, 64, 2, 2, 6>(q, p.splits, st); break;
+    case k128x64: launch_tile<128, 64, 2, 2, 6>(q, p.splits, st); break;
+    case k128x128: launch_tile<128, 128, 2, 2, 3>(q, p.splits, st); break;
+    default: launch_tile<256, 256, 2, 4, 3>(q, 1, st); break;
+    }
+    SRQ_LAUNCH_CHECK("w4a8_linear");
+    if (p.kc) {
+        w4a8_join_kernel<<<(unsigned)srq_cdiv(M * N, 1024), 256, 0, st>>>(q, p.splits);
+        SRQ_LAUNCH_CHECK("w4a8_linear (join)");
+    }
+    return SRQ_OK;
+}

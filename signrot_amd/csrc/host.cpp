@@ -86,6 +86,11 @@ float as_float(PyObject *o) {
     return (float)as_int(o);
 }
 
+double as_double(PyObject *o) {
+    if (PyFloat_CheckExact(o)) return PyFloat_AS_DOUBLE(o);
+    return (double)as_int(o);
+}
+
 bool as_bool(PyObject *o) {
     if (!PyBool_Check(o)) throw Bad();
     return o == Py_True;
@@ -646,6 +651,189 @@ PyObject *w4a16_linear(PyObject *, PyObject *const *a, Py_ssize_t n_args) {
     });
 }
 
+// t [..., n] as rows of one spacing, dense in themselves
+void rows_view(const at::Tensor &t, int64_t &rows, int64_t &n, int64_t &step) {
+    if (t.dim() < 1 || t.numel() == 0) throw Bad();
+    n = t.size(-1);
+    rows = t.numel() / n;
+    if (n > 1 && t.stride(-1) != 1) throw Bad();
+    step = n;
+    int64_t want = -1;
+    for (int64_t d = t.dim() - 2; d >= 0; --d) {
+        if (t.size(d) == 1) continue;
+        if (want < 0) step = t.stride(d);
+        else if (t.stride(d) != want) throw Bad();
+        want = t.stride(d) * t.size(d);
+    }
+}
+
+// rmsnorm_quant_i8(x, eps, mean_dim, residual, weight, clip_ratio, return_norm, out) ->
+// (q, scale[, sum][, norm])
+PyObject *rmsnorm_quant_i8(PyObject *, PyObject *const *a, Py_ssize_t n_args) {
+    return guarded(n_args, 8, [&]() -> PyObject * {
+        const at::Tensor &x = strided(a[0], kF16);
+        const at::Device dev = x.device();
+        int64_t rows, n, xs, rs = 0;
+        rows_view(x, rows, n, xs);
+        const double eps = as_double(a[1]), clip = as_double(a[5]);
+        const int64_t mean_dim = a[2] == Py_None ? n : as_int(a[2]);
+        const bool add = a[3] != Py_None, keep = as_bool(a[6]);
+        void *res = nullptr;
+        if (add) {
+            const at::Tensor &r = strided(a[3], kF16);
+            int64_t r_rows, r_n;
+            if (r.sizes() != x.sizes() || r.device() != dev) throw Bad();
+            rows_view(r, r_rows, r_n, rs);
+            res = r.data_ptr();
+        }
+        if (a[4] != Py_None && plain(a[4], kF16).dim() != 1) throw Bad();
+        void *w = opt_ptr(a[4], kF16, n, dev);
+        at::Tensor h, q, sc, y;
+        if (a[7] != Py_None) {
+            h = plain(a[7], kF16);
+            if (!add || h.sizes() != x.sizes() || h.device() != dev) throw Bad();
+        }
+        int rc;
+        {
+            NoGil nogil;
+            const c10::DeviceGuard on(dev);
+            q = alloc(x.sizes(), kI8, dev);
+            sc = alloc(with_last(x, 1), kF32, dev);
+            if (add && !h.defined()) h = alloc(x.sizes(), kF16, dev);
+            if (keep) y = alloc(x.sizes(), kF16, dev);
+            rc = srq_rmsnorm_quant_i8(x.data_ptr(), xs, res, rs, w, rows, n, eps, mean_dim, clip,
+                                      add ? h.data_ptr() : nullptr, keep ? y.data_ptr() : nullptr,
+                                      q.data_ptr(), sc.data_ptr(), stream_of(dev));
+        }
+        check(rc, "srq_rmsnorm_quant_i8");
+        if (add && keep) return wrap({q, sc, h, y});
+        if (add) return wrap({q, sc, h});
+        if (keep) return wrap({q, sc, y});
+        return wrap({q, sc});
+    });
+}
+
+// sym_quant_dynamic_i8(x, clip_ratio) -> (q, scale)
+PyObject *sym_quant_dynamic_i8(PyObject *, PyObject *const *a, Py_ssize_t n_args) {
+    return guarded(n_args, 2, [&]() -> PyObject * {
+        const at::Tensor &x = strided(a[0], kF16);
+        const at::Device dev = x.device();
+        int64_t rows, n, xs;
+        rows_view(x, rows, n, xs);
+        const double clip = as_double(a[1]);
+        at::Tensor q, sc;
+        int rc;
+        {
+            NoGil nogil;
+            const c10::DeviceGuard on(dev);
+            q = alloc(x.sizes(), kI8, dev);
+            sc = alloc(with_last(x, 1), kF32, dev);
+            rc = srq_sym_quant_dynamic_i8(x.data_ptr(), xs, rows, n, clip, q.data_ptr(),
+                                          sc.data_ptr(), stream_of(dev));
+        }
+        check(rc, "srq_sym_quant_dynamic_i8");
+        return wrap({q, sc});
+    });
+}
+
+// w4a8_linear(A, a_scale, B, b_scale, bias, residual, out) -> out
+PyObject *w4a8_linear(PyObject *, PyObject *const *a, Py_ssize_t n_args) {
+    return guarded(n_args, 7, [&]() -> PyObject * {
+        const at::Tensor &A = plain(a[0], kI8), &B = plain(a[2], kU8);
+        const at::Device dev = A.device();
+        if (A.dim() < 1 || B.dim() != 2 || A.numel() == 0 || B.numel() == 0 || B.device() != dev)
+            throw Bad();
+        const int64_t N = B.size(0), K = 2 * B.size(1);
+        if (A.size(-1) != K) throw Bad();
+        const int64_t M = A.numel() / K;
+        void *sa = ptr(a[1], kF32, M, dev), *sb = ptr(a[3], kF16, N, dev);
+        void *bias = opt_ptr(a[4], kF16, N, dev);
+        const auto shape = with_last(A, N);
+        for (int i = 5; i < 7; ++i)
+            if (a[i] != Py_None && plain(a[i], kF16).sizes() != at::IntArrayRef(shape)) throw Bad();
+        void *res = opt_ptr(a[5], kF16, M * N, dev);
+        at::Tensor out, ws;
+        if (a[6] != Py_None) {
+            out = plain(a[6], kF16);
+            if (out.device() != dev) throw Bad();
+        }
+        int64_t wb = 0;
+        check(srq_w4a8_linear_workspace(M, N, K, &wb), "srq_w4a8_linear_workspace");
+        int rc;
+        {
+            NoGil nogil;
+            const c10::DeviceGuard on(dev);
+            if (!out.defined()) out = alloc(shape, kF16, dev);
+            if (wb > 0) ws = alloc({wb}, kU8, dev);
+            rc = srq_w4a8_linear(A.data_ptr(), sa, B.data_ptr(), sb, bias, res, M, N, K,
+                                 out.data_ptr(), wb > 0 ? ws.data_ptr() : nullptr, wb,
+                                 stream_of(dev));
+            ws.reset();
+        }
+        check(rc, "srq_w4a8_linear");
+        return wrap({out});
+    });
+}
+
+// lora_add(y, x, lora_a, lora_b, ids, scaling, slices, out) -> out
+PyObject *lora_add(PyObject *, PyObject *const *a, Py_ssize_t n_args) {
+    return guarded(n_args, 8, [&]() -> PyObject * {
+        const at::Tensor &y = strided(a[0], kF16), &x = strided(a[1], kF16);
+        const at::Tensor &la = plain(a[2], kF16), &lb = plain(a[3], kF16), &ids = plain(a[4], kI32);
+        const at::Device dev = y.device();
+        if (x.device() != dev || la.device() != dev || lb.device() != dev || ids.device() != dev ||
+            la.dim() != 3 || lb.dim() != 3 || la.size(0) != lb.size(0) || y.dim() != x.dim() ||
+            ids.dim() != 1)
+            throw Bad();
+        const int64_t L = la.size(0), R = la.size(1), K = la.size(2), N = lb.size(1);
+        const int64_t r = lb.size(2);
+        int64_t cols[8], slices = 1, sum = 0;
+        if (a[6] == Py_None) {
+            cols[0] = sum = N;
+        } else {
+            if (!PyTuple_CheckExact(a[6])) throw Bad();
+            slices = (int64_t)PyTuple_GET_SIZE(a[6]);
+            if (slices < 1 || slices > 8) throw Bad();
+            for (int64_t i = 0; i < slices; ++i) sum += cols[i] = as_int(PyTuple_GET_ITEM(a[6], i));
+        }
+        if (sum != N || R != slices * r) throw Bad();
+        int64_t M, rows, kx, ny, xs, ys, os;
+        rows_view(x, M, kx, xs);
+        rows_view(y, rows, ny, ys);
+        if (kx != K || ny != N || rows != M || ids.size(0) != M) throw Bad();
+        for (int64_t d = 0; d + 1 < y.dim(); ++d)
+            if (y.size(d) != x.size(d)) throw Bad();
+        if (a[5] != Py_None && plain(a[5], kF32).dim() != 1) throw Bad();
+        void *sc = opt_ptr(a[5], kF32, L, dev);
+        at::Tensor out, ws;
+        if (a[7] != Py_None) {
+            out = strided(a[7], kF16);
+            if (out.sizes() != y.sizes() || out.device() != dev) throw Bad();
+        }
+        int64_t wb = 0;
+        check(srq_lora_workspace(M, K, r, slices, &wb), "srq_lora_workspace");
+        if (out.defined()) {
+            int64_t o_rows, o_n;
+            rows_view(out, o_rows, o_n, os);
+        } else {
+            os = N;
+        }
+        int rc;
+        {
+            NoGil nogil;
+            const c10::DeviceGuard on(dev);
+            if (!out.defined()) out = alloc(y.sizes(), kF16, dev);
+            ws = alloc({wb}, kU8, dev);
+            rc = srq_lora_add(y.data_ptr(), ys, x.data_ptr(), xs, la.data_ptr(), lb.data_ptr(),
+                              (const int32_t *)ids.data_ptr(), (const float *)sc, M, K, L, r,
+                              slices, cols, out.data_ptr(), os, ws.data_ptr(), wb, stream_of(dev));
+            ws.reset();
+        }
+        check(rc, "srq_lora_add");
+        return wrap({out});
+    });
+}
+
 // stream(t): the current stream of the tensor's device, as an address
 PyObject *stream(PyObject *, PyObject *const *a, Py_ssize_t n_args) {
     return guarded(n_args, 1, [&]() -> PyObject * {
@@ -664,6 +852,8 @@ PyMethodDef kMethods[] = {OP(had_sign_quant),       OP(had_sign_asym_quant),
                           OP(w4a4_linear_swiglu),   OP(qk_norm_rope),
                           OP(append_kv_i8),         OP(qkv_norm_rope_append_i8),
                           OP(batch_attention_i8),   OP(w4a16_linear),
+                          OP(rmsnorm_quant_i8),     OP(sym_quant_dynamic_i8),
+                          OP(w4a8_linear),          OP(lora_add),
                           OP(stream),
                           {nullptr, nullptr, 0, nullptr}};
 

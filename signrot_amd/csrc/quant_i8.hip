@@ -1,0 +1,340 @@
+// Rows to int8 codes with one fp32 scale each, behind the residual's addition and an
+// RMSNorm or as they are:
+//   h = fp16(x + residual),  y = h / sqrt(sum h^2 / mean_dim + eps) * w
+//   s = fp32(clip max|y| / 127),  code = clamp(rne(y / s), -127, 127)
+// One pass: a row stays in registers (16-byte loads, up to 32 values a thread), and
+// the sum of squares and max|h w| are joined in one exchange, since the maximum of y
+// is that of h w times the norm's factor.
+// The codes are those of 64-bit arithmetic: h w is exact in fp32 (22 bits), the sum of
+// squares is added in 64 bits, and a quotient that fp32 puts within 2^-15 of a tie (its
+// error is at most 127 * 2^-23 = 2^-16, two roundings) is decided in 64 bits, which
+// happens to one value in 16000.  So a code does not depend on the order of a sum.
+// HBM bounds it: 7 bytes a value with the residual, 3 without a norm.
+#include "common.h"
+
+namespace {
+
+struct RowArgs {
+    const f16 *x, *res, *w;
+    int64_t xs, rs;           // row strides of x and res
+    f16 *sum, *norm;          // [rows, n] or null
+    int8_t *q;                // [rows, n]
+    float *scale;             // [rows]
+    int64_t rows, n;
+    double eps, mean_dim;
+    double clip;
+};
+
+// 8 values that may begin at any element: the hardware takes unaligned vector accesses
+struct __attribute__((packed, aligned(2))) U8h { v8h v; };
+struct __attribute__((packed, aligned(1))) U8b { u32 v[2]; };
+
+SRQ_DEV v8h load8(const f16 *p, int64_t left) {
+    if (left >= 8) return reinterpret_cast<const U8h *>(p)->v;
+    v8h v = (v8h)(f16)0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (i < left) v[i] = p[i];
+    return v;
+}
+
+SRQ_DEV void store8(f16 *p, const v8h &v, int64_t left) {
+    if (left >= 8) {
+        reinterpret_cast<U8h *>(p)->v = v;
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (i < left) p[i] = v[i];
+}
+
+SRQ_DEV float max_nan(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+
+// What a row's codes follow from: the norm's factor, the scale, and their quotient.
+struct Row {
+    double r, s;
+    float c, scale;
+    bool bad;   // NaN or infinite values: the scale is NaN, the codes are 0
+};
+
+template <bool NORM>
+SRQ_DEV Row row_of(const RowArgs &a, double sq, float top) {
+    Row o;
+    o.r = NORM ? 1.0 / __builtin_sqrt(sq / a.mean_dim + a.eps) : 1.0;
+    const double y = (double)top * o.r;
+    o.scale = (float)(y * a.clip / 127.0);
+    o.s = (double)o.scale;
+    o.bad = !(y <= 1e300) || !(o.scale <= 3e38f);
+    if (o.bad) o.scale = __builtin_nanf("");
+    o.c = o.bad || o.scale == 0.f ? 0.f : (float)(o.r / o.s);
+    return o;
+}
+
+// Codes of 8 values t (h w, exact): bytes in order.
+SRQ_DEV U8b codes8(const float (&t)[8], const Row &o) {
+    float q[8], k[8], far = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        q[i] = t[i] * o.c;
+        q[i] = __builtin_amdgcn_fmed3f(q[i], -127.25f, 127.25f);
+        k[i] = __builtin_rintf(q[i]);
+        far = fmaxf(far, fabsf(q[i] - k[i]));
+    }
+    if (far > 0.5f - 0x1p-15f) {   // next to a tie
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (fabsf(q[i] - k[i]) > 0.5f - 0x1p-15f) {
+                const double e = __builtin_rint((double)t[i] * o.r / o.s);
+                k[i] = (float)fmin(fmax(e, -127.0), 127.0);
+            }
+    }
+    u32 b[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) b[i] = (u32)(int)k[i];
+    U8b out;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const u32 lo = __builtin_amdgcn_perm(b[4 * h + 1], b[4 * h], 0x0C0C0400u);
+        const u32 hi = __builtin_amdgcn_perm(b[4 * h + 3], b[4 * h + 2], 0x04000C0Cu);
+        out.v[h] = lo | hi;
+    }
+    return out;
+}
+
+// T threads a row, V vectors of 8 a thread; rows of T = 64 share a block of 4 waves.
+template <int T, int V, bool NORM, bool WT, bool RES>
+__global__ __launch_bounds__(T == 64 ? 256 : T) void row_quant_kernel(RowArgs a) {
+    constexpr int W = T / 64;
+    __shared__ double part_sq[W > 1 ? W : 1];
+    __shared__ float part_top[W > 1 ? W : 1];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t row = W > 1 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
+    if (row >= a.rows) return;   // whole waves, and no barrier behind it where W == 1
+    const int at = W > 1 ? threadIdx.x : lane;
+    const f16 *x = a.x + row * a.xs;
+    v8h h[V], wv[WT ? V : 1];
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        const int64_t i = 8 * ((int64_t)v * T + at);
+        h[v] = load8(x + i, a.n - i);
+    }
+    if constexpr (WT) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            const int64_t i = 8 * ((int64_t)v * T + at);
+            wv[v] = load8(a.w + i, a.n - i);
+        }
+    }
+    if constexpr (RES) {
+        v8h r[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            const int64_t i = 8 * ((int64_t)v * T + at);
+            r[v] = load8(a.res + row * a.rs + i, a.n - i);
+        }
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            const int64_t i = 8 * ((int64_t)v * T + at);
+            h[v] = h[v] + r[v];   // one rounding to fp16 a value
+            if (a.sum) store8(a.sum + row * a.n + i, h[v], a.n - i);
+        }
+    }
+    double sq = 0;
+    float top = 0.f;
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float f = (float)h[v][i];
+            if constexpr (NORM) sq = __builtin_fma((double)f, (double)f, sq);
+            top = max_nan(top, fabsf(WT ? f * (float)wv[v][i] : f));
+        }
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) {
+        if constexpr (NORM) sq += __shfl_xor(sq, off, 64);
+        top = max_nan(top, __shfl_xor(top, off, 64));
+    }
+    if constexpr (W > 1) {
+        if (lane == 0) {
+            part_sq[wave] = sq;
+            part_top[wave] = top;
+        }
+        __syncthreads();
+        sq = part_sq[0];
+        top = part_top[0];
+#pragma unroll
+        for (int i = 1; i < W; ++i) {
+            sq += part_sq[i];
+            top = max_nan(top, part_top[i]);
+        }
+    }
+    const Row o = row_of<NORM>(a, sq, top);
+    if (at == 0) a.scale[row] = o.scale;
+    const float r32 = (float)o.r;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        const int64_t i = 8 * ((int64_t)v * T + at);
+        if (i >= a.n) continue;
+        float t[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            t[k] = WT ? (float)h[v][k] * (float)wv[v][k] : (float)h[v][k];
+        if (NORM && a.norm) {
+            v8h y;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) y[k] = f16_rn(t[k] * r32);
+            store8(a.norm + row * a.n + i, y, a.n - i);
+        }
+        U8b c = codes8(t, o);
+        if (o.bad) c.v[0] = c.v[1] = 0;
+        int8_t *q = a.q + row * a.n + i;
+        if (a.n - i >= 8) {
+            *reinterpret_cast<U8b *>(q) = c;
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (i + k < a.n) q[k] = (int8_t)(c.v[k / 4] >> (8 * (k % 4)));
+        }
+    }
+}
+
+// Rows of more than 32 values a thread: the row is read twice, the second time as the
+// sum that the same thread stored, where there is one.
+template <bool NORM, bool WT, bool RES>
+__global__ __launch_bounds__(1024) void row_quant_long_kernel(RowArgs a) {
+    __shared__ double part_sq[16];
+    __shared__ float part_top[16];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t row = blockIdx.x;
+    const f16 *x = a.x + row * a.xs;
+    // without a buffer for the sum it is formed again: then nothing is overwritten
+    auto sum_of = [&](int64_t i) __attribute__((always_inline)) {
+        v8h h = load8(x + i, a.n - i);
+        if constexpr (RES) h = h + load8(a.res + row * a.rs + i, a.n - i);
+        return h;
+    };
+    double sq = 0;
+    float top = 0.f;
+    for (int64_t i = 8 * (int64_t)threadIdx.x; i < a.n; i += 8 * 1024) {
+        const v8h h = sum_of(i);
+        if (RES && a.sum) store8(a.sum + row * a.n + i, h, a.n - i);
+        v8h w = (v8h)(f16)1;
+        if constexpr (WT) w = load8(a.w + i, a.n - i);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const float f = (float)h[k];
+            if constexpr (NORM) sq = __builtin_fma((double)f, (double)f, sq);
+            top = max_nan(top, fabsf(WT ? f * (float)w[k] : f));
+        }
+    }
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) {
+        if constexpr (NORM) sq += __shfl_xor(sq, off, 64);
+        top = max_nan(top, __shfl_xor(top, off, 64));
+    }
+    if (lane == 0) {
+        part_sq[wave] = sq;
+        part_top[wave] = top;
+    }
+    __syncthreads();
+    sq = part_sq[0];
+    top = part_top[0];
+    for (int i = 1; i < 16; ++i) {
+        sq += part_sq[i];
+        top = max_nan(top, part_top[i]);
+    }
+    const Row o = row_of<NORM>(a, sq, top);
+    if (threadIdx.x == 0) a.scale[row] = o.scale;
+    const float r32 = (float)o.r;
+    for (int64_t i = 8 * (int64_t)threadIdx.x; i < a.n; i += 8 * 1024) {
+        const v8h h = RES && a.sum ? load8(a.sum + row * a.n + i, a.n - i) : sum_of(i);
+        v8h w = (v8h)(f16)1;
+        if constexpr (WT) w = load8(a.w + i, a.n - i);
+        float t[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) t[k] = WT ? (float)h[k] * (float)w[k] : (float)h[k];
+        if (NORM && a.norm) {
+            v8h y;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) y[k] = f16_rn(t[k] * r32);
+            store8(a.norm + row * a.n + i, y, a.n - i);
+        }
+        U8b c = codes8(t, o);
+        if (o.bad) c.v[0] = c.v[1] = 0;
+        int8_t *q = a.q + row * a.n + i;
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (i + k < a.n) q[k] = (int8_t)(c.v[k / 4] >> (8 * (k % 4)));
+    }
+}
+
+template <bool NORM, bool WT, bool RES>
+void launch(const RowArgs &a, hipStream_t st) {
+    const dim3 one((unsigned)a.rows), four((unsigned)srq_cdiv(a.rows, 4));
+    // A wave a row up to 1024 values (no barrier), then the block grows with the row, so
+    // that no thread holds more than 32.
+    if (a.n <= 512)
+        row_quant_kernel<64, 1, NORM, WT, RES><<<four, 256, 0, st>>>(a);
+    else if (a.n <= 1024)
+        row_quant_kernel<64, 2, NORM, WT, RES><<<four, 256, 0, st>>>(a);
+    else if (a.n <= 2048)
+        row_quant_kernel<256, 1, NORM, WT, RES><<<one, 256, 0, st>>>(a);
+    else if (a.n <= 4096)
+        row_quant_kernel<256, 2, NORM, WT, RES><<<one, 256, 0, st>>>(a);
+    else if (a.n <= 8192)
+        row_quant_kernel<256, 4, NORM, WT, RES><<<one, 256, 0, st>>>(a);
+    else if (a.n <= 16384)
+        row_quant_kernel<1024, 2, NORM, WT, RES><<<one, 1024, 0, st>>>(a);
+    else if (a.n <= 32768)
+        row_quant_kernel<1024, 4, NORM, WT, RES><<<one, 1024, 0, st>>>(a);
+    else
+        row_quant_long_kernel<NORM, WT, RES><<<one, 1024, 0, st>>>(a);
+}
+
+}  // namespace
+
+extern "C" int srq_rmsnorm_quant_i8(const void *x, int64_t x_stride, const void *residual,
+                                    int64_t res_stride, const void *weight, int64_t rows,
+                                    int64_t cols, double eps, int64_t mean_dim, double clip_ratio,
+                                    void *sum, void *norm, void *q, void *scale, void *stream) {
+    SRQ_CHECK_ARG(rows >= 0 && cols >= 0, "rmsnorm_quant_i8: negative size");
+    SRQ_CHECK_ARG(rows <= 0x7FFFFFFF, "rmsnorm_quant_i8: more than 2^31 - 1 rows");
+    SRQ_CHECK_ARG(mean_dim > 0, "rmsnorm_quant_i8: mean_dim must be positive");
+    SRQ_CHECK_ARG(eps >= 0.0 && eps <= 1e300, "rmsnorm_quant_i8: eps must be finite and >= 0");
+    SRQ_CHECK_ARG(clip_ratio > 0.0 && clip_ratio <= 1.0,
+                  "rmsnorm_quant_i8: clip_ratio must lie in (0, 1]");
+    if (rows == 0) return SRQ_OK;
+    SRQ_CHECK_ARG(cols > 0, "rmsnorm_quant_i8: empty rows");
+    SRQ_CHECK_ARG(x && q && scale, "rmsnorm_quant_i8: null pointer");
+    SRQ_CHECK_ARG(!sum || residual, "rmsnorm_quant_i8: a sum without a residual");
+    SRQ_CHECK_ARG(x_stride >= cols && (!residual || res_stride >= cols),
+                  "rmsnorm_quant_i8: row stride below the row's length");
+    RowArgs a{(const f16 *)x, (const f16 *)residual, (const f16 *)weight, x_stride, res_stride,
+              (f16 *)sum, (f16 *)norm, (int8_t *)q, (float *)scale, rows, cols, eps, (double)mean_dim,
+              clip_ratio};
+    hipStream_t st = (hipStream_t)stream;
+    if (weight)
+        residual ? launch<true, true, true>(a, st) : launch<true, true, false>(a, st);
+    else
+        residual ? launch<true, false, true>(a, st) : launch<true, false, false>(a, st);
+    SRQ_LAUNCH_CHECK("rmsnorm_quant_i8");
+    return SRQ_OK;
+}
+
+extern "C" int srq_sym_quant_dynamic_i8(const void *x, int64_t x_stride, int64_t rows,
+                                        int64_t cols, double clip_ratio, void *q, void *scale,
+                                        void *stream) {
+    SRQ_CHECK_ARG(rows >= 0 && cols >= 0, "sym_quant_dynamic_i8: negative size");
+    SRQ_CHECK_ARG(rows <= 0x7FFFFFFF, "sym_quant_dynamic_i8: more than 2^31 - 1 rows");
+    SRQ_CHECK_ARG(clip_ratio > 0.0 && clip_ratio <= 1.0,
+                  "sym_quant_dynamic_i8: clip_ratio must lie in (0, 1]");
+    if (rows == 0) return SRQ_OK;
+    SRQ_CHECK_ARG(cols > 0, "sym_quant_dynamic_i8: empty rows");
+    SRQ_CHECK_ARG(x && q && scale, "sym_quant_dynamic_i8: null pointer");
+    SRQ_CHECK_ARG(x_stride >= cols, "sym_quant_dynamic_i8: row stride below the row's length");
+    RowArgs a{(const f16 *)x, nullptr, nullptr, x_stride, 0, nullptr, nullptr, (int8_t *)q,
+              (float *)scale, rows, cols, 0.0, 1.0, clip_ratio};
+    launch<false, false, false>(a, (hipStream_t)stream);
+    SRQ_LAUNCH_CHECK("sym_quant_dynamic_i8");
+    return SRQ_OK;
+}
