@@ -70,6 +70,17 @@ SRQ_DEV uint32_t lds_addr(const void *p) {
     return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void *)p;
 }
 
+SRQ_DEV v4i lds16(uint32_t addr) {
+    return *(__attribute__((address_space(3))) const v4i *)(uintptr_t)addr;
+}
+
+// Between the lanes of a wave: what one wrote to LDS, another reads.
+SRQ_DEV void wave_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // At most `ahead` groups of PER loads of this wave are still in flight (ahead < 8; the
 // counter goes to 63, and a smaller count waits for more).
 template <int PER>
@@ -119,7 +130,7 @@ __global__ __launch_bounds__(W * 64) void w4a8_stream_kernel(A8Args a) {
 #pragma unroll
     for (int i = 0; i < AR / 8; ++i) {
         const int r = 8 * i + (lane >> 3);
-        aoff[i] = r < a.M ? (uint32_t)(r * a.K) + 16 * ((lane & 7) ^ (r & 7)) : kOob;
+        aoff[i] = r < a.M ? (uint32_t)(r * a.K) + 16 * ((lane & 7) ^ (r >> 1 & 7)) : kOob;
     }
     bk = 16 * ((lane & 3) ^ ((lane >> 4) & 3));
 #pragma unroll
@@ -159,7 +170,7 @@ __global__ __launch_bounds__(W * 64) void w4a8_stream_kernel(A8Args a) {
 #pragma unroll
             for (int h = 0; h < 2; ++h)
                 av[i][h] = *reinterpret_cast<const v4i *>(
-                    st + (16 * i + mr) * 128 + 16 * ((2 * g + h) ^ (mr & 7)));
+                    st + (16 * i + mr) * 128 + 16 * ((2 * g + h) ^ (mr >> 1)));
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             const v4i w = *reinterpret_cast<const v4i *>(
@@ -206,8 +217,19 @@ __global__ __launch_bounds__(W * 64) void w4a8_stream_kernel(A8Args a) {
 // stage is filled next, has been read by all.
 struct __attribute__((packed, aligned(2))) U8h { v8h v; };
 
+template <int BM, int BN>
+struct Scales {
+    float sa[BM], sb[BN], bias[BN];   // of a tile
+};
+
 template <int BM, int BN, int WM, int WN, int NSTG>
-__global__ __launch_bounds__(64 * WM * WN) void w4a8_tile_kernel(A8Args a) {
+constexpr int ring_bytes() {
+    return NSTG * (BM * 128 + BN * 64);
+}
+
+// One tile, from row m0 and column n0 on.
+template <int BM, int BN, int WM, int WN, int NSTG>
+SRQ_DEV void tile_body(const A8Args &a, uint8_t *smem, Scales<BM, BN> &sc, int64_t m0, int64_t n0) {
     constexpr int NW = WM * WN, FM = BM / WM / 32, FN = BN / WN / 32;
     static_assert(FM * WM * 32 == BM && FN * WN * 32 == BN, "tile");
     constexpr int kStage = BM * 128 + BN * 64;
@@ -216,19 +238,9 @@ __global__ __launch_bounds__(64 * WM * WN) void w4a8_tile_kernel(A8Args a) {
     static_assert(NSTG >= 2 && NSTG <= 8 && (NSTG - 2) * PER <= 63, "loads in flight");
     constexpr int kTileW = 32 * FN + 8;                 // row stride of a wave's output rows
     constexpr int kRing = NSTG * kStage;
-    static_assert(NW * 32 * kTileW * 2 <= kRing, "output rows");
-    __shared__ __attribute__((aligned(1024))) uint8_t smem[kRing];
+    static_assert(NW * 32 * FM * kTileW * 2 <= kRing, "output rows");
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-
-    // Block b runs on XCD b % 8: each XCD takes a run of tiles, rows fastest, so that
-    // the blocks which share its L2 read the same few weight panels.
-    const uint32_t tiles_m = (uint32_t)srq_cdiv(a.M, BM), total = gridDim.x;
-    const uint32_t x = blockIdx.x % 8, per = total / 8, rem = total % 8;
-    const uint32_t idx = x * per + min(x, rem) + blockIdx.x / 8;
-    const uint32_t tn = uni(idx / tiles_m);
-    const int64_t m0 = (int64_t)(idx - tn * tiles_m) * BM, n0 = (int64_t)tn * BN;
-
     const int64_t KB = a.K / 2;
     const int64_t k_lo = a.kc ? (int64_t)blockIdx.y * a.kc : 0;
     const int64_t k_hi = a.kc ? min(a.K, k_lo + a.kc) : a.K;
@@ -238,70 +250,123 @@ __global__ __launch_bounds__(64 * WM * WN) void w4a8_tile_kernel(A8Args a) {
     const __amdgpu_buffer_rsrc_t br = make_rsrc(a.w + n0 * KB, rows_bytes(a.N - n0, BN, KB));
     const uint32_t ring0 = lds_addr(smem);
 
+    // (ahead of the ring's loads, which are counted)
+    if (!a.kc) {
+        for (int i = threadIdx.x; i < BM; i += NW * 64) sc.sa[i] = m0 + i < a.M ? a.sa[m0 + i] : 0.f;
+        for (int i = threadIdx.x; i < BN; i += NW * 64) {
+            const bool in = n0 + i < a.N;
+            sc.sb[i] = in ? (float)a.sb[n0 + i] : 0.f;
+            sc.bias[i] = in && a.bias ? (float)a.bias[n0 + i] : 0.f;
+        }
+    }
+
     uint32_t aoff[PA], boff[PB];
 #pragma unroll
     for (int q = 0; q < PA; ++q) {
         const int r = 8 * (q * NW + wave) + (lane >> 3);
-        aoff[q] = (uint32_t)(r * a.K + k_lo) + 16 * ((lane & 7) ^ (r & 7));
+        aoff[q] = (uint32_t)(r * a.K + k_lo) + 16 * ((lane & 7) ^ (r >> 1 & 7));
     }
     const int bk = 16 * ((lane & 3) ^ ((lane >> 4) & 3));
 #pragma unroll
     for (int q = 0; q < PB; ++q)
         boff[q] = (uint32_t)((16 * (q * NW + wave) + (lane >> 2)) * KB + k_lo / 2) + bk;
-    auto issue = [&](int s) __attribute__((always_inline)) {
-        const uint32_t dst = ring0 + (s % NSTG) * kStage + wave * 1024;
-#pragma unroll
-        for (int q = 0; q < PA; ++q) dma16(ar, aoff[q] + 128u * s, dst + q * NW * 1024);
+    // loads q_lo .. q_hi of this wave's of step s, into the stage at dst
+    auto issue = [&](int s, uint32_t dst, int q_lo, int q_hi) __attribute__((always_inline)) {
         // past K: zero weights cancel whatever the rows hold there
         const bool in = k_lo / 2 + 64 * (int64_t)s + bk < KB;
+        dst += ring0 + wave * 1024;
 #pragma unroll
-        for (int q = 0; q < PB; ++q)
-            dma16(br, in ? boff[q] + 64u * s : kOob, dst + BM * 128 + q * NW * 1024);
+        for (int q = 0; q < PER; ++q) {
+            if (q < q_lo || q >= q_hi) continue;
+            if (q < PA)
+                dma16(ar, aoff[q] + 128u * s, dst + q * NW * 1024);
+            else
+                dma16(br, in ? boff[q - PA] + 64u * s : kOob, dst + BM * 128 + (q - PA) * NW * 1024);
+        }
     };
 #pragma unroll
-    for (int p = 0; p < NSTG - 1; ++p)
-        if (p < steps) issue(p);
+    for (int p = 0; p < NSTG; ++p)
+        if (p < steps) issue(p, p * kStage, 0, PER);
 
     const int wm = wave / WN, wn = wave % WN;
     const int rr = lane & 31, g = lane >> 5;
+    // LDS addresses of this lane's chunks of the first block of rows, by slice of 32 codes
+    // (slice 2 p + h of a lane: chunk 4 p + 2 g + h of a row, half h of weight chunk 2 p + g)
+    uint32_t al[4], bl[2];
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+        al[c] = ring0 + (wm * (FM * 32) + rr) * 128 + 16 * ((4 * (c >> 1) + 2 * g + (c & 1)) ^ (rr >> 1 & 7));
+#pragma unroll
+    for (int p = 0; p < 2; ++p)
+        bl[p] = ring0 + BM * 128 + (wn * (FN * 32) + rr) * 64 + 16 * ((2 * p + g) ^ (rr >> 2 & 3));
     v16i acc[FM][FN];
 #pragma unroll
     for (int i = 0; i < FM; ++i)
 #pragma unroll
         for (int j = 0; j < FN; ++j) acc[i][j] = (v16i){};
+    v4i av[2][FM], wv[2][FN], bv[2][FN];
+    auto fetch_a = [&](int c, uint32_t st) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < FM; ++i) av[c & 1][i] = lds16(al[c] + st + i * 4096);
+    };
+    auto fetch_b = [&](int p, uint32_t st) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < FN; ++j) wv[p][j] = lds16(bl[p] + st + j * 2048);
+    };
+    auto unpack = [&](int c) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+            bv[c & 1][j] = codes16((u32)wv[c >> 1][j][2 * (c & 1)], (u32)wv[c >> 1][j][2 * (c & 1) + 1]);
+    };
+    // The operands of a slice are read and unpacked beside the products of the one before,
+    // across the steps too: the barrier stands ahead of a step's last products, when its
+    // stage has been read and the next one is needed.
+    wait_ahead<PER>(min(NSTG - 1, steps - 1));
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    fetch_b(0, 0);
+    fetch_a(0, 0);
+    unpack(0);
+    // A step's loads are spread over four slices, the first behind the barrier that frees
+    // their stage: a wave stalls on a burst of them, and its products with it.
+    uint32_t st = 0, fst = 0;
+    int fill = steps;
     for (int s = 0; s < steps; ++s) {
-        wait_ahead<PER>(min(NSTG - 2, steps - 1 - s));
-        // this wave's reads of step s - 1 have returned
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-        if (s + NSTG - 1 < steps) issue(s + NSTG - 1);
-        const uint8_t *sa = smem + (s % NSTG) * kStage, *sb = sa + BM * 128;
+        const uint32_t nst = st == (NSTG - 1) * kStage ? 0 : st + kStage;
 #pragma unroll
-        for (int p = 0; p < 2; ++p) {
-            v4i wv[FN];
-#pragma unroll
-            for (int j = 0; j < FN; ++j) {
-                const int r = wn * (FN * 32) + j * 32 + rr;
-                wv[j] = *reinterpret_cast<const v4i *>(sb + r * 64 + 16 * ((2 * p + g) ^ ((r >> 2) & 3)));
+        for (int c = 0; c < 4; ++c) {
+            if (c < 3) {
+                if (c == 0) fetch_b(1, st);
+                fetch_a(c + 1, st);
+            } else if (s + 1 < steps) {
+                // step s + 1 has landed and this wave has read all of step s ..
+                wait_ahead<PER>(min(NSTG - 2, steps - 2 - s));
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                // .. and so it is for all waves
+                __builtin_amdgcn_s_barrier();
+                asm volatile("" ::: "memory");
+                fetch_b(0, nst);
+                fetch_a(0, nst);
+                fill = s + NSTG;
+                fst = st;
             }
+            if (fill < steps) issue(fill, fst, PER * ((c + 1) & 3) / 4, PER * (((c + 1) & 3) + 1) / 4);
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                v4i av[FM];
+            for (int j = 0; j < FN; ++j)
 #pragma unroll
-                for (int i = 0; i < FM; ++i) {
-                    const int r = wm * (FM * 32) + i * 32 + rr;
-                    av[i] = *reinterpret_cast<const v4i *>(sa + r * 128 +
-                                                           16 * ((4 * p + 2 * g + h) ^ (r & 7)));
-                }
+                for (int i = 0; i < FM; ++i) acc[i][j] = mfma32x32(av[c & 1][i], bv[c & 1][j], acc[i][j]);
+            unpack((c + 1) & 3);
+            constexpr int kMf = FM * FN, kValu = (10 * FN + kMf - 1) / kMf;
+            if (c == 0) __builtin_amdgcn_sched_group_barrier(0x100, FM + FN, 0);
+            else if (c < 3) __builtin_amdgcn_sched_group_barrier(0x100, FM, 0);
 #pragma unroll
-                for (int j = 0; j < FN; ++j) {
-                    const v4i b = codes16((u32)wv[j][2 * h], (u32)wv[j][2 * h + 1]);
-#pragma unroll
-                    for (int i = 0; i < FM; ++i) acc[i][j] = mfma32x32(av[i], b, acc[i][j]);
-                }
+            for (int k = 0; k < kMf; ++k) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x002, kValu, 0);
             }
+            __builtin_amdgcn_sched_barrier(0);
         }
+        st = nst;
     }
 
     const int64_t mw = m0 + wm * (FM * 32), nw = n0 + wn * (FN * 32);
@@ -320,57 +385,121 @@ __global__ __launch_bounds__(64 * WM * WN) void w4a8_tile_kernel(A8Args a) {
             }
         return;
     }
-    // 32 rows of the wave at a time through its own piece of LDS, so that they leave in
-    // 16 bytes a lane
+    // The wave's rows pass through its own piece of LDS, so that they leave, and a residual
+    // comes, in 16 bytes a lane.
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    f16 *tile = reinterpret_cast<f16 *>(smem) + wave * 32 * kTileW;
-    float sbv[FN], bv[FN];
+    f16 *tile = reinterpret_cast<f16 *>(smem) + wave * (32 * FM) * kTileW;
+    constexpr int LPR = 4 * FN, RPI = 64 / LPR;   // lanes a row, rows an instruction
+    const int c8 = 8 * (lane % LPR);
+    const int64_t n8 = nw + c8;
+    if (a.res) {
 #pragma unroll
-    for (int j = 0; j < FN; ++j) {
-        const int64_t n = nw + j * 32 + rr;
-        sbv[j] = n < a.N ? (float)a.sb[n] : 0.f;
-        bv[j] = a.bias && n < a.N ? (float)a.bias[n] : 0.f;
-    }
-#pragma unroll
-    for (int i = 0; i < FM; ++i) {
-#pragma unroll
-        for (int v = 0; v < 16; ++v) {
-            const int lr = 8 * (v / 4) + 4 * g + v % 4;
-            const int64_t m = mw + i * 32 + lr;
-            const float sa = m < a.M ? a.sa[m] : 0.f;
-#pragma unroll
-            for (int j = 0; j < FN; ++j) {
-                const int64_t n = nw + j * 32 + rr;
-                float o = dequant(acc[i][j][v], sa, sbv[j]) + bv[j];
-                if (a.res && m < a.M && n < a.N) o += (float)a.res[m * a.N + n];
-                tile[lr * kTileW + j * 32 + rr] = f16_rn(o);
-            }
-        }
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-        constexpr int LPR = 4 * FN, RPI = 64 / LPR;   // lanes a row, rows an instruction
-#pragma unroll
-        for (int r0 = 0; r0 < 32; r0 += RPI) {
-            const int lr = r0 + lane / LPR, c = 8 * (lane % LPR);
-            const int64_t m = mw + i * 32 + lr, n = nw + c;
-            if (m >= a.M || n >= a.N) continue;
-            const v8h o = *reinterpret_cast<const v8h *>(tile + lr * kTileW + c);
-            f16 *dst = a.out + m * a.N + n;
-            if (n + 8 <= a.N) {
-                reinterpret_cast<U8h *>(dst)->v = o;
+        for (int r0 = 0; r0 < 32 * FM; r0 += RPI) {
+            const int lr = r0 + lane / LPR;
+            const int64_t m = mw + lr;
+            if (m >= a.M || n8 >= a.N) continue;
+            const f16 *src = a.res + m * a.N + n8;
+            v8h o;
+            if (n8 + 8 <= a.N) {
+                o = reinterpret_cast<const U8h *>(src)->v;
             } else {
 #pragma unroll
-                for (int k = 0; k < 8; ++k)
-                    if (n + k < a.N) dst[k] = o[k];
+                for (int k = 0; k < 8; ++k) o[k] = n8 + k < a.N ? src[k] : (f16)0;
             }
+            *reinterpret_cast<v8h *>(tile + lr * kTileW + c8) = o;
         }
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        wave_fence();
     }
+    float sbv[FN], biasv[FN];
+#pragma unroll
+    for (int j = 0; j < FN; ++j) {
+        sbv[j] = sc.sb[wn * (FN * 32) + j * 32 + rr];
+        biasv[j] = sc.bias[wn * (FN * 32) + j * 32 + rr];
+    }
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int v4 = 0; v4 < 4; ++v4) {
+            const int lr = i * 32 + 8 * v4 + 4 * g;
+            const v4f sa = *reinterpret_cast<const v4f *>(sc.sa + wm * (FM * 32) + lr);
+#pragma unroll
+            for (int v = 0; v < 4; ++v)
+#pragma unroll
+                for (int j = 0; j < FN; ++j) {
+                    f16 &at = tile[(lr + v) * kTileW + j * 32 + rr];
+                    float o = dequant(acc[i][j][4 * v4 + v], sa[v], sbv[j]) + biasv[j];
+                    if (a.res) o += (float)at;
+                    at = f16_rn(o);
+                }
+        }
+    wave_fence();
+#pragma unroll
+    for (int r0 = 0; r0 < 32 * FM; r0 += RPI) {
+        const int lr = r0 + lane / LPR;
+        const int64_t m = mw + lr;
+        if (m >= a.M || n8 >= a.N) continue;
+        const v8h o = *reinterpret_cast<const v8h *>(tile + lr * kTileW + c8);
+        f16 *dst = a.out + m * a.N + n8;
+        if (n8 + 8 <= a.N) {
+            reinterpret_cast<U8h *>(dst)->v = o;
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (n8 + k < a.N) dst[k] = o[k];
+        }
+    }
+}
+
+// Tile `idx` of tiles_m x tiles_n in bands of 8 rows of tiles, columns of a band one after
+// the other.
+SRQ_DEV void tile_place(uint32_t idx, uint32_t tiles_m, uint32_t tiles_n, uint32_t &tm,
+                        uint32_t &tn) {
+    const uint32_t band = uni(idx / (8 * tiles_n)), in_band = idx - band * 8 * tiles_n;
+    const uint32_t high = min(8u, tiles_m - 8 * band);
+    tn = uni(in_band / high);
+    tm = 8 * band + in_band - tn * high;
+}
+
+// Block b runs on XCD b % 8: each XCD takes a run of tiles, and with the bands the blocks
+// that share its L2 read a square of panels.
+SRQ_DEV uint32_t place_of(uint32_t b, uint32_t total) {
+    const uint32_t x = b % 8, per = total / 8, rem = total % 8;
+    return x * per + min(x, rem) + b / 8;
+}
+
+template <int BM, int BN, int WM, int WN, int NSTG>
+__global__ __launch_bounds__(64 * WM * WN) void w4a8_tile_kernel(A8Args a) {
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[ring_bytes<BM, BN, WM, WN, NSTG>()];
+    __shared__ Scales<BM, BN> sc;
+    uint32_t tm, tn;
+    tile_place(place_of(blockIdx.x, gridDim.x), (uint32_t)srq_cdiv(a.M, BM),
+               (uint32_t)srq_cdiv(a.N, BN), tm, tn);
+    tile_body<BM, BN, WM, WN, NSTG>(a, smem, sc, (int64_t)tm * BM, (int64_t)tn * BN);
+}
+
+// Many rows: `whole` tiles of 256 x 256, a multiple of the 256 CUs, and the rest, where it
+// is half a round at most, as twice as many of 256 x 128.
+__global__ __launch_bounds__(512) void w4a8_large_kernel(A8Args a, uint32_t whole) {
+    constexpr int kBytes = ring_bytes<256, 256, 2, 4, 3>();
+    static_assert(ring_bytes<256, 128, 4, 2, 3>() <= kBytes, "ring");
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[kBytes];
+    __shared__ union {
+        Scales<256, 256> whole;
+        Scales<256, 128> half;
+    } sc;
+    const uint32_t tiles_m = (uint32_t)srq_cdiv(a.M, 256), tiles_n = (uint32_t)srq_cdiv(a.N, 256);
+    uint32_t tm, tn;
+    if (blockIdx.x < whole) {
+        tile_place(place_of(blockIdx.x, whole), tiles_m, tiles_n, tm, tn);
+        tile_body<256, 256, 2, 4, 3>(a, smem, sc.whole, (int64_t)tm * 256, (int64_t)tn * 256);
+        return;
+    }
+    const uint32_t at = place_of(blockIdx.x - whole, gridDim.x - whole);
+    tile_place(whole + at / 2, tiles_m, tiles_n, tm, tn);
+    const int64_t n0 = (int64_t)tn * 256 + 128 * (at & 1);
+    if (n0 < a.N) tile_body<256, 128, 4, 2, 3>(a, smem, sc.half, (int64_t)tm * 256, n0);
 }
 
 // The splits' int32 sums, joined, and the epilogue: 4 columns a thread.
@@ -407,44 +536,40 @@ __global__ __launch_bounds__(256) void w4a8_join_kernel(A8Args a, int splits) {
 }
 
 // How a product runs, by its sizes alone.
+enum { kStream, k64x128, k128x128, kLarge };
 struct Plan {
-    int kind;        // 0: stream, else a tile form
-    int splits;      // over K (tile forms)
+    int kind;
+    int splits;      // over K
     int64_t kc;
 };
-enum { kStream, k64x64, k128x64, k128x128, k256x256 };
-
-void split(Plan &p, int64_t tiles, int64_t K) {
-    const int64_t steps = srq_cdiv(K, 128);
-    int64_t s = 256 / (tiles > 0 ? tiles : 1);
-    if (s > steps / 8) s = steps / 8;   // at least 8 steps a split
-    if (s > 16) s = 16;
-    if (s < 2) return;
-    const int64_t per = srq_cdiv(steps, s);
-    p.kc = per * 128;
-    p.splits = (int)srq_cdiv(steps, per);
-    if (p.splits < 2) p = Plan{p.kind, 1, 0};
-}
 
 Plan plan_of(int64_t M, int64_t N, int64_t K) {
     Plan p{kStream, 1, 0};
     if (M <= 32) return p;
-    if (M > 512 && srq_cdiv(M, 256) * srq_cdiv(N, 256) >= 200) {
-        p.kind = k256x256;
+    // The largest tile of which there are enough for most of the 256 CUs: a CU takes in
+    // about 40 bytes a ns, and larger tiles need fewer.  us on one MI355X: 512 x 6144 x
+    // 4096, 128 x 128 / 64 x 128 21.3 / 24.6; 512 x 4096 x 4096 20.1 / 18.1 (128 and 256
+    // tiles); 200 x 28672 x 4096, 256 x 128 / 128 x 128 35.6 / 36.9.
+    const int64_t enough = 190, n128 = srq_cdiv(N, 128);
+    if (M > 128 && srq_cdiv(M, 256) * n128 >= enough) {
+        p.kind = kLarge;
         return p;
     }
-    if (M <= 64) {
-        p.kind = k64x64;
-        split(p, srq_cdiv(M, 64) * srq_cdiv(N, 64), K);
-        return p;
-    }
-    const int64_t t128 = srq_cdiv(M, 128) * srq_cdiv(N, 128);
-    if (t128 >= 200) {
-        p.kind = k128x128;
-        return p;
-    }
-    p.kind = k128x64;
-    split(p, srq_cdiv(M, 128) * srq_cdiv(N, 64), K);
+    const int64_t t128 = srq_cdiv(M, 128) * n128, t64 = srq_cdiv(M, 64) * n128;
+    p.kind = M > 64 && (t128 >= enough || t64 < enough) ? k128x128 : k64x128;
+    const int64_t tiles = p.kind == k128x128 ? t128 : t64;
+    if (tiles >= enough) return p;
+    // Else K is split, at least 8 steps of 128 codes each: 128 x 4096 x 14336 in 8 parts
+    // 20.8, in 4 23.4; 64 x 4096 x 14336 16.6 (8 parts of 64 x 128).
+    const int64_t steps = srq_cdiv(K, 128);
+    int64_t s = (p.kind == k64x128 ? 512 : 256) / tiles;
+    if (s > steps / 8) s = steps / 8;
+    if (s > 8) s = 8;
+    if (s < 2) return p;
+    const int64_t per = srq_cdiv(steps, s);
+    if (srq_cdiv(steps, per) < 2) return p;
+    p.kc = per * 128;
+    p.splits = (int)srq_cdiv(steps, per);
     return p;
 }
 
@@ -456,12 +581,21 @@ void launch_tile(const A8Args &a, int splits, hipStream_t st) {
 
 template <int AR>
 void launch_stream(const A8Args &a, hipStream_t st) {
+    // 16 columns a block up to a block a CU (256), then 32, which halves what the rows
+    // cost; more blocks than 256 run best two to a CU, which their LDS has to allow, and
+    // at 17 rows and more with 64 columns.  us, 28672 x 4096: 1 row 14 (32 columns, 4
+    // stages and so one block a CU: 17.7; 16 columns 13 to 14), 16 rows 16.2 (19.7), 32
+    // rows 20 (23.4 with 32 columns); 8192 x 28672: 16 rows 28.8 (16 columns: 35.4).
     const int64_t cb = srq_cdiv(a.N, 16);
+    auto grid = [&](int nt) { return dim3((unsigned)srq_cdiv(cb, nt)); };
     if (cb <= 256)
-        w4a8_stream_kernel<AR, 1, AR == 32 ? 3 : 6><<<(unsigned)cb, W * 64, 0, st>>>(a);
-    else
-        w4a8_stream_kernel<AR, 2, AR == 32 ? 3 : 4>
-            <<<(unsigned)srq_cdiv(cb, 2), W * 64, 0, st>>>(a);
+        w4a8_stream_kernel<AR, 1, AR == 32 ? 2 : 4><<<grid(1), W * 64, 0, st>>>(a);
+    else if (cb <= 512 || AR == 8)
+        w4a8_stream_kernel<AR, 2, 3><<<grid(2), W * 64, 0, st>>>(a);
+    else if constexpr (AR == 16)
+        w4a8_stream_kernel<AR, 2, 2><<<grid(2), W * 64, 0, st>>>(a);
+    else if constexpr (AR == 32)
+        w4a8_stream_kernel<AR, 4, 2><<<grid(4), W * 64, 0, st>>>(a);
 }
 
 }  // namespace
@@ -483,8 +617,8 @@ extern "C" int srq_w4a8_linear(const void *a, const void *a_scale, const void *w
     SRQ_CHECK_ARG(K > 0 && K % 32 == 0, "w4a8_linear: K=%lld must be a positive multiple of 32",
                   (long long)K);
     SRQ_CHECK_ARG(K <= kMaxK, "w4a8_linear: K=%lld must be below 131072", (long long)K);
-    SRQ_CHECK_ARG(M <= (int64_t)1 << 31 && N <= (int64_t)1 << 31 &&
-                      srq_cdiv(M, 64) * srq_cdiv(N, 64) <= 0x7FFFFFFF / 4,
+    // a launch has fewer than 2^32 threads in x: 512 for 16 columns, or for a tile
+    SRQ_CHECK_ARG(M <= 1 << 30 && N <= 1 << 26 && srq_cdiv(M, 64) * srq_cdiv(N, 64) < 1 << 23,
                   "w4a8_linear: shape out of range");
     if (M == 0 || N == 0) return SRQ_OK;
     SRQ_CHECK_ARG(a && a_scale && w && w_scale && out, "w4a8_linear: null pointer");
@@ -502,10 +636,13 @@ extern "C" int srq_w4a8_linear(const void *a, const void *a_scale, const void *w
         M <= 8 ? launch_stream<8>(q, st) : M <= 16 ? launch_stream<16>(q, st)
                                                    : launch_stream<32>(q, st);
         break;
-    case k64x64: launch_tile<64, 64, 2, 2, 6>(q, p.splits, st); break;
-    case k128x64: launch_tile<128, 64, 2, 2, 6>(q, p.splits, st); break;
-    case k128x128: launch_tile<128, 128, 2, 2, 3>(q, p.splits, st); break;
-    default: launch_tile<256, 256, 2, 4, 3>(q, 1, st); break;
+    case k64x128: launch_tile<64, 128, 2, 4, 4>(q, p.splits, st); break;
+    case k128x128: launch_tile<128, 128, 2, 4, 3>(q, p.splits, st); break;
+    default: {
+        const int64_t tiles = srq_cdiv(M, 256) * srq_cdiv(N, 256), rest = tiles % 256;
+        const int64_t whole = rest <= 128 ? tiles - rest : tiles;
+        w4a8_large_kernel<<<(unsigned)(whole + 2 * (tiles - whole)), 512, 0, st>>>(q, (uint32_t)whole);
+    }
     }
     SRQ_LAUNCH_CHECK("w4a8_linear");
     if (p.kc) {

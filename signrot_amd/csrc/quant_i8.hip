@@ -108,7 +108,8 @@ __global__ __launch_bounds__(T == 64 ? 256 : T) void row_quant_kernel(RowArgs a)
     __shared__ double part_sq[W > 1 ? W : 1];
     __shared__ float part_top[W > 1 ? W : 1];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t row = W > 1 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
+    const int64_t block = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
+    const int64_t row = W > 1 ? block : block * 4 + wave;
     if (row >= a.rows) return;   // whole waves, and no barrier behind it where W == 1
     const int at = W > 1 ? threadIdx.x : lane;
     const f16 *x = a.x + row * a.xs;
@@ -205,7 +206,8 @@ __global__ __launch_bounds__(1024) void row_quant_long_kernel(RowArgs a) {
     __shared__ double part_sq[16];
     __shared__ float part_top[16];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t row = blockIdx.x;
+    const int64_t row = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
+    if (row >= a.rows) return;
     const f16 *x = a.x + row * a.xs;
     // without a buffer for the sum it is formed again: then nothing is overwritten
     auto sum_of = [&](int64_t i) __attribute__((always_inline)) {
@@ -270,7 +272,12 @@ __global__ __launch_bounds__(1024) void row_quant_long_kernel(RowArgs a) {
 
 template <bool NORM, bool WT, bool RES>
 void launch(const RowArgs &a, hipStream_t st) {
-    const dim3 one((unsigned)a.rows), four((unsigned)srq_cdiv(a.rows, 4));
+    // a launch has fewer than 2^32 threads in x
+    auto grid = [](int64_t blocks) {
+        const int64_t most = 1 << 20;
+        return blocks <= most ? dim3((unsigned)blocks) : dim3(most, (unsigned)srq_cdiv(blocks, most));
+    };
+    const dim3 one = grid(a.rows), four = grid(srq_cdiv(a.rows, 4));
     // A wave a row up to 1024 values (no barrier), then the block grows with the row, so
     // that no thread holds more than 32.
     if (a.n <= 512)

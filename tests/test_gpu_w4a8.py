@@ -30,7 +30,9 @@ SHAPES = [(1, 1, 32), (1, 16, 128), (2, 17, 96), (7, 33, 160), (8, 48, 4096), (9
           (5, 8200, 512), (20, 4104, 1056), (33, 65, 128), (33, 64, 4096), (64, 130, 14336),
           (64, 4100, 96), (65, 63, 2048), (100, 1111, 8192), (128, 128, 32), (129, 257, 4064),
           (300, 515, 1024), (200, 8193, 512), (513, 128, 4096), (1000, 515, 2208),
-          (257, 12800, 256), (1030, 12801, 288), (515, 17000, 128)]
+          (257, 12800, 256), (1030, 12801, 288), (515, 17000, 128),
+          # a round of large tiles and a rest of half ones
+          (1300, 13000, 160), (2049, 8300, 96)]
 
 
 @pytest.mark.parametrize("M,N,K", SHAPES)
