@@ -40,7 +40,7 @@ struct LoraArgs {
     int slices, splits;
     int kc;                  // columns of K in a split (a multiple of 64)
     int col_end[kMaxSlices];    // of each slice
-    int tile_end[kMaxSlices];   // its column tiles (second product of many tokens)
+    int run_end[kMaxSlices];    // its runs of column tiles (second product of many tokens)
 };
 
 SRQ_DEV uint32_t uni(uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); }
@@ -109,32 +109,135 @@ __global__ __launch_bounds__(256) void lora_expand_few_kernel(LoraArgs a) {
     a.out[m * a.os + n] = f16_rn(__builtin_fmaf(acc, f, (float)a.y[m * a.ys + n]));
 }
 
+// Few tokens and a small adapter in one launch: a block takes 1024 columns of a slice for
+// one token and computes that slice's t itself, from rows of A that then come from L2;
+// y and its rows of B are loaded meanwhile.  RV rows of A a wave (r <= 8 RV).
+constexpr int kFewCols = 1024;
+constexpr int kFewK = 16384;
+
+template <int RV>
+__global__ __launch_bounds__(512) void lora_one_kernel(LoraArgs a) {
+    __shared__ __attribute__((aligned(16))) f16 xl[kFewK];
+    __shared__ float t[8 * RV];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int64_t m = blockIdx.y;
+    const int id = __builtin_amdgcn_readfirstlane(adapter_of(a, m));
+    const int at = blockIdx.x, K = (int)a.K, r = a.r;
+    int s = 0;
+    while (at >= a.run_end[s]) ++s;
+    const int n_hi = a.col_end[s];
+    const int n0 = (s ? a.col_end[s - 1] : 0) + (at - (s ? a.run_end[s - 1] : 0)) * kFewCols +
+                   (int)threadIdx.x;
+    const f16 *y = a.y + m * a.ys;
+    f16 *out = a.out + m * a.os;
+    if (id < 0) {
+        if (a.out == a.y) return;
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+            if (n0 + 512 * c < n_hi) out[n0 + 512 * c] = y[n0 + 512 * c];
+        return;
+    }
+    for (int k = 8 * (int)threadIdx.x; k < K; k += 8 * 512)
+        *reinterpret_cast<v8h *>(xl + k) = *reinterpret_cast<const v8h *>(a.x + m * a.xs + k);
+    v8h bv[2][RV];
+    float yv[2];
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+        const int n = min(n0 + 512 * c, n_hi - 1);
+        yv[c] = (float)y[n];
+        const f16 *b = a.b + ((int64_t)id * a.N + n) * r;
+#pragma unroll
+        for (int i = 0; i < RV; ++i) bv[c][i] = *reinterpret_cast<const v8h *>(b + min(8 * i, r - 8));
+    }
+    const float f = a.scaling ? a.scaling[id] : 1.f;
+    __syncthreads();
+    const f16 *w[RV];
+    float acc[RV][2] = {};
+#pragma unroll
+    for (int j = 0; j < RV; ++j)
+        w[j] = a.a + ((int64_t)id * a.R + s * r + min(RV * wave + j, r - 1)) * a.K;
+    auto add = [&](const v8h &p, const v8h &q, float (&c)[2]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) c[i & 1] = __builtin_fmaf((float)p[i], (float)q[i], c[i & 1]);
+    };
+    int k = 8 * lane;
+    constexpr int U = RV == 4 ? 2 : 4;
+    for (; k + 512 * (U - 1) < K; k += 512 * U) {
+        v8h q[U][RV];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int j = 0; j < RV; ++j) q[u][j] = *reinterpret_cast<const v8h *>(w[j] + k + 512 * u);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const v8h p = *reinterpret_cast<const v8h *>(xl + k + 512 * u);
+#pragma unroll
+            for (int j = 0; j < RV; ++j) add(p, q[u][j], acc[j]);
+        }
+    }
+    for (; k < K; k += 512) {
+        const v8h p = *reinterpret_cast<const v8h *>(xl + k);
+#pragma unroll
+        for (int j = 0; j < RV; ++j) add(p, *reinterpret_cast<const v8h *>(w[j] + k), acc[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < RV; ++j) {
+        const float v = wave_sum(acc[j][0] + acc[j][1]);
+        if (lane == 0 && RV * wave + j < r) t[RV * wave + j] = v;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+        float v = 0.f;
+#pragma unroll
+        for (int i = 0; i < RV; ++i)
+            if (8 * i < r)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v = __builtin_fmaf((float)bv[c][i][e], t[8 * i + e], v);
+        if (n0 + 512 * c < n_hi) out[n0 + 512 * c] = f16_rn(__builtin_fmaf(v, f, yv[c]));
+    }
+}
+
 // ------------------------------------------------------------ many tokens
 
 constexpr int kTok = 64;   // tokens of a tile: one a lane
 
-// The distinct adapters of a tile, one at a time: those with j % nz == z are this block's.
+// The distinct adapters of a tile of 64 Q tokens, one at a time: those with j % nz == z
+// are this block's.
+template <int Q>
 struct Turns {
-    uint64_t left, invalid;
-    int id, j;
+    uint64_t left[Q], invalid[Q];
+    int id[Q], j;
     SRQ_DEV Turns(const LoraArgs &a, int64_t m0, int lane) : j(0) {
-        const int64_t m = m0 + lane;
-        id = m < a.M ? adapter_of(a, m) : -1;
-        left = __ballot(id >= 0);
-        invalid = __ballot(m < a.M && id < 0);
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+            const int64_t m = m0 + 64 * q + lane;
+            id[q] = m < a.M ? adapter_of(a, m) : -1;
+            left[q] = __ballot(id[q] >= 0);
+            invalid[q] = __ballot(m < a.M && id[q] < 0);
+        }
     }
     // the next adapter of this block and the mask of its tokens, or -1
-    SRQ_DEV int next(int z, int nz, uint64_t &same) {
-        while (left) {
-            const int first = __builtin_ctzll(left);
-            const int cur = __builtin_amdgcn_readlane(id, first);
-            same = __ballot(id == cur);
-            left &= ~same;
-            if (j++ % nz == z) return cur;
-        }
+    SRQ_DEV int next(int z, int nz, uint64_t (&same)[Q]) {
+#pragma unroll
+        for (int q = 0; q < Q; ++q)
+            while (left[q]) {
+                const int cur = __builtin_amdgcn_readlane(id[q], __builtin_ctzll(left[q]));
+#pragma unroll
+                for (int p = 0; p < Q; ++p) {
+                    same[p] = __ballot(id[p] == cur);
+                    left[p] &= ~same[p];
+                }
+                if (j++ % nz == z) return cur;
+            }
         return -1;
     }
 };
+
+SRQ_DEV v8h lds16(uint32_t addr) {
+    return *(__attribute__((address_space(3))) const v8h *)(uintptr_t)addr;
+}
 
 SRQ_DEV v4f mfma16(v8h a, v8h b, v4f c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
@@ -146,119 +249,138 @@ SRQ_DEV v16f mfma32(v8h a, v8h b, v16f c) {
 
 // Block b runs on XCD b % 8: its place in the work such that each XCD, with its own L2,
 // has a run of neighbouring token tiles, which share their adapters.
-SRQ_DEV uint32_t place_of_block() {
-    const uint32_t x = blockIdx.x % 8, per = gridDim.x / 8, rem = gridDim.x % 8;
-    return x * per + min(x, rem) + blockIdx.x / 8;
+SRQ_DEV uint32_t place_of(uint32_t b, uint32_t total) {
+    const uint32_t x = b % 8, per = total / 8, rem = total % 8;
+    return x * per + min(x, rem) + b / 8;
 }
 
-// t of 64 tokens x 16 RT rows of A, K in steps of 64 through a ring of four LDS stages
-// (64 rows of x, 16 RT of A, 128 bytes each, the 16-byte chunks of a row exchanged by its
-// number).  A block takes as many rows of A as there are, up to 192: x then crosses the
-// fabric once.  The waves share the rows of A out first, and the tokens where those are
-// fewer than four fragments.
-constexpr int kStages = 4;
-
-template <int RT>
-__global__ __launch_bounds__(256) void lora_shrink_kernel(LoraArgs a, int groups, int nz) {
-    constexpr int kStage = (kTok + 16 * RT) * 128;
-    constexpr int PER = 2 + RT / 2;   // loads of a wave in a stage
-    constexpr int WR = RT < 4 ? RT : 4, WT = 4 / WR, FT = 4 / WT, FR = RT / WR;
-    static_assert(RT % 2 == 0 && WR * FR == RT && WR * WT == 4 && 2 * PER < 64, "waves");
-    __shared__ __attribute__((aligned(1024))) uint8_t smem[kStages * kStage];
+// t of 64 Q tokens x 16 RT rows of A, K in steps of 64 through a ring of NST stages in LDS
+// (64 Q rows of x, 16 RT of A, 128 bytes each, the 16-byte chunks of a row exchanged by its
+// number).  A block takes as many rows of A as there are, up to 192, so that x crosses the
+// fabric once; 128 tokens halve what A costs, which comes from L2 for every tile.  Eight
+// waves: 4 share the rows of A out, 2 the tokens.  The operands of half a step are read
+// beside the products of the half before, and the loads are spread over them: a wave
+// stalls on a burst of loads, and its products with it.
+template <int RT, int Q, int NST>
+__global__ __launch_bounds__(512) void lora_shrink_kernel(LoraArgs a, int groups, int nz) {
+    constexpr int kStage = (64 * Q + 16 * RT) * 128;
+    constexpr int PX = Q, PA = RT / 4, PER = PX + PA;   // loads of a wave in a stage
+    constexpr int FT = 2 * Q, FR = RT / 4;              // 16 x 16 products of a wave
+    static_assert(RT % 4 == 0 && (NST - 1) * PER < 64 && NST * kStage <= 160 * 1024, "ring");
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[NST * kStage];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const uint32_t at = place_of_block(), zs = uni(at / (uint32_t)nz);
-    const int z = (int)(at - zs * nz);
-    const uint32_t gy = groups * a.splits, tile = uni(zs / gy), part = zs - tile * gy;
+    // the blocks of z = 0 first: of the others most find no adapter left
+    const uint32_t live = gridDim.x / nz, zb = uni(blockIdx.x / live);
+    const uint32_t at = place_of(blockIdx.x - zb * live, live);
+    const int z = (int)zb;
+    const uint32_t gy = groups * a.splits, tile = uni(at / gy), part = at - tile * gy;
     const int split = (int)uni(part / (uint32_t)groups), rg = (int)(part - split * groups) * 16 * RT;
-    const int64_t m0 = (int64_t)tile * kTok;
+    const int64_t m0 = (int64_t)tile * (64 * Q);
     const int K = (int)a.K, k_lo = split * a.kc;
     const int steps = (int)uni((uint32_t)((min(K, k_lo + a.kc) - k_lo + 63) / 64));
-    const int64_t rows = min((int64_t)kTok, a.M - m0);
+    const int64_t rows = min((int64_t)(64 * Q), a.M - m0);
     const uint32_t xbytes = uni((uint32_t)(2 * ((rows - 1) * a.xs + a.K)));
     const __amdgpu_buffer_rsrc_t xr = make_rsrc(a.x + m0 * a.xs, xbytes);
     const int arows = min(16 * RT, a.R - rg);
     const uint32_t ring0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void *)smem;
     const int r8 = lane >> 3, m = lane & 15, g = lane >> 4;
-    const int wr = wave % WR, wt = wave / WR;
+    const int wr = wave & 3, wt = wave >> 2;
 
     // byte offsets of this lane's chunks in step 0 of the split; rows past the last lie
     // outside the buffers and read zeros
-    uint32_t xo[2], ao[RT / 2];
-    int xk[2], ak[RT / 2];
+    uint32_t off[PER];
+    int ck[PER];
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
-        const int row = 8 * (2 * wave + q) + r8;
-        xk[q] = k_lo + 8 * ((lane & 7) ^ (row >> 1 & 7));
-        xo[q] = (uint32_t)(2 * (row * a.xs + xk[q]));
+    for (int q = 0; q < PER; ++q) {
+        const int row = 8 * (q < PX ? PX * wave + q : PA * wave + q - PX) + r8;
+        ck[q] = k_lo + 8 * ((lane & 7) ^ (row >> 1 & 7));
+        off[q] = (uint32_t)(2 * (row * (q < PX ? a.xs : a.K) + ck[q]));
     }
+    // LDS addresses of this lane's chunks of the wave's first rows
+    uint32_t xl[2], al[2];
 #pragma unroll
-    for (int q = 0; q < RT / 2; ++q) {
-        const int row = 8 * (RT / 2 * wave + q) + r8;
-        ak[q] = k_lo + 8 * ((lane & 7) ^ (row >> 1 & 7));
-        ao[q] = (uint32_t)(2 * (row * a.K + ak[q]));
+    for (int h = 0; h < 2; ++h) {
+        const int c = 16 * ((4 * h + g) ^ (m >> 1));
+        xl[h] = ring0 + (16 * FT * wt + m) * 128 + c;
+        al[h] = ring0 + 64 * Q * 128 + (16 * FR * wr + m) * 128 + c;
     }
 
-    Turns turns(a, m0, lane);
-    uint64_t same;
+    Turns<Q> turns(a, m0, lane);
+    uint64_t same[Q];
     for (int id; (id = turns.next(z, nz, same)) >= 0;) {
         const __amdgpu_buffer_rsrc_t ar =
             make_rsrc(a.a + ((int64_t)id * a.R + rg) * a.K, (int64_t)arows * a.K * 2);
-        auto issue = [&](int s) __attribute__((always_inline)) {
-            const uint32_t dst = ring0 + (s % kStages) * kStage;
+        auto issue = [&](int s, uint32_t dst, int q_lo, int q_hi) __attribute__((always_inline)) {
             const int left = K - 64 * s;   // past K: zeros, on both sides
+            dst += ring0;
 #pragma unroll
-            for (int q = 0; q < 2; ++q)
-                dma16(xr, xk[q] < left ? xo[q] + 128 * s : kOob, dst + (2 * wave + q) * 1024);
-#pragma unroll
-            for (int q = 0; q < RT / 2; ++q)
-                dma16(ar, ak[q] < left ? ao[q] + 128 * s : kOob,
-                      dst + kTok * 128 + (RT / 2 * wave + q) * 1024);
+            for (int q = 0; q < PER; ++q) {
+                if (q < q_lo || q >= q_hi) continue;
+                const uint32_t o = ck[q] < left ? off[q] + 128 * s : kOob;
+                if (q < PX) dma16(xr, o, dst + (PX * wave + q) * 1024);
+                else dma16(ar, o, dst + (8 * Q + PA * wave + q - PX) * 1024);
+            }
         };
         v4f acc[FT][FR];
 #pragma unroll
         for (int i = 0; i < FT; ++i)
 #pragma unroll
             for (int f = 0; f < FR; ++f) acc[i][f] = (v4f)0.f;
+        v8h xv[2][FT], av[2][FR];
+        auto fetch = [&](int h, uint32_t st) __attribute__((always_inline)) {
 #pragma unroll
-        for (int p = 0; p < kStages - 1; ++p)
-            if (p < steps) issue(p);
-        for (int s = 0; s < steps; ++s) {
-            const int ahead = min(kStages - 2, steps - 1 - s);
-            if (ahead == 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * PER) : "memory");
+            for (int i = 0; i < FT; ++i) xv[h][i] = lds16(xl[h] + st + i * 2048);
+#pragma unroll
+            for (int f = 0; f < FR; ++f) av[h][f] = lds16(al[h] + st + f * 2048);
+        };
+        auto wait = [&](int ahead) __attribute__((always_inline)) {   // loads of `ahead` steps stay
+            if (ahead >= 3) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(3 * PER) : "memory");
+            else if (ahead == 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * PER) : "memory");
             else if (ahead == 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PER) : "memory");
             else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            __builtin_amdgcn_s_barrier();
-            asm volatile("" ::: "memory");
-            if (s + kStages - 1 < steps) issue(s + kStages - 1);
-            const uint8_t *xs = smem + (s % kStages) * kStage, *as = xs + kTok * 128;
+        };
+        static_assert(NST <= 4, "wait");
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int c = 16 * ((4 * h + g) ^ (m >> 1));
-                v8h xv[FT], av[FR];
-#pragma unroll
-                for (int i = 0; i < FT; ++i)
-                    xv[i] = *reinterpret_cast<const v8h *>(xs + (16 * (FT * wt + i) + m) * 128 + c);
-#pragma unroll
-                for (int f = 0; f < FR; ++f)
-                    av[f] = *reinterpret_cast<const v8h *>(as + (16 * (FR * wr + f) + m) * 128 + c);
-#pragma unroll
-                for (int i = 0; i < FT; ++i)
-#pragma unroll
-                    for (int f = 0; f < FR; ++f) acc[i][f] = mfma16(xv[i], av[f], acc[i][f]);
-            }
-        }
-        // the ring is filled anew for the next adapter
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        for (int p = 0; p < NST; ++p)
+            if (p < steps) issue(p, p * kStage, 0, PER);
+        wait(min(NST - 1, steps - 1));
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
+        fetch(0, 0);
+        uint32_t st = 0, fst = 0;
+        int fill = steps;
+        for (int s = 0; s < steps; ++s) {
+            const uint32_t nst = st == (NST - 1) * kStage ? 0 : st + kStage;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                if (h == 0) {
+                    fetch(1, st);
+                } else {
+                    // this wave has read all of step s, and step s + 1 has landed ..
+                    if (s + 1 < steps) wait(min(NST - 2, steps - 2 - s));
+                    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                    // .. and so it is for all waves
+                    __builtin_amdgcn_s_barrier();
+                    asm volatile("" ::: "memory");
+                    if (s + 1 < steps) fetch(0, nst);
+                    fill = s + NST;
+                    fst = st;
+                }
+                if (fill < steps) issue(fill, fst, h ? 0 : (PER + 1) / 2, h ? (PER + 1) / 2 : PER);
+#pragma unroll
+                for (int i = 0; i < FT; ++i)
+#pragma unroll
+                    for (int f = 0; f < FR; ++f) acc[i][f] = mfma16(xv[h][i], av[h][f], acc[i][f]);
+            }
+            st = nst;
+        }
 #pragma unroll
         for (int i = 0; i < FT; ++i)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int row = 16 * (FT * wt + i) + 4 * g + e;
-                if (!(same >> row & 1)) continue;
+                if (!(same[row / 64] >> (row & 63) & 1)) continue;
                 float *t = a.t + ((int64_t)split * a.M + m0 + row) * a.R + rg;
 #pragma unroll
                 for (int f = 0; f < FR; ++f) {
@@ -286,8 +408,16 @@ __global__ __launch_bounds__(256) void lora_join_kernel(LoraArgs a) {
     for (int i = 0; i < V; ++i) {
         const int k = 64 * i + lane;
         v[i] = 0.f;
-        if (k < a.r)
-            for (int p = 0; p < a.splits; ++p) v[i] += a.t[(int64_t)p * a.M * a.R + at + k];
+        if (k >= a.r) continue;
+        for (int p = 0; p < a.splits; p += 4) {   // four loads in flight
+            float q[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                q[u] = a.t[(int64_t)min(p + u, a.splits - 1) * a.M * a.R + at + k];
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (p + u < a.splits) v[i] += q[u];
+        }
         top = fmaxf(top, fabsf(v[i]));
     }
     top = wave_max(top);
@@ -309,40 +439,58 @@ __global__ __launch_bounds__(256) void lora_join_kernel(LoraArgs a) {
 
 struct __attribute__((packed, aligned(2))) U8h { v8h v; };
 
-// out of 64 tokens x 128 columns of one slice: four waves of 32 x 64.  t (both halves) and
-// B pass through LDS, KW ranks at a time: in operand order neighbouring lanes are
-// different rows, each an access of its own.  The products go through the wave's own rows
-// of B's place, so that y and out move in 16 bytes a lane; y is loaded ahead.
+// A barrier for what passes through LDS: loads and stores of global memory stay in flight.
+SRQ_DEV void lds_barrier() {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// Between the lanes of a wave: what one wrote to LDS, another reads.
+SRQ_DEV void wave_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// out of 64 tokens x a run of tiles of 128 columns of one slice: four waves of 32 x 64.  t
+// (both halves, all ranks) stays in LDS, B passes through it KW ranks and one tile at a
+// time, the next part loaded beside the products of this one: in operand order
+// neighbouring lanes are different rows, each an access of its own.  A tile's products go
+// through the place of its B, so that y and out move in 16 bytes a lane; y is loaded a
+// tile ahead.
 constexpr int kCols = 128;
 
-template <int KW>
-__global__ __launch_bounds__(256, KW == 64 ? 3 : 4) void lora_expand_kernel(LoraArgs a, int tiles_n, int nz) {
+template <int KW, int NCH>
+__global__ __launch_bounds__(256, KW == 16 ? 4 : NCH == 4 ? 1 : NCH == 2 ? 2 : 3)
+void lora_expand_kernel(LoraArgs a, int runs, int run, int nz) {
     constexpr int C = KW / 8, RPD = 64 / C;        // chunks of a row, rows of a load
-    constexpr int kT = kTok * 2 * KW, kB = kCols * 2 * KW;
-    constexpr int kW = 64 + 4, kP = 4 * 16 * kW * 4;   // 16 rows of products a wave
-    __shared__ __attribute__((aligned(1024))) uint8_t smem[2 * kT + (kB > kP ? kB : kP)];
+    constexpr int kT = kTok * 2 * KW, kB = kCols * 2 * KW;   // a part of t, of B
+    constexpr int kP = 4 * 16 * 64 * 4, kBuf = kB > kP ? kB : kP;   // 16 rows of products a wave
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[2 * NCH * kT + 2 * kBuf];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int wm = wave >> 1, wn = wave & 1, rr = lane & 31, g = lane >> 5;
-    const uint32_t at = place_of_block();
-    const uint32_t zt = uni(at / (uint32_t)nz);
-    const int z = (int)(at - zt * nz);
-    const uint32_t tm = uni(zt / (uint32_t)tiles_n);
-    const int tile = (int)(zt - tm * tiles_n);
+    const uint32_t live = gridDim.x / nz, zb = uni(blockIdx.x / live);
+    const uint32_t zt = place_of(blockIdx.x - zb * live, live);
+    const int z = (int)zb;
+    const uint32_t tm = uni(zt / (uint32_t)runs);
+    const int at = (int)(zt - tm * runs);
     const int64_t m0 = (int64_t)tm * kTok;
     int s = 0;
-    while (tile >= a.tile_end[s]) ++s;
+    while (at >= a.run_end[s]) ++s;
     const int n_hi = a.col_end[s];
-    const int nb = (s ? a.col_end[s - 1] : 0) + (tile - (s ? a.tile_end[s - 1] : 0)) * kCols;
+    const int nb = (s ? a.col_end[s - 1] : 0) + (at - (s ? a.run_end[s - 1] : 0)) * run * kCols;
+    const int tiles = min(run, (n_hi - nb + kCols - 1) / kCols);
     // place in the row-wise pass: 8 rows of 64 columns an instruction
     const int pr = 32 * wm + (lane >> 3), pn = nb + 64 * wn + 8 * (lane & 7);
-    const bool full = pn + 8 <= n_hi;
     // 32-bit offsets from the tile's first row
     const f16 *y0 = a.y + m0 * a.ys;
     f16 *o0 = a.out + m0 * a.os;
     const float *u0 = a.unit + m0 * a.slices + s;
     const uint32_t ys = (uint32_t)a.ys, os = (uint32_t)a.os;
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void *)smem;
+    constexpr int kBuf0 = 2 * NCH * kT;
     // the 16-byte chunks of a row exchanged by its number: 16 rows of one chunk then lie
     // in all banks
     auto swz = [](int row, int c) __attribute__((always_inline)) {
@@ -353,113 +501,169 @@ __global__ __launch_bounds__(256, KW == 64 ? 3 : 4) void lora_expand_kernel(Lora
     const int64_t t0 = m0 * a.R + s * a.r;
     const __amdgpu_buffer_rsrc_t hr = make_rsrc(a.th + t0, tbytes);
     const __amdgpu_buffer_rsrc_t lr = make_rsrc(a.tl + t0, tbytes);
-    const uint32_t bbytes = uni((uint32_t)(2 * min(kCols, n_hi - nb) * a.r));
+    const uint32_t bbytes = uni((uint32_t)(2 * (int64_t)min(run * kCols, n_hi - nb) * a.r));
 
-    Turns turns(a, m0, lane);
-    uint64_t same;
-    for (int id; (id = turns.next(z, nz, same)) >= 0;) {
-        const __amdgpu_buffer_rsrc_t br = make_rsrc(a.b + ((int64_t)id * a.N + nb) * a.r, bbytes);
-        v16f acc[2] = {(v16f)0.f, (v16f)0.f};
-        v8h yv[4];
-        float unit[4];
-#pragma unroll 1
-        for (int k0 = 0; k0 < a.r; k0 += KW) {
-            __syncthreads();   // LDS is free
-            constexpr int DT = kT / 4096 ? kT / 4096 : 1, DB = kB / 4096;
+    // what does not wait for the adapters' numbers: t, the factors and the first of y (rows
+    // of other adapters are not used)
 #pragma unroll
-            for (int q = 0; q < DT; ++q) {
-                const int i = DT * wave + q, row = RPD * i + lane / C;
-                const int k = k0 + 8 * swz(row, lane % C);
-                if (i * 1024 >= kT) break;         // narrow rows: two waves' loads are enough
-                const uint32_t off = k < a.r ? (uint32_t)(2 * (row * a.R + k)) : kOob;
-                dma16(hr, off, lds0 + i * 1024);
-                dma16(lr, off, lds0 + kT + i * 1024);
-            }
+    for (int c = 0; c < NCH; ++c) {
+        constexpr int DT = kT / 4096 ? kT / 4096 : 1;
+#pragma unroll
+        for (int q = 0; q < DT; ++q) {
+            const int i = DT * wave + q, row = RPD * i + lane / C;
+            const int k = KW * c + 8 * swz(row, lane % C);
+            if (i * 1024 >= kT) break;         // narrow rows: two waves' loads are enough
+            const uint32_t off = k < a.r ? (uint32_t)(2 * (row * a.R + k)) : kOob;
+            dma16(hr, off, lds0 + 2 * c * kT + i * 1024);
+            dma16(lr, off, lds0 + (2 * c + 1) * kT + i * 1024);
+        }
+    }
+    v8h yv[4];
+    float unit[4];
+    auto load_y = [&](v8h (&v)[4], int tile) __attribute__((always_inline)) {
+        const int n = pn + tile * kCols;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const uint32_t row = pr + 8 * q;
+            if (row < rows && n + 8 <= n_hi)
+                v[q] = reinterpret_cast<const U8h *>(y0 + (row * ys + n))->v;
+        }
+    };
+    load_y(yv, 0);
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+        if (pr + 8 * q < rows) unit[q] = u0[(uint32_t)(pr + 8 * q) * a.slices];
+
+    Turns<1> turns(a, m0, lane);
+    uint64_t same1[1];
+    bool first = true;
+    for (int id; (id = turns.next(z, nz, same1)) >= 0;) {
+        const uint64_t same = same1[0];
+        const __amdgpu_buffer_rsrc_t br = make_rsrc(a.b + ((int64_t)id * a.N + nb) * a.r, bbytes);
+        auto load_b = [&](int tile, int c, int buf) __attribute__((always_inline)) {
+            constexpr int DB = kB / 4096;
 #pragma unroll
             for (int q = 0; q < DB; ++q) {
                 const int i = DB * wave + q, row = RPD * i + lane / C;
-                const int k = k0 + 8 * swz(row, lane % C);
-                dma16(br, k < a.r ? (uint32_t)(2 * (row * a.r + k)) : kOob, lds0 + 2 * kT + i * 1024);
+                const int k = KW * c + 8 * swz(row, lane % C);
+                dma16(br, k < a.r ? (uint32_t)(2 * ((tile * kCols + row) * a.r + k)) : kOob,
+                      lds0 + kBuf0 + buf * kBuf + i * 1024);
             }
-            if (k0 == 0) {
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const uint32_t row = pr + 8 * q;
-                    if (!(same >> row & 1)) continue;
-                    unit[q] = u0[row * a.slices];
-                    if (full) yv[q] = reinterpret_cast<const U8h *>(y0 + (row * ys + pn))->v;
-                }
-            }
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            __syncthreads();
-#pragma unroll
-            for (int st = 0; st < KW / 16; ++st) {
-                const int row = 32 * wm + rr, c = row * 2 * KW + 16 * swz(row, 2 * st + g);
-                const v8h h = *reinterpret_cast<const v8h *>(smem + c);
-                const v8h l = *reinterpret_cast<const v8h *>(smem + kT + c);
-#pragma unroll
-                for (int f = 0; f < 2; ++f) {
-                    const int col = 64 * wn + 32 * f + rr;
-                    const v8h w = *reinterpret_cast<const v8h *>(smem + 2 * kT + col * 2 * KW +
-                                                                 16 * swz(col, 2 * st + g));
-                    acc[f] = mfma32(h, w, acc[f]);
-                    acc[f] = mfma32(l, w, acc[f]);
-                }
-            }
+        };
+        if (!first) {
+            lds_barrier();   // the last adapter's products have been read
+            load_y(yv, 0);
         }
-        __syncthreads();   // B's place is free
-        float *mine = reinterpret_cast<float *>(smem + 2 * kT) + wave * 16 * kW;
+        first = false;
+        load_b(0, 0, 0);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        int buf = 0;
+#pragma unroll 1
+        for (int tile = 0; tile < tiles; ++tile) {
+            v16f acc[2] = {(v16f)0.f, (v16f)0.f};
+            v8h yn[4];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {   // 16 rows at a time
+            for (int c = 0; c < NCH; ++c) {
+                lds_barrier();   // this part of B is there, and the other buffer free
+                if (c + 1 < NCH) {
+                    load_b(tile, c + 1, buf ^ 1);
+                } else if (tile + 1 < tiles) {
+                    load_b(tile + 1, 0, buf ^ 1);
+                    load_y(yn, tile + 1);
+                }
+                const uint8_t *tp = smem + 2 * c * kT, *bp = smem + kBuf0 + buf * kBuf;
+#pragma unroll 2
+                for (int st = 0; st < KW / 16; ++st) {
+                    const int row = 32 * wm + rr, o = row * 2 * KW + 16 * swz(row, 2 * st + g);
+                    const v8h h = *reinterpret_cast<const v8h *>(tp + o);
+                    const v8h l = *reinterpret_cast<const v8h *>(tp + kT + o);
 #pragma unroll
-            for (int v = 0; v < 8; ++v)
+                    for (int f = 0; f < 2; ++f) {
+                        const int col = 64 * wn + 32 * f + rr;
+                        const v8h w = *reinterpret_cast<const v8h *>(bp + col * 2 * KW +
+                                                                     16 * swz(col, 2 * st + g));
+                        acc[f] = mfma32(h, w, acc[f]);
+                        acc[f] = mfma32(l, w, acc[f]);
+                    }
+                }
+                if (c + 1 < NCH) {
+                    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                    buf ^= 1;
+                }
+            }
+            lds_barrier();   // the tile's B has been read
+            // 16 rows at a time; columns of rows 4 .. 7 and 12 .. 15 exchanged by halves, so
+            // that the two halves of the wave write to different banks
+            float *mine = reinterpret_cast<float *>(smem + kBuf0 + buf * kBuf) + wave * 16 * 64;
+            const int n = pn + tile * kCols;
+            const bool full = n + 8 <= n_hi;
 #pragma unroll
-                for (int f = 0; f < 2; ++f)
-                    mine[(8 * (v / 4) + 4 * g + v % 4) * kW + 32 * f + rr] = acc[f][8 * i + v];
-            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+            for (int i = 0; i < 2; ++i) {
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                const uint32_t row = pr + 16 * i + 8 * q;
-                const float u = unit[2 * i + q];
-                const float *p = mine + (8 * q + (lane >> 3)) * kW + 8 * (lane & 7);
-                const v4f lo = *reinterpret_cast<const v4f *>(p);
-                const v4f hi = *reinterpret_cast<const v4f *>(p + 4);
-                if (!(same >> row & 1)) continue;
-                f16 *o = o0 + (row * os + pn);
-                if (full) {
-                    v8h v = yv[2 * i + q];
+                for (int v = 0; v < 8; ++v)
+#pragma unroll
+                    for (int f = 0; f < 2; ++f)
+                        mine[(8 * (v / 4) + 4 * g + v % 4) * 64 + 32 * (f ^ g) + rr] =
+                            acc[f][8 * i + v];
+                wave_fence();
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    const int lrow = 8 * q + (lane >> 3);
+                    const float *p = mine + lrow * 64 + (8 * (lane & 7) ^ 32 * (lrow >> 2 & 1));
+                    const v4f lo = *reinterpret_cast<const v4f *>(p);
+                    const v4f hi = *reinterpret_cast<const v4f *>(p + 4);
+                    const float u = unit[2 * i + q];
+                    v8h &v = yv[2 * i + q];
+                    if (!full) {
+                        const uint32_t row = pr + 16 * i + 8 * q;
+#pragma unroll
+                        for (int k = 0; k < 8; ++k)
+                            if (row < rows && n + k < n_hi) v[k] = y0[row * ys + n + k];
+                    }
 #pragma unroll
                     for (int k = 0; k < 8; ++k)
                         v[k] = f16_rn(__builtin_fmaf(k < 4 ? lo[k & 3] : hi[k & 3], u, (float)v[k]));
-                    reinterpret_cast<U8h *>(o)->v = v;
+                }
+                wave_fence();
+            }
+            // the next part of B and of y are there, and so are the stores of the last
+            // tile; those of this one stay in flight
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const uint32_t row = pr + 8 * q;
+                if (!(same >> row & 1)) continue;
+                f16 *o = o0 + (row * os + n);
+                if (full) {
+                    reinterpret_cast<U8h *>(o)->v = yv[q];
                 } else {
-                    const f16 *y = y0 + (row * ys + pn);
 #pragma unroll
                     for (int k = 0; k < 8; ++k)
-                        if (pn + k < n_hi)
-                            o[k] = f16_rn(
-                                __builtin_fmaf(k < 4 ? lo[k & 3] : hi[k & 3], u, (float)y[k]));
+                        if (n + k < n_hi) o[k] = yv[q][k];
                 }
             }
-            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+            for (int q = 0; q < 4; ++q) yv[q] = yn[q];
+            buf ^= 1;
         }
     }
+    // no load into LDS outlives the block
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     // tokens without an adapter
-    if (z == 0 && a.out != a.y && turns.invalid && pn < n_hi)
+    if (z == 0 && a.out != a.y && turns.invalid[0])
         for (int q = 0; q < 4; ++q) {
             const uint32_t row = pr + 8 * q;
-            if (!(turns.invalid >> row & 1)) continue;
-            const f16 *y = y0 + (row * ys + pn);
-            f16 *o = o0 + (row * os + pn);
-            if (full) {
-                reinterpret_cast<U8h *>(o)->v = reinterpret_cast<const U8h *>(y)->v;
-            } else {
-                for (int k = 0; k < 8; ++k)
-                    if (pn + k < n_hi) o[k] = y[k];
+            if (!(turns.invalid[0] >> row & 1)) continue;
+            for (int tile = 0; tile < tiles; ++tile) {
+                const int n = pn + tile * kCols;
+                const f16 *y = y0 + (row * ys + n);
+                f16 *o = o0 + (row * os + n);
+                if (n + 8 <= n_hi) {
+                    reinterpret_cast<U8h *>(o)->v = reinterpret_cast<const U8h *>(y)->v;
+                } else {
+                    for (int k = 0; k < 8; ++k)
+                        if (n + k < n_hi) o[k] = y[k];
+                }
             }
         }
 }
@@ -468,18 +672,20 @@ __global__ __launch_bounds__(256, KW == 64 ? 3 : 4) void lora_expand_kernel(Lora
 constexpr int64_t kFew = 64;
 
 struct Plan {
-    int rt, groups, splits, kc;
+    int rt, tokens, groups, splits, kc;   // rt 0: few tokens
 };
 
 Plan plan_of(int64_t M, int64_t R, int64_t K) {
-    Plan p{0, 1, 1, 0};
+    Plan p{0, 0, 1, 1, 0};
     if (M <= kFew) return p;
-    p.rt = R <= 32 ? 2 : R <= 64 ? 4 : R <= 128 ? 8 : 12;
+    p.rt = R <= 64 ? 4 : R <= 128 ? 8 : 12;
+    p.tokens = M > 1024 ? 128 : 64;
     p.groups = (int)srq_cdiv(R, 16 * p.rt);
-    // a block for each place on the 256 CUs (two of the small ones fit one), of at least
-    // 8 steps
-    const int64_t blocks = srq_cdiv(M, kTok) * p.groups, steps = srq_cdiv(K, 64);
-    int64_t s = (p.rt <= 4 ? 512 : 256) / blocks;
+    // blocks of at least 8 steps for four in five of the places on the 256 CUs (two of the
+    // small ones fit one): the rest takes the second adapters of tiles that have two.
+    // 4875 tokens of four requests, rank 64 x 3, K = 8192: 89 us, with all places taken 97.
+    const int64_t blocks = srq_cdiv(M, p.tokens) * p.groups, steps = srq_cdiv(K, 64);
+    int64_t s = (p.rt == 4 ? 400 : 200) / blocks;
     if (s > steps / 8) s = steps / 8;
     if (s > 16) s = 16;
     if (s < 1) s = 1;
@@ -487,6 +693,14 @@ Plan plan_of(int64_t M, int64_t R, int64_t K) {
     p.kc = (int)(64 * per);
     p.splits = (int)srq_cdiv(steps, per);
     return p;
+}
+
+template <int RT>
+void launch_shrink(const LoraArgs &a, const Plan &p, unsigned blocks, int nz, hipStream_t st) {
+    if (p.tokens == 128)
+        lora_shrink_kernel<RT, 2, 3><<<blocks, 512, 0, st>>>(a, p.groups, nz);
+    else
+        lora_shrink_kernel<RT, 1, RT == 8 ? 3 : 4><<<blocks, 512, 0, st>>>(a, p.groups, nz);
 }
 
 // t, and with many tokens its two halves and factors
@@ -527,7 +741,6 @@ extern "C" int srq_lora_add(const void *y, int64_t y_stride, const void *x, int6
         a.N += slice_cols[i];
         tiles += srq_cdiv(slice_cols[i], kCols);
         a.col_end[i] = (int)a.N;
-        a.tile_end[i] = (int)tiles;
     }
     if (M == 0) return SRQ_OK;
     SRQ_CHECK_ARG(y && x && ids && out && (adapters == 0 || (lora_a && lora_b)),
@@ -541,9 +754,7 @@ extern "C" int srq_lora_add(const void *y, int64_t y_stride, const void *x, int6
     const Plan p = plan_of(M, rank * slices, K);
     SRQ_CHECK_ARG(ws && srq_aligned(ws, 16) && ws_bytes >= workspace(p, M, rank * slices, slices),
                   "lora_add: the workspace is missing or too small");
-    // a launch has fewer than 2^32 threads in x
-    SRQ_CHECK_ARG(srq_cdiv(M, kTok) * tiles < 1 << 24 && M * slices < 1 << 26,
-                  "lora_add: shape out of range");
+    SRQ_CHECK_ARG(M * slices < 1 << 26, "lora_add: shape out of range");
     a.y = (const f16 *)y;
     a.x = (const f16 *)x;
     a.a = (const f16 *)lora_a;
@@ -567,6 +778,24 @@ extern "C" int srq_lora_add(const void *y, int64_t y_stride, const void *x, int6
     a.splits = p.splits;
     a.kc = p.kc;
     hipStream_t st = (hipStream_t)stream;
+    if (M <= kFew && rank <= 32 && K <= kFewK) {
+        // One launch where the blocks' rows of A, each block its own, are little enough to
+        // come from L2 in the time of a launch: us a call, one launch / two: 1 token, rank
+        // 16, 4096 x 4096 6.8 / 10.1; 32 tokens, q/k/v of 4096 + 2 x 1024 7.2 / 9.8.
+        int64_t blocks = 0;
+        for (int64_t i = 0; i < slices; ++i) {
+            blocks += srq_cdiv(slice_cols[i], kFewCols);
+            a.run_end[i] = (int)blocks;
+        }
+        if (blocks * M * rank * K * 2 <= 32 << 20) {
+            const dim3 grid((unsigned)blocks, (unsigned)M);
+            if (rank <= 8) lora_one_kernel<1><<<grid, 512, 0, st>>>(a);
+            else if (rank <= 16) lora_one_kernel<2><<<grid, 512, 0, st>>>(a);
+            else lora_one_kernel<4><<<grid, 512, 0, st>>>(a);
+            SRQ_LAUNCH_CHECK("lora_add");
+            return SRQ_OK;
+        }
+    }
     if (M <= kFew) {
         lora_shrink_few_kernel<<<dim3((unsigned)srq_cdiv(a.R, 4), (unsigned)M), 256, 0, st>>>(a);
         SRQ_LAUNCH_CHECK("lora_add");
@@ -574,35 +803,40 @@ extern "C" int srq_lora_add(const void *y, int64_t y_stride, const void *x, int6
         SRQ_LAUNCH_CHECK("lora_add (second product)");
         return SRQ_OK;
     }
-    // Neighbouring blocks share out a tile's adapters: a tile of single-token requests has
-    // up to 64, and few tiles then leave the CUs idle; and where one of many tiles has two
-    // adapters, the second does not wait for the first.
-    auto shares = [&](int64_t blocks) {
-        int64_t z = srq_cdiv(1024, blocks), most = adapters < kTok ? adapters : kTok;
-        if (z > most) z = most;
+    // Several blocks share out a tile's adapters where there are idle CUs: a tile of
+    // single-token requests has up to 64.
+    auto shares = [&](int64_t blocks, int64_t places) {
+        int64_t z = places / blocks;
+        if (z > adapters) z = adapters;
+        if (z > 64) z = 64;
         return (int)(z < 1 ? 1 : z);
     };
-    const unsigned tm = (unsigned)srq_cdiv(M, kTok), gy = (unsigned)(p.groups * p.splits);
-    const int z1 = shares((int64_t)tm * gy), z2 = shares((int64_t)tm * tiles);
-    SRQ_CHECK_ARG((int64_t)tm * tiles * z2 < 1 << 24 && (int64_t)tm * gy * z1 < 1 << 24,
-                  "lora_add: shape out of range");
-    const unsigned grid = tm * gy * z1;
+    // runs of tiles that leave about four blocks a CU
+    int64_t run = srq_cdiv(M, kTok) * tiles / 1280, runs = 0;
+    run = run < 1 ? 1 : run > 8 ? 8 : run;
+    for (int64_t i = 0; i < slices; ++i) {
+        runs += srq_cdiv(slice_cols[i], run * kCols);
+        a.run_end[i] = (int)runs;
+    }
+    const int64_t b1 = srq_cdiv(M, p.tokens) * p.groups * p.splits, b2 = srq_cdiv(M, kTok) * runs;
+    const int z1 = shares(b1, 512), z2 = shares(b2, 1024);
+    // a launch has fewer than 2^32 threads in x
+    SRQ_CHECK_ARG(b1 * z1 < 1 << 23 && b2 * z2 < 1 << 24, "lora_add: shape out of range");
     switch (p.rt) {
-    case 2: lora_shrink_kernel<2><<<grid, 256, 0, st>>>(a, p.groups, z1); break;
-    case 4: lora_shrink_kernel<4><<<grid, 256, 0, st>>>(a, p.groups, z1); break;
-    case 8: lora_shrink_kernel<8><<<grid, 256, 0, st>>>(a, p.groups, z1); break;
-    default: lora_shrink_kernel<12><<<grid, 256, 0, st>>>(a, p.groups, z1); break;
+    case 4: launch_shrink<4>(a, p, (unsigned)(b1 * z1), z1, st); break;
+    case 8: launch_shrink<8>(a, p, (unsigned)(b1 * z1), z1, st); break;
+    default: launch_shrink<12>(a, p, (unsigned)(b1 * z1), z1, st); break;
     }
     SRQ_LAUNCH_CHECK("lora_add");
     lora_join_kernel<<<(unsigned)srq_cdiv(M * slices, 4), 256, 0, st>>>(a);
     SRQ_LAUNCH_CHECK("lora_add (join)");
-    const unsigned blocks = (unsigned)(tm * tiles * z2);
-    if (rank <= 16)
-        lora_expand_kernel<16><<<blocks, 256, 0, st>>>(a, (int)tiles, z2);
-    else if (rank <= 32)
-        lora_expand_kernel<32><<<blocks, 256, 0, st>>>(a, (int)tiles, z2);
-    else
-        lora_expand_kernel<64><<<blocks, 256, 0, st>>>(a, (int)tiles, z2);
+    const dim3 grid((unsigned)(b2 * z2));
+    const int n = (int)runs, w = (int)run;
+    if (rank <= 16) lora_expand_kernel<16, 1><<<grid, 256, 0, st>>>(a, n, w, z2);
+    else if (rank <= 32) lora_expand_kernel<32, 1><<<grid, 256, 0, st>>>(a, n, w, z2);
+    else if (rank <= 64) lora_expand_kernel<64, 1><<<grid, 256, 0, st>>>(a, n, w, z2);
+    else if (rank <= 128) lora_expand_kernel<64, 2><<<grid, 256, 0, st>>>(a, n, w, z2);
+    else lora_expand_kernel<64, 4><<<grid, 256, 0, st>>>(a, n, w, z2);
     SRQ_LAUNCH_CHECK("lora_add (second product)");
     return SRQ_OK;
 }

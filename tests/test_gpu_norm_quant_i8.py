@@ -32,7 +32,8 @@ def _check(x, got, residual=None, weight=None, eps=1e-5, mean_dim=None, clip=1.0
 
 # every length class: a wave a row (512, 1024), blocks, the long form; odd lengths
 SIZES = [(1, 1), (3, 2), (5, 7), (2, 8), (9, 511), (4, 512), (6, 513), (3, 1000), (5, 1025),
-         (2, 2047), (1, 2048), (3, 2049), (1, 4096), (7, 4097), (33, 5120), (2, 8191), (3, 8192),
+         (2, 2047), (1, 2048), (3, 2049), (1, 4096), (7, 4097), (33, 5120), (600, 5120),
+         (520, 4096), (513, 8192), (514, 11008), (520, 16000), (2, 8191), (3, 8192),
          (2, 8200), (2, 14336), (3, 16385), (2, 28672), (1, 32768), (3, 32769), (2, 40007)]
 
 
