@@ -31,6 +31,10 @@ __all__ = [
     "w4a4_linear_moe_asym",
     "qk_norm_rope",
     "w4a16_linear",
+    "rmsnorm_quant_i8",
+    "sym_quant_dynamic_i8",
+    "w4a8_linear",
+    "lora_add",
     "PackedQuantizedTensor",
 ]
 
@@ -52,7 +56,8 @@ class ShapeHandler:
 
 class PackedQuantizedTensor:
     """Quantized-activation carrier (kernel.py:32-52): packed int4 codes
-    [..., K/2] u8, per-token fp16 scales [..., 1], zeros (asym only)."""
+    [..., K/2] u8, per-token fp16 scales [..., 1], zeros (asym only); or int8 codes
+    [..., K] with fp32 scales [..., 1]."""
 
     def __init__(self, quantized_x: torch.Tensor, scales_x: torch.Tensor,
                  zeros_x: torch.Tensor | None = None):
@@ -234,6 +239,27 @@ def w4a16_linear(x, weight, scales, zeros=None, bias=None):
     """fp16 x [..., K] through 4-bit weights u8 [N, K / 2] with scales (and zero
     points) [N, K / group] for each group of input columns: fp16 [..., N]."""
     return _CUDA.w4a16_linear(x.contiguous(), weight, scales, zeros, bias)
+
+
+def rmsnorm_quant_i8(x, eps, mean_dim=None, residual=None, weight=None, clip_ratio=1.0,
+                     return_norm=False, out=None):
+    """The residual's addition, RMSNorm and int8 quantization of rows fp16 [..., n]."""
+    return _CUDA.rmsnorm_quant_i8(x, eps, mean_dim, residual, weight, clip_ratio, return_norm, out)
+
+
+def sym_quant_dynamic_i8(x, clip_ratio=1.0):
+    """int8 codes [..., n] and fp32 scales [..., 1] of rows fp16 [..., n]."""
+    return _CUDA.sym_quant_dynamic_i8(x, clip_ratio)
+
+
+def w4a8_linear(A, a_scale, B, b_scale, bias=None, residual=None, out=None):
+    """int8 rows [..., K] through packed int4 weights: fp16 [..., N]."""
+    return _CUDA.w4a8_linear(A, a_scale, B, b_scale, bias, residual, out)
+
+
+def lora_add(y, x, lora_a, lora_b, ids, scaling=None, slices=None, out=None):
+    """The low-rank adapters of a batch's tokens beside a projection that they share."""
+    return _CUDA.lora_add(y, x, lora_a, lora_b, ids, scaling, slices, out)
 
 
 def swiglu(gate, up):

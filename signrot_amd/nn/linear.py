@@ -19,7 +19,8 @@ class Linear4bit(torch.nn.Module):
     subtracts zeros_x ⊗ weight_sum from the int32 product, as the reference's
     matmul_ui4_si4 -> matmul_colrow_i8_i32 -> `x -= zeros` -> sym_dequant
     chain does (linear.py:35-50); weight_sum = sum_i4(weight) is computed on
-    the first such call and kept as a non-persistent buffer.
+    the first such call and kept as a non-persistent buffer.  With int8 codes
+    (Quantizer8bit) the product runs on w4a8_linear.
     forward(fp16 tensor) dequantizes the weight and calls F.linear, as the
     reference does (linear.py:31-34).
     """
@@ -46,6 +47,8 @@ class Linear4bit(torch.nn.Module):
             w_deq = quant_utils.sym_dequant(quant_utils.unpack_i4(self.weight), self.weight_scales)
             return torch.nn.functional.linear(x, w_deq, self.bias)
         q, s = x.quantized_x, x.scales_x
+        if q.dtype == torch.int8:
+            return kernel.w4a8_linear(q, s, self.weight, self._scales_f16(), self.bias)
         assert q.shape[-1] * 2 % 32 == 0, "K: {} must be a multiple of 32".format(q.shape[-1] * 2)
         if x.zeros_x is not None:
             if not hasattr(self, "weight_sum"):

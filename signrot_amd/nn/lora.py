@@ -1,0 +1,76 @@
+"""Low-rank adapters of many requests beside a projection that they share."""
+import torch
+
+from ..functional import kernel
+
+
+class LoraAdapters(torch.nn.Module):
+    """Up to `adapters` low-rank adapters of one projection, of ranks up to `rank` (a
+    multiple of 8 up to 256): forward(y, x, ids) adds to the projection's output y [...,
+    out] for the input x [..., in] each token's own scaling * (x A^T) B^T, its adapter
+    being ids[token] (int32; outside [0, adapters): none).
+
+    out_features may be a tuple: the widths of a projection that is several in one
+    (q/k/v, gate/up), each slice with an A and B of its own.
+
+    Buffers: lora_a f16 [adapters, slices * rank, in], lora_b f16 [adapters, out, rank],
+    scaling f32 [adapters].  A smaller rank is padded with zeros."""
+
+    lora_a: torch.Tensor
+    lora_b: torch.Tensor
+    scaling: torch.Tensor
+
+    def __init__(self, in_features, out_features, rank, adapters):
+        super().__init__()
+        widths = (out_features,) if isinstance(out_features, int) else tuple(out_features)
+        if rank <= 0 or rank % 8 or rank > 256:
+            raise ValueError("rank must be a multiple of 8 up to 256")
+        if in_features % 8 or not 1 <= len(widths) <= 8 or min(widths) <= 0:
+            raise ValueError("in_features must be a multiple of 8, out_features 1 to 8 widths")
+        self.in_features, self.widths, self.rank, self.adapters = in_features, widths, rank, adapters
+        self.register_buffer("lora_a", torch.zeros(adapters, len(widths) * rank, in_features,
+                                                   dtype=torch.float16))
+        self.register_buffer("lora_b", torch.zeros(adapters, sum(widths), rank,
+                                                   dtype=torch.float16))
+        self.register_buffer("scaling", torch.ones(adapters, dtype=torch.float32))
+
+    @torch.no_grad()
+    def load(self, index, a, b, scaling=1.0):
+        """Adapter `index` becomes scaling * B A: a [r, in] and b [out, r] (r <= rank),
+        or with several slices a sequence of each, None where a slice has no adapter."""
+        if not 0 <= index < self.adapters:
+            raise ValueError(f"adapter {index} outside [0, {self.adapters})")
+        if isinstance(a, torch.Tensor) or a is None:
+            a, b = (a,), (b,)
+        if len(a) != len(self.widths) or len(b) != len(self.widths):
+            raise ValueError(f"expected {len(self.widths)} slices")
+        for m, l, n in zip(a, b, self.widths):
+            if (m is None) != (l is None):
+                raise ValueError("a slice has both a and b, or neither")
+            if m is not None and (m.dim() != 2 or l.dim() != 2 or m.shape[1] != self.in_features
+                                  or l.shape != (n, m.shape[0]) or m.shape[0] > self.rank):
+                raise ValueError(f"expected a [r, {self.in_features}] and b [{n}, r] with r <= "
+                                 f"{self.rank}, got {tuple(m.shape)} and {tuple(l.shape)}")
+        self.clear(index)
+        at = 0
+        for i, (m, l, n) in enumerate(zip(a, b, self.widths)):
+            if m is not None:
+                r = m.shape[0]
+                self.lora_a[index, i * self.rank: i * self.rank + r] = m.to(self.lora_a)
+                self.lora_b[index, at: at + n, :r] = l.to(self.lora_b)
+            at += n
+        self.scaling[index] = scaling
+
+    @torch.no_grad()
+    def clear(self, index):
+        """Adapter `index` adds nothing."""
+        self.lora_a[index] = 0
+        self.lora_b[index] = 0
+        self.scaling[index] = 1
+
+    def forward(self, y, x, ids, out=None):
+        return kernel.lora_add(y, x, self.lora_a, self.lora_b, ids, self.scaling, self.widths, out)
+
+    def extra_repr(self):
+        return (f"{self.in_features} -> {self.widths}, rank {self.rank}, "
+                f"{self.adapters} adapters")

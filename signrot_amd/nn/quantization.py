@@ -34,6 +34,15 @@ class Quantizer(QuantizerBase):
         return kernel.PackedQuantizedTensor(quantized_x, scales_x)
 
 
+class Quantizer8bit(QuantizerBase):
+    """Per-token symmetric int8 quantizer in one launch -> PackedQuantizedTensor with
+    int8 codes and fp32 scales, which Linear4bit takes as it takes int4 codes: the same
+    weights with activations of twice the bits, where 4 cost too much."""
+
+    def forward(self, x) -> kernel.PackedQuantizedTensor:
+        return kernel.PackedQuantizedTensor(*kernel.sym_quant_dynamic_i8(x, self.clip_ratio))
+
+
 class SymQuantizer(QuantizerBase):
     """Symmetric quantizer with a configurable bit width
     (quantization.py:31-56); the fused kernel serves the int4, clip 1 case."""

@@ -23,6 +23,7 @@ from ..functional import kernel
 from ..functional.hadamard import _inv_sqrt_f32, get_hadK, matmul_hadU_cuda
 from ..functional.quantization import rtn_weight_pack
 from ..nn.derived import derived
+from ..nn.lora import LoraAdapters
 from ..nn.normalization import RMSNorm
 from .kv_cache import HFCacheAdapter, MultiLayerPagedKVCache4Bit, qkv_prefill_of
 from .kv_cache_i8 import MultiLayerPagedKVCache8Bit
@@ -40,6 +41,12 @@ def _refuse_held(cache, layer_idx, tokens):
     if isinstance(cache, MultiLayerPagedKVCache4Bit) and tokens != 1:
         raise ValueError("after the prefill, update() appends one token per request")
     raise RuntimeError("prefill: the cache already holds this layer's context")
+
+
+def _plain_norm(n):
+    """Whether a fused kernel does all that calling the norm module would."""
+    return (type(n) is RMSNorm and "forward" not in vars(n) and not n._forward_pre_hooks
+            and not n._forward_hooks)
 
 
 def rope_cos_sin(positions, head_dim, theta, device):
@@ -61,17 +68,24 @@ class W4A4LlamaDecodeLayer(torch.nn.Module):
     rotation).  qk_norm: each query and key head goes through an RMSNorm before
     the rotary embedding (fp16 weights q_norm, k_norm [head_dim]).
 
+    act_bits=8: the linears take int8 activations (w4a8_linear) over the same weights.
+    add_adapters() puts low-rank adapters beside the projections; forward() and prefill()
+    then take adapter_ids, one adapter a request.
+
     The cache may also be a MultiLayerPagedKVCache8Bit.  Its decode step runs the
     q/k/v pass in fp32 with one rounding, so there the fused and the op-by-op form
     agree within fp16 roundings, and not bit for bit."""
 
     def __init__(self, hidden, n_heads, n_kv_heads, head_dim, ffn, layer_idx=0, eps=1e-5,
-                 rope_theta=500000.0, qk_norm=False):
+                 rope_theta=500000.0, qk_norm=False, act_bits=4):
         super().__init__()
+        if act_bits not in (4, 8):
+            raise ValueError(f"act_bits must be 4 or 8, got {act_bits}")
         assert hidden == n_heads * head_dim and n_heads % n_kv_heads == 0
         self.hidden, self.n_heads, self.n_kv = hidden, n_heads, n_kv_heads
         self.head_dim, self.ffn, self.layer_idx = head_dim, ffn, layer_idx
-        self.rope_theta = rope_theta
+        self.rope_theta, self.act_bits = rope_theta, act_bits
+        self.adapters = torch.nn.ModuleDict()
         self.input_layernorm = RMSNorm(hidden, eps)
         self.post_attention_layernorm = RMSNorm(hidden, eps)
         nqkv = (n_heads + 2 * n_kv_heads) * head_dim
@@ -128,7 +142,7 @@ class W4A4LlamaDecodeLayer(torch.nn.Module):
         return kernel.rope_qk(q, k, cos, sin)
 
     def forward(self, hidden_states, cache, cos, sin, trace=None, fused=True,
-                attention_mask=None):
+                attention_mask=None, adapter_ids=None):
         """hidden_states fp16 [B, 1, hidden]; cos/sin fp16 [1 or B, 1, head_dim]
         for the new position; returns fp16 [B, 1, hidden].  The cache must
         already hold this layer's context (its first update was a prefill).
@@ -136,7 +150,13 @@ class W4A4LlamaDecodeLayer(torch.nn.Module):
         1 per decoded token ([B, prompt + steps]; it gives each request's
         length), else None.  With a dict `trace`, the intermediates are
         stored in it (checkers) and the op-by-op path runs; otherwise
-        (fused=True) the fused kernels run, with bit-identical results."""
+        (fused=True) the fused kernels run, with bit-identical results.
+        adapter_ids: int32 [B], each request's adapter (outside [0, adapters):
+        none), or None for the layer itself; with them, and with act_bits=8,
+        there is one path, whatever `fused` is."""
+        if self.act_bits == 8 or adapter_ids is not None:
+            return self._forward_rows(hidden_states, cache, cos, sin, trace, attention_mask,
+                                      adapter_ids)
         if fused and trace is None:
             return self._forward_fused(hidden_states, cache, cos, sin, attention_mask)
         return self._forward_ops(hidden_states, cache, cos, sin, trace, attention_mask)
@@ -218,7 +238,148 @@ class W4A4LlamaDecodeLayer(torch.nn.Module):
         x2 = self._attn_out(attn, x2, keep)
         return self._mlp(x2, keep).view(B, 1, self.hidden)
 
-    def prefill(self, hidden_states, cache, cos, sin, attention_mask=None, trace=None):
+    # ------------------------------------------- 8-bit activations, adapters
+
+    def add_adapters(self, rank, adapters, names=("qkv", "o", "gu", "down")):
+        """Low-rank adapters beside the projections `names`: LoraAdapters modules in
+        self.adapters, to be filled with their load() (q, k, v and gate, up are slices of
+        one).  The inputs that they see are the projections' own: the norms' outputs, the
+        attention output ahead of its head-axis rotation, and the SwiGLU ahead of
+        down_proj's rotation and signs."""
+        D, Hq, Hk = self.head_dim, self.n_heads, self.n_kv
+        shapes = {"qkv": (self.hidden, (Hq * D, Hk * D, Hk * D)), "o": (self.hidden, self.hidden),
+                  "gu": (self.hidden, (self.ffn, self.ffn)), "down": (self.ffn, self.hidden)}
+        for name in names:
+            if name not in shapes:
+                raise ValueError(f"adapters of {name!r}: expected one of {tuple(shapes)}")
+            self.adapters[name] = LoraAdapters(*shapes[name], rank, adapters).to(self.w_qkv.device)
+        return self.adapters
+
+    def _adapt(self, name, y, x, ids):
+        """y, with the adapters beside projection `name` added in place."""
+        if ids is None or name not in self.adapters:
+            return y
+        return self.adapters[name](y, x, ids, out=y)
+
+    def _norm_rows(self, norm, x2, residual, keep):
+        """The codes, scales and fp16 rows (None unless `keep`) behind a norm of x2 (+
+        residual), and that sum."""
+        if self.act_bits == 8 and _plain_norm(norm):
+            out = kernel.rmsnorm_quant_i8(x2, norm.eps, norm.mean_dim, residual, return_norm=keep)
+            return (*out[:2], out[-1] if keep else None, x2 if residual is None else out[2])
+        h = x2 if residual is None else x2 + residual
+        if not _plain_norm(norm):
+            y = norm(h)
+            return (*self._quant_rows(y), y, h)
+        out = _CUDA.rmsnorm_quant(h, norm.eps, norm.mean_dim, return_norm=keep)
+        return (*out[:2], out[2] if keep else None, h)
+
+    def _rows_linear(self, name, q, s, residual=None):
+        w, ws = getattr(self, f"w_{name}"), getattr(self, f"s_{name}")
+        if self.act_bits == 8:
+            return kernel.w4a8_linear(q, s, w, ws, None, residual)
+        if residual is None:
+            return _CUDA.w4a4_linear(q, s.view(-1), w, ws)
+        return _CUDA.w4a4_linear_residual(q, s.view(-1), w, ws, residual)
+
+    def _quant_rows(self, x):
+        return kernel.sym_quant_dynamic_i8(x) if self.act_bits == 8 else kernel.sym_quant_dynamic(x)
+
+    def _rows_qkv(self, x2, ids, trace, keep):
+        q1, s1, n1, _ = self._norm_rows(self.input_layernorm, x2, None,
+                                        trace is not None or (ids is not None
+                                                              and "qkv" in self.adapters))
+        keep("norm1", n1)
+        keep("q1", q1)
+        keep("s1", s1)
+        qkv = self._adapt("qkv", self._rows_linear("qkv", q1, s1), n1, ids)
+        keep("qkv", qkv)
+        return qkv
+
+    def _rows_rest(self, attn, x2, ids, trace, keep):
+        """From the attention output [R, Hq, D] on; x2 the layer's input rows."""
+        R, Hq = x2.shape[0], self.n_heads
+        attn = attn.reshape(R, Hq, self.head_dim)
+        keep("attn", attn)
+        if 8 <= Hq <= 64 and Hq & (Hq - 1) == 0 and self.head_dim == 128:
+            rot = _CUDA.head_had_quant(attn, _inv_sqrt_f32(Hq), return_rot=True)[2]
+        else:
+            rot = matmul_hadU_cuda(attn.transpose(-1, -2).contiguous(), None, 1)
+            rot = rot.transpose(-1, -2).reshape(R, self.hidden)
+        keep("attn_rot", rot)
+        oq, os = self._quant_rows(rot)
+        keep("oq", oq)
+        keep("os", os)
+        o = self._adapt("o", self._rows_linear("o", oq, os), attn.reshape(R, self.hidden), ids)
+        keep("o", o)
+        q2, s2, n2, x2 = self._norm_rows(self.post_attention_layernorm, o, x2,
+                                         trace is not None or (ids is not None
+                                                               and "gu" in self.adapters))
+        keep("resid1", x2)
+        keep("norm2", n2)
+        keep("q2", q2)
+        keep("s2", s2)
+        gu = self._adapt("gu", self._rows_linear("gu", q2, s2), n2, ids)
+        keep("gu", gu)
+        a = kernel.swiglu(gu[:, : self.ffn], gu[:, self.ffn:])
+        keep("act", a)
+        if self.act_bits == 8:
+            rot = _CUDA.online_hadamard(a, self.down_hadk, self.down_k, self.down_sign)
+            keep("act_rot", rot)
+            qd, sd = self._quant_rows(rot)
+        else:
+            qd, sd = _CUDA.had_sign_quant(a, self.down_hadk, self.down_k, self.down_sign)
+        keep("down_q", qd)
+        keep("down_s", sd)
+        out = self._rows_linear("down", qd, sd, x2)
+        keep("down", out)
+        return self._adapt("down", out, a, ids)
+
+    def _forward_rows(self, hidden_states, cache, cos, sin, trace, attention_mask, adapter_ids):
+        """The decode step with 8-bit activations or adapters: the projections on
+        w4a8_linear (w4a4_linear), the attention the cache's own."""
+        B = hidden_states.shape[0]
+        x2, keep = hidden_states.reshape(B, self.hidden), self._keeper(trace)
+        ids = self._adapter_rows(adapter_ids, B, 1)
+        qkv = self._rows_qkv(x2, ids, trace, keep)
+        if type(cache) is MultiLayerPagedKVCache4Bit and not self.qk_norm:
+            attn = cache.update_qkv_decode(qkv, cos, sin, self.layer_idx, self.n_heads,
+                                           attention_mask)
+        elif type(cache) is MultiLayerPagedKVCache8Bit:
+            if not cache._filled[self.layer_idx]:
+                raise RuntimeError("forward: the layer has no prefill yet")
+            norm = (self.q_norm, self.k_norm, self.eps) if self.qk_norm else (None, None, None)
+            q = cache.update_qkv(qkv.view(B, 1, -1), cos, sin, self.layer_idx, self.n_heads, *norm,
+                                 attention_mask)
+            attn = cache.attend(q, self.layer_idx)
+        else:
+            heads = qkv.view(B, 1, -1, self.head_dim)
+            q, k, v = (t.contiguous() for t in heads.split((self.n_heads, self.n_kv, self.n_kv), 2))
+            q, k = self._rope(q, k, cos, sin)
+            attn = cache.update(k, v, self.layer_idx, {"attention_mask": attention_mask})(q)
+        return self._rows_rest(attn, x2, ids, trace, keep).view(B, 1, self.hidden)
+
+    def _prefill_rows(self, hidden_states, cache, cos, sin, attention_mask, trace, adapter_ids):
+        B, T, _ = hidden_states.shape
+        x2, keep = hidden_states.reshape(B * T, self.hidden), self._keeper(trace)
+        ids = self._adapter_rows(adapter_ids, B, T)
+        qkv = self._rows_qkv(x2, ids, trace, keep)
+        attn = self._prefill_attention(qkv, cache, cos, sin, attention_mask, B, T)
+        return self._rows_rest(attn, x2, ids, trace, keep).view(B, T, self.hidden)
+
+    def _adapter_rows(self, adapter_ids, B, T):
+        """One adapter a row of B requests of T tokens, or None."""
+        if adapter_ids is None:
+            return None
+        if not self.adapters:
+            raise ValueError("adapter_ids without adapters: call add_adapters() first")
+        if adapter_ids.shape != (B,):
+            raise ValueError(f"adapter_ids must be [{B}], one a request")
+        ids = adapter_ids.to(torch.int32)
+        return ids.contiguous() if T == 1 else ids.repeat_interleave(T, output_size=B * T)
+
+    def prefill(self, hidden_states, cache, cos, sin, attention_mask=None, trace=None,
+                adapter_ids=None):
         """The layer's first update: T tokens per request
         (modeling_llama.py:26-100 with the cache's first update,
         kv_cache.py:295-395).  hidden_states fp16 [B, T, hidden]; cos/sin
@@ -231,7 +392,10 @@ class W4A4LlamaDecodeLayer(torch.nn.Module):
         padding positions are computed but carry no meaning.  With a dict
         `trace` the intermediates are stored in it and the op-by-op path
         runs; otherwise the fused kernels do where they have a form for the
-        sizes, with bit-identical results."""
+        sizes, with bit-identical results.  adapter_ids as for forward()."""
+        if self.act_bits == 8 or adapter_ids is not None:
+            return self._prefill_rows(hidden_states, cache, cos, sin, attention_mask, trace,
+                                      adapter_ids)
         if trace is None and self._prefill_fusable(hidden_states):
             return self._prefill_fused(hidden_states, cache, cos, sin, attention_mask)
         B, T, _ = hidden_states.shape
@@ -264,8 +428,7 @@ class W4A4LlamaDecodeLayer(torch.nn.Module):
         either: hadamard_transform starts at 8), and nothing that only calls
         of the modules and torch's own adds would see: hooks on the norms or
         another norm in their place, gradients of the residual stream."""
-        plain = all(type(n) is RMSNorm and "forward" not in vars(n)
-                    and not n._forward_pre_hooks and not n._forward_hooks
+        plain = all(_plain_norm(n)
                     for n in (self.input_layernorm, self.post_attention_layernorm))
         hooked = torch.nn.modules.module._global_forward_pre_hooks or \
             torch.nn.modules.module._global_forward_hooks
@@ -283,11 +446,30 @@ class W4A4LlamaDecodeLayer(torch.nn.Module):
         views -> head_had_quant -> o_proj GEMM + residual -> rmsnorm_quant ->
         gate/up GEMM -> swiglu_had_sign_quant -> down GEMM + residual."""
         B, T, _ = hidden_states.shape
-        D, Hq, Hk = self.head_dim, self.n_heads, self.n_kv
+        D, Hq = self.head_dim, self.n_heads
         x2 = hidden_states.reshape(B * T, self.hidden).contiguous()
         n1, n2 = self.input_layernorm, self.post_attention_layernorm
         q1, s1 = _CUDA.rmsnorm_quant(x2, n1.eps, n1.mean_dim)
         qkv = _CUDA.w4a4_linear(q1, s1.view(-1), self.w_qkv, self.s_qkv)
+        attn = self._prefill_attention(qkv, cache, cos, sin, attention_mask, B, T)
+        qa, sa = _CUDA.head_had_quant(attn.view(B * T, Hq, D), _inv_sqrt_f32(Hq))
+        x2 = _CUDA.w4a4_linear_residual(qa, sa.view(-1), self.w_o, self.s_o, x2)
+        q2, s2 = _CUDA.rmsnorm_quant(x2, n2.eps, n2.mean_dim)
+        # The weights themselves and not decode's derived copy: a prefill may be
+        # the layer's first call, on any stream or inside a graph capture, after
+        # any change of the weights, and a program that only prefills holds them
+        # once.  GEMM and swiglu_had_sign_quant at 101 / 512 / 2048 rows of 8B
+        # widths: 34 / 100 / 287 us (from the copy 29 / 85 / 252, with the copy
+        # made each time 106 / 162 / 327).
+        qd, sd = self._swiglu_rotate_quant(
+            _CUDA.w4a4_linear(q2, s2.view(-1), self.w_gu, self.s_gu))
+        out = _CUDA.w4a4_linear_residual(qd, sd.view(-1), self.w_down, self.s_down, x2, out=x2)
+        return out.view(B, T, self.hidden)
+
+    def _prefill_attention(self, qkv, cache, cos, sin, attention_mask, B, T):
+        """The rotary embedding (and norms) of a prompt's q/k/v rows, the cache's first
+        update and the causal attention: [B, T, Hq, D]."""
+        D, Hq, Hk = self.head_dim, self.n_heads, self.n_kv
         fill = None
         if attention_mask is None and not self.qk_norm:
             fill = qkv_prefill_of(cache)
@@ -306,25 +488,12 @@ class W4A4LlamaDecodeLayer(torch.nn.Module):
             if not isinstance(out, tuple):
                 raise RuntimeError("prefill: the cache already holds this layer's context")
             k, v = out
-        attn = _CUDA.prefill_attention(q, k, v, attention_mask, causal=True)
-        qa, sa = _CUDA.head_had_quant(attn.view(B * T, Hq, D), _inv_sqrt_f32(Hq))
-        x2 = _CUDA.w4a4_linear_residual(qa, sa.view(-1), self.w_o, self.s_o, x2)
-        q2, s2 = _CUDA.rmsnorm_quant(x2, n2.eps, n2.mean_dim)
-        # The weights themselves and not decode's derived copy: a prefill may be
-        # the layer's first call, on any stream or inside a graph capture, after
-        # any change of the weights, and a program that only prefills holds them
-        # once.  GEMM and swiglu_had_sign_quant at 101 / 512 / 2048 rows of 8B
-        # widths: 34 / 100 / 287 us (from the copy 29 / 85 / 252, with the copy
-        # made each time 106 / 162 / 327).
-        qd, sd = self._swiglu_rotate_quant(
-            _CUDA.w4a4_linear(q2, s2.view(-1), self.w_gu, self.s_gu))
-        out = _CUDA.w4a4_linear_residual(qd, sd.view(-1), self.w_down, self.s_down, x2, out=x2)
-        return out.view(B, T, self.hidden)
+        return _CUDA.prefill_attention(q, k, v, attention_mask, causal=True)
 
     @staticmethod
     def _keeper(trace):
         def keep(name, t):
-            if trace is not None:
+            if trace is not None and t is not None:
                 trace[name] = t.clone()
         return keep
 

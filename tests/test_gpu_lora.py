@@ -41,7 +41,10 @@ CASES = [(1, 64, (40,), 8, 1), (1, 4096, (4096,), 16, 4), (3, 1000, (111, 7), 8,
          (65, 64, (40,), 8, 1), (70, 1000, (111, 77), 8, 5), (100, 4096, (300,), 16, 3),
          (200, 512, (256, 128, 129), 16, 7), (129, 2056, (1025,), 40, 4), (257, 320, (128,), 64, 64),
          (66, 72, (33, 260), 256, 3), (500, 1096, (65,), 128, 2), (321, 8, (5,), 8, 40),
-         (90, 96, (9, 8, 7, 6, 5, 4, 3, 2), 24, 6)]
+         (90, 96, (9, 8, 7, 6, 5, 4, 3, 2), 24, 6), (2, 16392, (20,), 8, 2), (3, 64, (2100, 9), 32, 2),
+         # tiles of 128 tokens; runs of several column tiles; more rows of A than a block's
+         (1100, 264, (700, 60), 16, 3), (1500, 520, (129,), 72, 5), (1300, 128, (20000, 300), 8, 4),
+         (1100, 96, (300,) * 8, 24, 6), (1200, 200, (600,), 200, 2)]
 
 
 @pytest.mark.parametrize("M,K,widths,r,L", CASES)

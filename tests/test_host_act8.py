@@ -101,3 +101,50 @@ def test_reference_quantizer_rounds_as_rational_numbers():
                    for v in near)
         for v, c in zip(row, codes):
             assert round(Fraction(v) / Fraction(float(scale[0]))) == c
+
+
+def test_lora_adapters_hold_what_is_loaded():
+    import torch
+    from signrot_amd.nn import LoraAdapters
+    ad = LoraAdapters(16, (24, 8), 8, 3)
+    a, b = torch.randn(4, 16), torch.randn(8, 4)
+    ad.load(2, (None, a), (None, b), 0.5)
+    assert torch.equal(ad.lora_a[2, 8:12], a.half()) and torch.equal(ad.lora_b[2, 24:, :4], b.half())
+    assert not ad.lora_a[2, :8].any() and not ad.lora_a[2, 12:].any() and not ad.lora_a[:2].any()
+    assert not ad.lora_b[2, :24].any() and not ad.lora_b[2, 24:, 4:].any()
+    assert ad.scaling.tolist() == [1, 1, 0.5]
+    # a smaller one in its place leaves nothing of it
+    ad.load(2, (torch.ones(1, 16), None), (torch.ones(24, 1), None))
+    assert ad.lora_a[2].sum() == 16 and ad.lora_b[2].sum() == 24 and ad.scaling[2] == 1
+    ad.clear(2)
+    assert not ad.lora_a.any() and not ad.lora_b.any()
+    one = LoraAdapters(16, 24, 8, 1)
+    one.load(0, torch.ones(8, 16), torch.ones(24, 8))
+    with pytest.raises(ValueError, match="outside"):
+        one.load(1, torch.ones(8, 16), torch.ones(24, 8))
+    before = one.lora_a.clone()
+    for x, y in [(torch.ones(9, 16), torch.ones(24, 9)), (torch.ones(8, 15), torch.ones(24, 8)),
+                 (torch.ones(8, 16), torch.ones(23, 8)), (torch.ones(8, 16), torch.ones(24, 7)),
+                 (torch.ones(16), torch.ones(24, 1)), (torch.ones(8, 16), None)]:
+        with pytest.raises(ValueError):
+            one.load(0, x, y)
+    with pytest.raises(ValueError, match="slices"):
+        ad.load(0, (a,), (b,))
+    assert torch.equal(one.lora_a, before)
+    for bad in [dict(rank=4), dict(rank=0), dict(rank=264), dict(in_features=12),
+                dict(out_features=()), dict(out_features=(8,) * 9), dict(out_features=(8, 0))]:
+        with pytest.raises(ValueError):
+            LoraAdapters(**{**dict(in_features=16, out_features=24, rank=8, adapters=1), **bad})
+
+
+def test_decode_layer_refuses_other_widths():
+    from signrot_amd.transformers.decode_layer import W4A4LlamaDecodeLayer
+    with pytest.raises(ValueError, match="act_bits"):
+        W4A4LlamaDecodeLayer(256, 2, 1, 128, 384, act_bits=6)
+    layer = W4A4LlamaDecodeLayer(256, 2, 1, 128, 384)
+    with pytest.raises(ValueError, match="adapters of"):
+        layer.add_adapters(8, 1, ("q",))
+    with pytest.raises(ValueError, match="rank"):
+        layer.add_adapters(12, 1)
+    assert set(layer.add_adapters(8, 2, ("o", "down"))) == {"o", "down"}
+    assert layer.adapters["down"].in_features == 384
