@@ -745,6 +745,7 @@ extern "C" int srq_lora_add(const void *y, int64_t y_stride, const void *x, int6
     if (M == 0) return SRQ_OK;
     SRQ_CHECK_ARG(y && x && ids && out && (adapters == 0 || (lora_a && lora_b)),
                   "lora_add: null pointer");
+    SRQ_CHECK_ARG(out != x, "lora_add: out may be y, not x");
     SRQ_CHECK_ARG(srq_aligned(x, 16) && srq_aligned(lora_a, 16) && srq_aligned(lora_b, 16) &&
                       x_stride % 8 == 0,
                   "lora_add: x (its rows too) and the adapters must be 16-byte aligned");
@@ -811,9 +812,11 @@ extern "C" int srq_lora_add(const void *y, int64_t y_stride, const void *x, int6
         if (z > 64) z = 64;
         return (int)(z < 1 ? 1 : z);
     };
-    // runs of tiles that leave about four blocks a CU
-    int64_t run = srq_cdiv(M, kTok) * tiles / 1280, runs = 0;
-    run = run < 1 ? 1 : run > 8 ? 8 : run;
+    // runs of up to 5 tiles that leave more than a block a CU: us a call, runs of 1 / 3 /
+    // 5: 504 tokens x 28672 columns (1792 tiles) 31 / 29 / 27, 300 x 4096 (160) 14.0 / 15.0
+    // / 16.9; 4876 x 10240 97 / 93 / 95, of 8 100.
+    int64_t run = srq_cdiv(M, kTok) * tiles / 352, runs = 0;
+    run = run < 1 ? 1 : run > 5 ? 5 : run;
     for (int64_t i = 0; i < slices; ++i) {
         runs += srq_cdiv(slice_cols[i], run * kCols);
         a.run_end[i] = (int)runs;

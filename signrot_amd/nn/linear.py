@@ -48,6 +48,8 @@ class Linear4bit(torch.nn.Module):
             return torch.nn.functional.linear(x, w_deq, self.bias)
         q, s = x.quantized_x, x.scales_x
         if q.dtype == torch.int8:
+            if x.zeros_x is not None:
+                raise RuntimeError("Linear4bit: int8 codes have no zero points")
             return kernel.w4a8_linear(q, s, self.weight, self._scales_f16(), self.bias)
         assert q.shape[-1] * 2 % 32 == 0, "K: {} must be a multiple of 32".format(q.shape[-1] * 2)
         if x.zeros_x is not None:

@@ -259,6 +259,10 @@ def test_copies_and_refusals():
         plain(h, _cache(4, 2, 9, 1), cos, sin, adapter_ids=ids)
     with pytest.raises(ValueError, match="one a request"):
         layer(h, _cache(4, 2, 9, 1), cos, sin, adapter_ids=ids[:1])
+    m = snn.Linear4bit(64, 16).to(DEV)
+    q, s = kernel.sym_quant_dynamic_i8(torch.ones(2, 64, dtype=torch.float16, device=DEV))
+    with pytest.raises(RuntimeError, match="zero points"):
+        m(kernel.PackedQuantizedTensor(q, s, torch.zeros(2, 1, dtype=torch.int8, device=DEV)))
     empty = MultiLayerPagedKVCache8Bit(2, 32, 32, DEV, 1, HKV, D)
     with pytest.raises(RuntimeError, match="no prefill"):
         layer(h, empty, cos, sin)

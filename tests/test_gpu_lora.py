@@ -178,6 +178,42 @@ def test_stream_and_graph(M):
             assert np.array_equal(to_np(out), want)
 
 
+@pytest.mark.parametrize("M", [3, 70])
+def test_offsets_past_32_bits(M):
+    """The last of adapters of 4.4 GB."""
+    rng = np.random.default_rng(M)
+    K, N, r, L = 64, 28672, 256, 300
+    y, x, la, lb, _ = _operands(rng, M, K, (N,), r, 1)
+    ad = torch.zeros(L, r, K, dtype=torch.float16, device=DEV)
+    bd = torch.zeros(L, N, r, dtype=torch.float16, device=DEV)
+    ad[-1], bd[-1] = to_dev(la[0]), to_dev(lb[0])
+    ids = np.full(M, L - 1, np.int32)
+    ids[1] = 0
+    got = to_np(_CUDA.lora_add(to_dev(y), to_dev(x), ad, bd, to_dev(ids)))
+    want, tol = ref.lora(y, x, la, lb, np.where(ids == 0, -1, 0), None, (N,))
+    assert (np.abs(got - want) <= tol).all()
+
+
+def test_two_streams_at_once():
+    rng = np.random.default_rng(5)
+    calls = []
+    for M, r in ((300, 16), (1200, 64)):
+        y, x, la, lb, sc = _operands(rng, M, 2048, (512, 128), r, 6)
+        ids = _ids(rng, M, 6, "runs")
+        t = [to_dev(v) for v in (y, x, la, lb, ids, sc)]
+        calls.append((t, to_np(_CUDA.lora_add(*t, (512, 128))), torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    outs = [[], []]
+    for _ in range(5):
+        for (t, _, s), o in zip(calls, outs):
+            with torch.cuda.stream(s):
+                o.append(_CUDA.lora_add(*t, (512, 128)))
+    torch.cuda.synchronize()
+    for (_, want, _), o in zip(calls, outs):
+        for got in o:
+            assert np.array_equal(to_np(got), want)
+
+
 def test_refusals():
     f16 = torch.float16
 
@@ -208,6 +244,9 @@ def test_refusals():
     refused("rank=4", la=z(3, 8, 64), lb=z(3, 48, 4))
     refused("K=60", la=z(3, 16, 60), x=z(4, 60))
     refused("GPU", y=y.cpu())
+    square = z(4, 64)
+    with pytest.raises(bad, match="not x"):
+        _CUDA.lora_add(z(4, 64), square, z(3, 8, 64), z(3, 64, 8), ids, out=square)
     with pytest.raises(bad, match="out must have"):
         _CUDA.lora_add(*ok, out=z(4, 40))
     assert _CUDA.lora_add(y[:0], x[:0], la, lb, ids[:0], None, (32, 16)).shape == (0, 48)

@@ -165,6 +165,29 @@ def test_many_rows():
     assert np.array_equal(to_np(got[1]), s) and np.array_equal(to_np(got[0]), q)
 
 
+def test_more_blocks_than_a_launch_dimension_takes():
+    rng = np.random.default_rng(6)
+    x = rng.standard_normal(((1 << 22) + 9, 8)).astype(np.float16)
+    got = _CUDA.sym_quant_dynamic_i8(to_dev(x))
+    q, s = ref.quant(x.astype(np.float64))
+    assert np.array_equal(to_np(got[1]), s) and np.array_equal(to_np(got[0]), q)
+
+
+def test_offsets_past_32_bits():
+    """Rows beyond element 2^31 of a strided buffer, sum in place."""
+    n, rows = 4099, 530000
+    x = torch.zeros(rows, n, dtype=torch.float16, device=DEV)
+    g = torch.Generator(device=DEV).manual_seed(1)
+    at = torch.tensor([0, 523776, 524288, rows - 1], device=DEV)
+    x[at] = torch.randn(4, n, device=DEV, generator=g).half()
+    r = torch.zeros_like(x)
+    r[at] = torch.randn(4, n, device=DEV, generator=g).half()
+    xs, rs = to_np(x[at]), to_np(r[at])
+    got = _CUDA.rmsnorm_quant_i8(x, 1e-5, residual=r, out=r)
+    _check(xs, [t[at] for t in got], rs)
+    assert not got[1][1:523776].any() and not got[0][1:1000].any()
+
+
 def test_stream_and_graph():
     """On a stream of its own and replayed on new inputs."""
     rng = np.random.default_rng(4)

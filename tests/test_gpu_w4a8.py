@@ -131,6 +131,46 @@ def test_stream_and_graph(M):
             assert np.array_equal(to_np(out), want)
 
 
+def test_offsets_past_32_bits():
+    """An output of 4.6 GB, and rows of activations beyond 4 GiB."""
+    rng = np.random.default_rng(3)
+    M, N, K = 40000, 57344, 32
+    a, sa, c, sb = _operands(rng, M, N, K)
+    out = _CUDA.w4a8_linear(*(to_dev(t) for t in (a, sa, ref.pack(c), sb)))
+    rows = np.array([0, 17, 37449, 39999])
+    want, tol = ref.linear(a[rows], sa[rows], c, sb)
+    assert (np.abs(to_np(out[torch.from_numpy(rows).to(DEV)]) - want) <= tol).all()
+    del out
+    M, N, K = 70000, 130, 65536
+    a = torch.randint(-128, 128, (M, K), dtype=torch.int8, device=DEV)
+    c = rng.integers(-8, 8, (N, K)).astype(np.int8)
+    sa, sb = rng.uniform(0.001, 0.01, M).astype(np.float32), sb[:N]
+    out = _CUDA.w4a8_linear(a, to_dev(sa), to_dev(ref.pack(c)), to_dev(sb))
+    rows = np.array([0, 32767, 32768, 65535, 65536, 69999])
+    want, tol = ref.linear(to_np(a[torch.from_numpy(rows).to(DEV)]), sa[rows], c, sb)
+    assert (np.abs(to_np(out[torch.from_numpy(rows).to(DEV)]) - want) <= tol).all()
+
+
+def test_two_streams_at_once():
+    """Products that are split over K, each with a workspace of its own."""
+    rng = np.random.default_rng(4)
+    calls = []
+    for M in (48, 130):
+        a, sa, c, sb = _operands(rng, M, 640, 8192)
+        t = [to_dev(v) for v in (a, sa, ref.pack(c), sb)]
+        calls.append((t, to_np(_CUDA.w4a8_linear(*t)), torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    outs = [[], []]
+    for _ in range(8):
+        for (t, _, s), o in zip(calls, outs):
+            with torch.cuda.stream(s):
+                o.append(_CUDA.w4a8_linear(*t))
+    torch.cuda.synchronize()
+    for (_, want, _), o in zip(calls, outs):
+        for got in o:
+            assert np.array_equal(to_np(got), want)
+
+
 def test_refusals():
     a = torch.zeros(4, 64, dtype=torch.int8, device=DEV)
     sa = torch.ones(4, device=DEV)

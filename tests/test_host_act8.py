@@ -59,14 +59,14 @@ def test_w4a8(lib, change, msg):
     (dict(r=0), "rank"), (dict(S=0), "slices"), (dict(S=9), "slices"), (dict(cols=None), "slices"),
     (dict(K=60), "K=60"), (dict(K=0), "K=0"), (dict(K=(1 << 20) + 8), "K="),
     (dict(widths=(0,)), "slice of"), (dict(widths=(-8,)), "slice of"), (dict(M=1 << 40), "range"),
-    (dict(x=None), "null"), (dict(ids=None), "null"), (dict(la=None), "null"),
+    (dict(x=None), "null"), (dict(ids=None), "null"), (dict(la=None), "null"), (dict(out=P), "not x"),
     (dict(x=ctypes.c_void_p(264)), "aligned"), (dict(lb=ctypes.c_void_p(258)), "aligned"),
     (dict(xs=65), "aligned"), (dict(xs=56), "row stride"), (dict(ys=39), "row stride"),
     (dict(os=39), "row stride"), (dict(xs=1 << 25), "row stride"), (dict(ws=None), "workspace"),
     (dict(wb=4 * 3 * 8 - 1), "workspace"), (dict(ws=ctypes.c_void_p(8)), "workspace")])
 def test_lora(lib, change, msg):
     a = dict(y=P, ys=40, x=P, xs=64, la=P, lb=P, ids=P, sc=None, M=3, K=64, L=2, r=8, S=1, cols=0,
-             out=P, os=40, ws=P, wb=4 * 3 * 8, st=None)
+             out=ctypes.c_void_p(512), os=40, ws=P, wb=4 * 3 * 8, st=None)
     widths = change.get("widths", (40,))
     a["cols"] = (ctypes.c_int64 * 9)(*widths)
     change = {k: v for k, v in change.items() if k != "widths"}
