@@ -520,16 +520,16 @@ void lora_expand_kernel(LoraArgs a, int runs, int run, int nz) {
     }
     v8h yv[4];
     float unit[4];
-    auto load_y = [&](v8h (&v)[4], int tile) __attribute__((always_inline)) {
+    auto load_y = [&](v8h (&v)[4], int tile, uint64_t mask) __attribute__((always_inline)) {
         const int n = pn + tile * kCols;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
             const uint32_t row = pr + 8 * q;
-            if (row < rows && n + 8 <= n_hi)
+            if ((mask >> row & 1) && n + 8 <= n_hi)
                 v[q] = reinterpret_cast<const U8h *>(y0 + (row * ys + n))->v;
         }
     };
-    load_y(yv, 0);
+    load_y(yv, 0, rows == kTok ? ~0ull : (1ull << rows) - 1);
 #pragma unroll
     for (int q = 0; q < 4; ++q)
         if (pr + 8 * q < rows) unit[q] = u0[(uint32_t)(pr + 8 * q) * a.slices];
@@ -552,7 +552,7 @@ void lora_expand_kernel(LoraArgs a, int runs, int run, int nz) {
         };
         if (!first) {
             lds_barrier();   // the last adapter's products have been read
-            load_y(yv, 0);
+            load_y(yv, 0, same);
         }
         first = false;
         load_b(0, 0, 0);
@@ -569,7 +569,7 @@ void lora_expand_kernel(LoraArgs a, int runs, int run, int nz) {
                     load_b(tile, c + 1, buf ^ 1);
                 } else if (tile + 1 < tiles) {
                     load_b(tile + 1, 0, buf ^ 1);
-                    load_y(yn, tile + 1);
+                    load_y(yn, tile + 1, same);
                 }
                 const uint8_t *tp = smem + 2 * c * kT, *bp = smem + kBuf0 + buf * kBuf;
 #pragma unroll 2
@@ -618,7 +618,7 @@ void lora_expand_kernel(LoraArgs a, int runs, int run, int nz) {
                         const uint32_t row = pr + 16 * i + 8 * q;
 #pragma unroll
                         for (int k = 0; k < 8; ++k)
-                            if (row < rows && n + k < n_hi) v[k] = y0[row * ys + n + k];
+                            if ((same >> row & 1) && n + k < n_hi) v[k] = y0[row * ys + n + k];
                     }
 #pragma unroll
                     for (int k = 0; k < 8; ++k)
