@@ -102,6 +102,9 @@ SRQ_DEV void wait_ahead(int ahead) {
 // each wave an eighth of K in units of 128 codes, which it streams through its own ring
 // of S stages in LDS (AR activation rows of 128 bytes, then 16 NT weight rows of 64)
 // without a barrier; the waves' int32 sums are joined through LDS at the end.
+// 1 x 4096 x 4096 3.8 us, a launch and one round trip; 16 rows of 28672 codes on 8192
+// columns 28.5 us, 4.1 TB/s of weights (22 us where they are cached): what a CU takes in,
+// with 16 rows as many bytes of rows as of weights.
 constexpr int W = 8;
 
 template <int AR, int NT, int S>
@@ -215,6 +218,10 @@ __global__ __launch_bounds__(W * 64) void w4a8_stream_kernel(A8Args a) {
 // (BM rows of 128 bytes, then BN rows of 64) that every wave fills with its share of
 // loads.  One barrier a step: behind it step s has landed for all and step s - 1, whose
 // stage is filled next, has been read by all.
+// Small tiles are bound by what a CU takes in: 101 rows, 14336 columns, K = 4096 18.1 us,
+// 0.5 MB a CU at 29 bytes a ns.  The large ones are bound by the instructions at the power
+// that the card gives them: 2048 rows, 28672 columns, K = 4096 215 us, 2.2 POPS, on zeros
+// 179 us.
 struct __attribute__((packed, aligned(2))) U8h { v8h v; };
 
 template <int BM, int BN>
@@ -480,7 +487,8 @@ __global__ __launch_bounds__(64 * WM * WN) void w4a8_tile_kernel(A8Args a) {
 }
 
 // Many rows: `whole` tiles of 256 x 256, a multiple of the 256 CUs, and the rest, where it
-// is half a round at most, as twice as many of 256 x 128.
+// is half a round at most, as twice as many of 256 x 128: 3.5 rounds of 2048 rows, 28672
+// columns, K = 4096 215 us, with the last in whole tiles 222.
 __global__ __launch_bounds__(512) void w4a8_large_kernel(A8Args a, uint32_t whole) {
     constexpr int kBytes = ring_bytes<256, 256, 2, 4, 3>();
     static_assert(ring_bytes<256, 128, 4, 2, 3>() <= kBytes, "ring");

@@ -6,18 +6,21 @@
 // t = x A^T (fp32, in the workspace), then out = y + t B^T, a launch each.  The adapters'
 // bytes bound few tokens, those of x, y and out many.
 //
-// Few tokens: each by itself.  A wave takes one row of A for one token, whole lines at a
-// time; then a thread takes one output column, whose row of B is r values, with t in
-// fp32 from LDS.
+// Few tokens, or little to read for each: each by itself.  A wave takes one row of A for
+// one token, whole lines at a time; then a thread takes one output column, whose row of B
+// is r values, with t in fp32 from LDS.  10 to 14 us a call: the two launches, from about
+// 60 MB on what L2 gives.  Blocks of one / 2 / 4 tokens, which read an adapter once that
+// they share: 500 tokens of 125 requests, rank 16, 4096 x 4096 19.5 / 17.2 / 18.5 us, of 500
+// 17.7 / 18.3 / 28.1.
 //
-// Many tokens: tiles of 64 consecutive ones, whose distinct adapters are found by ballots
-// (lane i holds the id of token i) and taken one after the other, or shared out among the
-// blocks in z; a request's tokens stand together, so a tile has one or two.  Rows of other
-// adapters are computed and not kept: never multiplied by zero, since another request's
-// infinities would then come through.  t is split over K where tiles are few, each part
-// stored for itself, and a launch between the two adds them in order.  In the second
-// product t is an fp16 number and the fp16 rest, scaled by a power of two of the token's
-// largest: 22 bits.
+// Many tokens: tiles of 64 or 128 consecutive ones, whose distinct adapters are found by
+// ballots (lane i holds the id of token i) and taken one after the other, or shared out
+// among the blocks in z; a request's tokens stand together, so a tile has one or two.
+// Rows of other adapters are computed and not kept: never multiplied by zero, since another
+// request's infinities would then come through.  t is split over K where tiles are few,
+// each part stored for itself, and a launch between the two adds them in order.  In the
+// second product t is an fp16 number and the fp16 rest, scaled by a power of two of the
+// token's largest: 22 bits.
 #include "common.h"
 
 namespace {
@@ -111,7 +114,9 @@ __global__ __launch_bounds__(256) void lora_expand_few_kernel(LoraArgs a) {
 
 // Few tokens and a small adapter in one launch: a block takes 1024 columns of a slice for
 // one token and computes that slice's t itself, from rows of A that then come from L2;
-// y and its rows of B are loaded meanwhile.  RV rows of A a wave (r <= 8 RV).
+// y and its rows of B are loaded meanwhile.  RV rows of A a wave (r <= 8 RV).  Dependent
+// round trips bound one token (id, A, the sums through LDS): 4.2 us at rank 16, 4096 x
+// 4096; L2 bounds 32 tokens, 25 MB in 5.4 to 7.4 us (q/k/v of 4096 + 2 x 1024).
 constexpr int kFewCols = 1024;
 constexpr int kFewK = 16384;
 
@@ -260,7 +265,9 @@ SRQ_DEV uint32_t place_of(uint32_t b, uint32_t total) {
 // fabric once; 128 tokens halve what A costs, which comes from L2 for every tile.  Eight
 // waves: 4 share the rows of A out, 2 the tokens.  The operands of half a step are read
 // beside the products of the half before, and the loads are spread over them: a wave
-// stalls on a burst of loads, and its products with it.
+// stalls on a burst of loads, and its products with it.  What a CU takes in bounds it,
+// about 40 bytes a ns: 4876 tokens x 192 rows of A, K = 8192, 42 us, 20 of them the second
+// adapters of three tiles.
 template <int RT, int Q, int NST>
 __global__ __launch_bounds__(512) void lora_shrink_kernel(LoraArgs a, int groups, int nz) {
     constexpr int kStage = (64 * Q + 16 * RT) * 128;
@@ -392,7 +399,8 @@ __global__ __launch_bounds__(512) void lora_shrink_kernel(LoraArgs a, int groups
 }
 
 // The splits' parts of t added in order, as an fp16 number, the fp16 rest and a factor
-// for each token and slice: a wave each.
+// for each token and slice: a wave each.  A launch and one round trip, 3 to 4 us; 8 us for
+// 4876 tokens x 192.
 __global__ __launch_bounds__(256) void lora_join_kernel(LoraArgs a) {
     const int lane = threadIdx.x & 63;
     const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -458,7 +466,7 @@ SRQ_DEV void wave_fence() {
 // time, the next part loaded beside the products of this one: in operand order
 // neighbouring lanes are different rows, each an access of its own.  A tile's products go
 // through the place of its B, so that y and out move in 16 bytes a lane; y is loaded a
-// tile ahead.
+// tile ahead.  y and out bound it: 4876 tokens x 10240 columns, rank 64, 46 us, 4.4 TB/s.
 constexpr int kCols = 128;
 
 template <int KW, int NCH>
@@ -668,11 +676,21 @@ void lora_expand_kernel(LoraArgs a, int runs, int run, int nz) {
         }
 }
 
-// Tokens up to which each is taken by itself.
+// Tokens taken by themselves: up to 64, and up to 1024 where what they read of their
+// adapters comes from L2 in the time of the tiles' third launch.  us a call, by themselves /
+// in tiles: 100 tokens, rank 64, 4096 x 4096 (100 MiB) of 4 requests 15.0 / 14.2, of 100
+// 21.5 / 54; 224 tokens, rank 16, 4096 x 4096 (56 MiB) of 4 requests 10.9 / 13.6, of 56
+// 11.1 / 21.6; 500 tokens, q/k/v of 4096 + 2 x 1024 (281 MiB) of 4 29 / 14, of 125 36 / 36.
 constexpr int64_t kFew = 64;
+constexpr int64_t kFewMost = 1024;
+constexpr int64_t kFewBytes = 96 << 20;
+
+bool few_tokens(int64_t M, int64_t N, int64_t K, int64_t rank, int64_t R) {
+    return M <= kFew || (M <= kFewMost && 2 * M * (R * K + N * rank) <= kFewBytes);
+}
 
 struct Plan {
-    int rt, tokens, groups, splits, kc;   // rt 0: few tokens
+    int rt, tokens, groups, splits, kc;   // rt 0: always few tokens
 };
 
 Plan plan_of(int64_t M, int64_t R, int64_t K) {
@@ -779,7 +797,8 @@ extern "C" int srq_lora_add(const void *y, int64_t y_stride, const void *x, int6
     a.splits = p.splits;
     a.kc = p.kc;
     hipStream_t st = (hipStream_t)stream;
-    if (M <= kFew && rank <= 32 && K <= kFewK) {
+    const bool few = few_tokens(M, a.N, K, rank, a.R);
+    if (few && rank <= 32 && K <= kFewK) {
         // One launch where the blocks' rows of A, each block its own, are little enough to
         // come from L2 in the time of a launch: us a call, one launch / two: 1 token, rank
         // 16, 4096 x 4096 6.8 / 10.1; 32 tokens, q/k/v of 4096 + 2 x 1024 7.2 / 9.8.
@@ -797,7 +816,7 @@ extern "C" int srq_lora_add(const void *y, int64_t y_stride, const void *x, int6
             return SRQ_OK;
         }
     }
-    if (M <= kFew) {
+    if (few) {
         lora_shrink_few_kernel<<<dim3((unsigned)srq_cdiv(a.R, 4), (unsigned)M), 256, 0, st>>>(a);
         SRQ_LAUNCH_CHECK("lora_add");
         lora_expand_few_kernel<<<dim3((unsigned)srq_cdiv(a.N, 256), (unsigned)M), 256, 0, st>>>(a);

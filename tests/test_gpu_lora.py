@@ -37,14 +37,19 @@ def _ids(rng, M, L, kind):
 CASES = [(1, 64, (40,), 8, 1), (1, 4096, (4096,), 16, 4), (3, 1000, (111, 7), 8, 5),
          (5, 520, (300,), 24, 3), (32, 4096, (512, 128, 128), 16, 32), (64, 256, (130,), 64, 9),
          (2, 8, (1,), 8, 2), (7, 3144, (64, 3), 256, 2), (33, 128, (9, 8, 7, 6, 5, 4, 3, 2), 8, 4),
-         # the tiled form
          (65, 64, (40,), 8, 1), (70, 1000, (111, 77), 8, 5), (100, 4096, (300,), 16, 3),
          (200, 512, (256, 128, 129), 16, 7), (129, 2056, (1025,), 40, 4), (257, 320, (128,), 64, 64),
          (66, 72, (33, 260), 256, 3), (500, 1096, (65,), 128, 2), (321, 8, (5,), 8, 40),
          (90, 96, (9, 8, 7, 6, 5, 4, 3, 2), 24, 6), (2, 16392, (20,), 8, 2), (3, 64, (2100, 9), 32, 2),
          # tiles of 128 tokens; runs of several column tiles; more rows of A than a block's
          (1100, 264, (700, 60), 16, 3), (1500, 520, (129,), 72, 5), (1300, 128, (20000, 300), 8, 4),
-         (1100, 96, (300,) * 8, 24, 6), (1200, 200, (600,), 200, 2)]
+         (1100, 96, (300,) * 8, 24, 6), (1200, 200, (600,), 200, 2),
+         # tiles of 64: their adapters' bytes past what is left to single tokens
+         (65, 4104, (700, 3), 200, 3), (130, 4096, (1025,), 104, 4), (333, 2056, (128, 129, 1), 40, 7),
+         (1000, 264, (4000,), 16, 64), (1024, 3208, (40, 5), 8, 9), (900, 1096, (65,) * 8, 8, 40),
+         (701, 6152, (300,), 16, 5), (257, 4096, (20000,), 8, 6),
+         # single tokens up to the last
+         (1024, 1096, (130,), 8, 40), (1024, 64, (300, 9), 24, 5)]
 
 
 @pytest.mark.parametrize("M,K,widths,r,L", CASES)
@@ -61,12 +66,12 @@ def test_matches(M, K, widths, r, L, kind):
     assert np.array_equal(got[none], y[none])
 
 
-@pytest.mark.parametrize("M", [40, 300])
-def test_integer_inputs_are_exact(M):
+@pytest.mark.parametrize("M,K", [(40, 512), (300, 512), (900, 2048), (1100, 512)])
+def test_integer_inputs_are_exact(M, K):
     """Whole numbers: t below 2^11 and every sum exact in fp32, so the result is the
     rounded exact one, in any order."""
     rng = np.random.default_rng(M)
-    K, widths, r, L = 512, (96, 40), 16, 5
+    widths, r, L = (96, 40), 16, 5
     y = rng.integers(-8, 9, (M, sum(widths))).astype(np.float16)
     x = rng.integers(-1, 2, (M, K)).astype(np.float16)
     la = rng.integers(-2, 3, (L, 2 * r, K)).astype(np.float16)
@@ -78,12 +83,12 @@ def test_integer_inputs_are_exact(M):
     assert np.array_equal(_run(y, x, la, lb, ids, sc, widths), want.astype(np.float16))
 
 
-@pytest.mark.parametrize("M", [20, 150])
-def test_requests_do_not_meet(M):
+@pytest.mark.parametrize("M,K", [(20, 256), (150, 256), (700, 4096), (1100, 256)])
+def test_requests_do_not_meet(M, K):
     """Another request's NaN and infinities, in its tokens or in its adapter, stay with
     it; ids outside the adapters keep y; an unused adapter is not read."""
     rng = np.random.default_rng(M)
-    K, widths, r, L = 256, (128, 33), 16, 6
+    widths, r, L = (128, 33), 16, 6
     y, x, la, lb, sc = _operands(rng, M, K, widths, r, L)
     ids = (np.arange(M) % L).astype(np.int32)
     ids[5], ids[11], ids[13] = -1, L, 2 ** 31 - 1
@@ -101,11 +106,11 @@ def test_requests_do_not_meet(M):
     assert np.isinf(got[6, 0]) and np.isfinite(got[6, 1:]).all()
 
 
-@pytest.mark.parametrize("M", [10, 100])
-def test_large_and_small_adapters(M):
+@pytest.mark.parametrize("M,K", [(10, 1024), (100, 1024), (800, 4096), (1100, 1024)])
+def test_large_and_small_adapters(M, K):
     """t beyond fp16's range and below its normal numbers: it is held in fp32."""
     rng = np.random.default_rng(M)
-    K, widths, r, L = 1024, (96,), 16, 3
+    widths, r, L = (96,), 16, 3
     y, x, la, lb, sc = _operands(rng, M, K, widths, r, L)
     ids = _ids(rng, M, L, "each")
     for up in (2.0 ** 13, 2.0 ** -9):
@@ -116,12 +121,12 @@ def test_large_and_small_adapters(M):
         assert (err <= tol).all()
 
 
-@pytest.mark.parametrize("M", [12, 130])
-def test_strides_and_in_place(M):
+@pytest.mark.parametrize("M,K", [(12, 264), (130, 264), (1000, 3272), (1100, 264)])
+def test_strides_and_in_place(M, K):
     """Column slices of one projection's output, tokens in two leading dims, out given
     and in place; what lies beside the slice stays."""
     rng = np.random.default_rng(M)
-    K, widths, r, L = 264, (128, 40), 8, 4
+    widths, r, L = (128, 40), 8, 4
     N = sum(widths)
     y, x, la, lb, sc = _operands(rng, M, K, widths, r, L)
     ids = _ids(rng, M, L, "runs")
@@ -145,7 +150,7 @@ def test_strides_and_in_place(M):
                           _run(y, x, la, lb, ids, None, widths))
 
 
-@pytest.mark.parametrize("M", [9, 140])
+@pytest.mark.parametrize("M", [9, 140, 800, 1100])
 def test_stream_and_graph(M):
     rng = np.random.default_rng(M)
     K, widths, r, L = 2048, (256, 64), 16, 8
@@ -197,13 +202,13 @@ def test_offsets_past_32_bits(M):
 def test_two_streams_at_once():
     rng = np.random.default_rng(5)
     calls = []
-    for M, r in ((300, 16), (1200, 64)):
+    for M, r in ((300, 16), (1200, 64), (900, 32)):
         y, x, la, lb, sc = _operands(rng, M, 2048, (512, 128), r, 6)
         ids = _ids(rng, M, 6, "runs")
         t = [to_dev(v) for v in (y, x, la, lb, ids, sc)]
         calls.append((t, to_np(_CUDA.lora_add(*t, (512, 128))), torch.cuda.Stream()))
     torch.cuda.synchronize()
-    outs = [[], []]
+    outs = [[], [], []]
     for _ in range(5):
         for (t, _, s), o in zip(calls, outs):
             with torch.cuda.stream(s):
