@@ -81,20 +81,18 @@ SRQ_DEV void wave_fence() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-// At most `ahead` groups of PER loads of this wave are still in flight (ahead < 8; the
-// counter goes to 63, and a smaller count waits for more).
-template <int PER>
-SRQ_DEV void wait_ahead(int ahead) {
-    switch (ahead) {
-    case 0: asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); break;
-    case 1: asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PER) : "memory"); break;
-    case 2: asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * PER) : "memory"); break;
-    case 3: asm volatile("s_waitcnt vmcnt(%0)" ::"n"(3 * PER) : "memory"); break;
-    case 4: asm volatile("s_waitcnt vmcnt(%0)" ::"n"(4 * PER < 64 ? 4 * PER : 63) : "memory"); break;
-    case 5: asm volatile("s_waitcnt vmcnt(%0)" ::"n"(5 * PER < 64 ? 5 * PER : 63) : "memory"); break;
-    case 6: asm volatile("s_waitcnt vmcnt(%0)" ::"n"(6 * PER < 64 ? 6 * PER : 63) : "memory"); break;
-    default: asm volatile("s_waitcnt vmcnt(%0)" ::"n"(7 * PER < 64 ? 7 * PER : 63) : "memory"); break;
-    }
+// At most N loads of this wave are still in flight.
+template <int N>
+SRQ_DEV void wait_loads() {
+    static_assert(N <= 63, "the counter's range");
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+// Every wave has come this far and its LDS reads have returned.
+SRQ_DEV void lds_barrier() {
+    __builtin_amdgcn_s_waitcnt(0xC07F);   // lgkmcnt(0), in a form that the compiler counts too
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
 }
 
 // ---------------------------------------------------------------------------
@@ -143,8 +141,8 @@ __global__ __launch_bounds__(W * 64) void w4a8_stream_kernel(A8Args a) {
         const uint32_t ka = (uint32_t)(u0 + u) * 128u, kb = ka / 2;
 #pragma unroll
         for (int i = 0; i < AR / 8; ++i)
-            dma16(ar, aoff[i] == kOob ? kOob : aoff[i] + ka, dst + i * 1024);
-        const bool in = kb + bk < KB;
+            dma16(ar, u >= cnt || aoff[i] == kOob ? kOob : aoff[i] + ka, dst + i * 1024);
+        const bool in = u < cnt && kb + bk < KB;
 #pragma unroll
         for (int t = 0; t < NT; ++t)
             dma16(br, in ? boff[t] + kb : kOob, dst + AR * 128 + t * 1024);
@@ -159,13 +157,13 @@ __global__ __launch_bounds__(W * 64) void w4a8_stream_kernel(A8Args a) {
     const int mr = AR == 8 ? m & 7 : m;   // with 8 rows staged the upper 8 results are not stored
 #pragma unroll
     for (int p = 0; p < S - 1; ++p)
-        if (p < cnt) issue(p, p);
+        issue(p, p);
     int slot = 0, free = S - 1;
     for (int u = 0; u < cnt; ++u) {
         // the reads of the stage that is filled next have returned
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        if (u + S - 1 < cnt) issue(u + S - 1, free);
-        wait_ahead<PER>(min(S - 1, cnt - 1 - u));
+        issue(u + S - 1, free);
+        wait_loads<(S - 1) * PER>();
         const uint8_t *st = ring + slot * kStage;
         v4i av[MT][2];
 #pragma unroll
@@ -188,7 +186,8 @@ __global__ __launch_bounds__(W * 64) void w4a8_stream_kernel(A8Args a) {
         slot = slot == S - 1 ? 0 : slot + 1;
         free = free == S - 1 ? 0 : free + 1;
     }
-    __syncthreads();   // the rings are free (every load has been waited for)
+    wait_loads<0>();
+    __syncthreads();   // the rings are free
     int *part = reinterpret_cast<int *>(smem);
 #pragma unroll
     for (int i = 0; i < MT; ++i)
@@ -213,15 +212,7 @@ __global__ __launch_bounds__(W * 64) void w4a8_stream_kernel(A8Args a) {
 }
 
 // ---------------------------------------------------------------------------
-// More rows: tiles of BM x BN, WM x WN waves with (BM / WM) x (BN / WN) each in blocks
-// of v_mfma_i32_32x32x32_i8, K in steps of 128 codes through a ring of NSTG stages
-// (BM rows of 128 bytes, then BN rows of 64) that every wave fills with its share of
-// loads.  One barrier a step: behind it step s has landed for all and step s - 1, whose
-// stage is filled next, has been read by all.
-// Small tiles are bound by what a CU takes in: 101 rows, 14336 columns, K = 4096 18.1 us,
-// 0.5 MB a CU at 29 bytes a ns.  The large ones are bound by the instructions at the power
-// that the card gives them: 2048 rows, 28672 columns, K = 4096 215 us, 2.2 POPS, on zeros
-// 179 us.
+// More rows: tiles.
 struct __attribute__((packed, aligned(2))) U8h { v8h v; };
 
 template <int BM, int BN>
@@ -229,6 +220,283 @@ struct Scales {
     float sa[BM], sb[BN], bias[BN];   // of a tile
 };
 
+template <int BM, int BN>
+SRQ_DEV void load_scales(const A8Args &a, Scales<BM, BN> &sc, int64_t m0, int64_t n0, int threads) {
+    for (int i = threadIdx.x; i < BM; i += threads) sc.sa[i] = m0 + i < a.M ? a.sa[m0 + i] : 0.f;
+    for (int i = threadIdx.x; i < BN; i += threads) {
+        const bool in = n0 + i < a.N;
+        sc.sb[i] = in ? (float)a.sb[n0 + i] : 0.f;
+        sc.bias[i] = in && a.bias ? (float)a.bias[n0 + i] : 0.f;
+    }
+}
+
+// A wave's ROWS x 32 FN outputs pass through its own piece of LDS, so that they leave, and
+// a residual comes, in 16 bytes a lane.
+template <int ROWS, int FN>
+struct OutRows {
+    static constexpr int kStride = 32 * FN + 8;
+    static constexpr int kBytes = ROWS * kStride * 2;
+    static constexpr int LPR = 4 * FN, RPI = 64 / LPR;   // lanes a row, rows an instruction
+    f16 *tile;
+    int64_t m, n;   // of the first
+    int row, col;   // of this lane in an instruction
+    SRQ_DEV OutRows(uint8_t *at, int64_t m0, int64_t n0, int lane)
+        : tile(reinterpret_cast<f16 *>(at)), m(m0), n(n0), row(lane / LPR), col(8 * (lane % LPR)) {}
+    SRQ_DEV f16 &at(int r, int c) const { return tile[r * kStride + c]; }
+    SRQ_DEV bool has(const A8Args &a, int r) const {
+        return r < ROWS && m + r < a.M && n + col < a.N;
+    }
+    SRQ_DEV void load(const A8Args &a, const f16 *from) const {
+#pragma unroll
+        for (int r0 = 0; r0 < ROWS; r0 += RPI) {
+            const int r = r0 + row;
+            if (!has(a, r)) continue;
+            const f16 *src = from + (m + r) * a.N + n + col;
+            v8h o;
+            if (n + col + 8 <= a.N) {
+                o = reinterpret_cast<const U8h *>(src)->v;
+            } else {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) o[k] = n + col + k < a.N ? src[k] : (f16)0;
+            }
+            *reinterpret_cast<v8h *>(&at(r, col)) = o;
+        }
+        wave_fence();
+    }
+    SRQ_DEV void store(const A8Args &a) const {
+        wave_fence();
+#pragma unroll
+        for (int r0 = 0; r0 < ROWS; r0 += RPI) {
+            const int r = r0 + row;
+            if (!has(a, r)) continue;
+            const v8h o = *reinterpret_cast<const v8h *>(&at(r, col));
+            f16 *dst = a.out + (m + r) * a.N + n + col;
+            if (n + col + 8 <= a.N) {
+                reinterpret_cast<U8h *>(dst)->v = o;
+            } else {
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    if (n + col + k < a.N) dst[k] = o[k];
+            }
+        }
+    }
+};
+
+// Tile `idx` of tiles_m x tiles_n in bands of 8 rows of tiles, columns of a band one after
+// the other.
+SRQ_DEV void tile_place(uint32_t idx, uint32_t tiles_m, uint32_t tiles_n, uint32_t &tm,
+                        uint32_t &tn) {
+    const uint32_t band = uni(idx / (8 * tiles_n)), in_band = idx - band * 8 * tiles_n;
+    const uint32_t high = min(8u, tiles_m - 8 * band);
+    tn = uni(in_band / high);
+    tm = 8 * band + in_band - tn * high;
+}
+
+// Block b runs on XCD b % 8: each XCD takes a run of tiles, and with the bands the blocks
+// that share its L2 read a square of panels.
+SRQ_DEV uint32_t place_of(uint32_t b, uint32_t total) {
+    const uint32_t x = b % 8, per = total / 8, rem = total % 8;
+    return x * per + min(x, rem) + b / 8;
+}
+
+// A step's LDS row of C chunks of 16 bytes holds them exchanged by this number, so that 8
+// lanes that read one chunk of 8 rows meet all banks.
+template <int C>
+SRQ_DEV int swizzle(int row) { return C >= 16 ? row & 15 : C == 8 ? row >> 1 & 7 : row >> 2 & 3; }
+
+// Up to a few rounds of tiles of BM x BN: K in steps of 64 KG codes through a ring of NSTG
+// stages (BM rows of 64 KG bytes, then BN of 32 KG) that every wave fills with its share of
+// loads; KG groups of waves take 64 codes of a step each, WN waves of a group BN / WN
+// columns each of all the rows, and the groups' int32 sums are joined through LDS.  So a
+// row's codes are read from LDS WN times and a weight is read and unpacked once.
+// One barrier a step: behind it step s + 1 has landed for all and step s, whose operands
+// are in registers and whose stage is filled next, has been read by all.  Steps past the
+// last load zeros from outside the buffers, so that the waits are constants and the loop
+// has no branch but its end: at one or two waves a SIMD every scalar instruction counts.
+// 101 rows, 14336 columns, K = 4096 12.5 us (waves that shared out the tile's rows and
+// columns instead, with the branches: 19.8), 128 x 28672 x 8192 32 us (42): what a CU takes
+// in bounds the small tiles, 50 to 80 bytes a ns, products and unpacking those of 128 x 128.
+template <int BM, int BN, int KG, int WN, int NSTG>
+__global__ __launch_bounds__(64 * KG * WN) void w4a8_tile_kernel(A8Args a) {
+    constexpr int NW = KG * WN, FM = BM / 32, FN = BN / WN / 32;
+    static_assert(FM * 32 == BM && FN * WN * 32 == BN, "tile");
+    constexpr int CA = 4 * KG, CB = 2 * KG;             // chunks of a row
+    constexpr int kA = BM * CA * 16, kStage = kA + BN * CB * 16;
+    constexpr int RA = 64 / CA, RB = 64 / CB;           // rows of a load
+    constexpr int PA = BM / RA / NW, PB = BN / RB / NW, PER = PA + PB;
+    static_assert(PA * NW * RA == BM && PB * NW * RB == BN && NSTG >= 2, "loads of a stage");
+    // the join: 8 rows of a column block are a unit, and a group's waves own UO of the U
+    constexpr int U = FM * 4, UO = U / KG;
+    static_assert(UO * KG == U, "units");
+    using Out = OutRows<8 * UO, FN>;
+    constexpr int kPart = NW * (U - UO) * 1024;         // a column block's parts
+    constexpr int ROUNDS = FN * kPart + NW * Out::kBytes <= 158 * 1024 ? 1 : FN, FR = FN / ROUNDS;
+    constexpr int kJoin = FR * kPart + NW * Out::kBytes;
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[NSTG * kStage > kJoin ? NSTG * kStage : kJoin];
+    __shared__ Scales<BM, BN> sc;
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    uint32_t tm, tn;
+    tile_place(place_of(blockIdx.x, gridDim.x), (uint32_t)srq_cdiv(a.M, BM),
+               (uint32_t)srq_cdiv(a.N, BN), tm, tn);
+    const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
+    const int64_t KB = a.K / 2;
+    const int k_lo = a.kc ? (int)(blockIdx.y * a.kc) : 0;
+    const int k_hi = (int)(a.kc ? min(a.K, k_lo + a.kc) : a.K);
+    const int steps = (k_hi - k_lo + 64 * KG - 1) / (64 * KG);
+    // addresses behind a tile's last row are out of the buffer's range and read zeros
+    const __amdgpu_buffer_rsrc_t ar = make_rsrc(a.a + m0 * a.K, rows_bytes(a.M - m0, BM, a.K));
+    const __amdgpu_buffer_rsrc_t br = make_rsrc(a.w + n0 * KB, rows_bytes(a.N - n0, BN, KB));
+    const uint32_t ring0 = lds_addr(smem);
+
+    if (!a.kc) load_scales(a, sc, m0, n0, NW * 64);   // ahead of the ring's loads, which are counted
+    uint32_t aoff[PA], boff[PB];
+    int bk[PB];
+#pragma unroll
+    for (int q = 0; q < PA; ++q) {
+        const int r = RA * (q * NW + wave) + lane / CA;
+        aoff[q] = (uint32_t)(r * a.K + k_lo) + 16 * ((lane % CA) ^ swizzle<CA>(r));
+    }
+#pragma unroll
+    for (int q = 0; q < PB; ++q) {
+        const int r = RB * (q * NW + wave) + lane / CB;
+        bk[q] = k_lo / 2 + 16 * ((lane % CB) ^ swizzle<CB>(r));
+        boff[q] = (uint32_t)(r * KB) + bk[q];
+    }
+    auto issue = [&](int s, uint32_t dst) __attribute__((always_inline)) {
+        dst += ring0 + wave * 1024;
+#pragma unroll
+        for (int q = 0; q < PA; ++q)
+            dma16(ar, s < steps ? aoff[q] + 64u * KG * s : kOob, dst + q * NW * 1024);
+        // past the split: zero weights cancel whatever the rows hold there
+#pragma unroll
+        for (int q = 0; q < PB; ++q)
+            dma16(br, bk[q] + 32 * KG * s < k_hi / 2 ? boff[q] + 32u * KG * s : kOob,
+                  dst + kA + q * NW * 1024);
+    };
+#pragma unroll
+    for (int p = 0; p < NSTG; ++p) issue(p, p * kStage);
+
+    const int kg = wave / WN, wn = wave % WN;
+    const int rr = lane & 31, g = lane >> 5;
+    // product h of a lane: chunk 4 kg + 2 g + h of a row, half h of weight chunk 2 kg + g
+    uint32_t al[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+        al[h] = ring0 + rr * CA * 16 + 16 * ((4 * kg + 2 * g + h) ^ swizzle<CA>(rr));
+    const uint32_t bl =
+        ring0 + kA + (wn * (FN * 32) + rr) * CB * 16 + 16 * ((2 * kg + g) ^ swizzle<CB>(rr));
+    v16i acc[FM][FN];
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) acc[i][j] = (v16i){};
+    v4i av[2][2][FM], wv[2][FN];   // of this step and the next
+    auto fetch = [&](int b, uint32_t st) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < FN; ++j) wv[b][j] = lds16(bl + st + j * 32 * CB * 16);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < FM; ++i) av[b][h][i] = lds16(al[h] + st + i * 32 * CA * 16);
+    };
+    wait_loads<(NSTG - 1) * PER>();
+    lds_barrier();
+    fetch(0, 0);
+    int s = 0;
+    do {
+#pragma unroll
+        for (int p = 0; p < (NSTG % 2 ? 2 * NSTG : NSTG); ++p) {
+            const int b = p & 1;
+            wait_loads<(NSTG - 2) * PER>();
+            lds_barrier();
+            fetch(b ^ 1, (p + 1) % NSTG * kStage);
+            issue(s + NSTG, p % NSTG * kStage);
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int j = 0; j < FN; ++j) {
+                    const v4i bv = codes16((u32)wv[b][j][2 * h], (u32)wv[b][j][2 * h + 1]);
+#pragma unroll
+                    for (int i = 0; i < FM; ++i) acc[i][j] = mfma32x32(av[b][h][i], bv, acc[i][j]);
+                }
+            if (++s == steps) break;
+        }
+    } while (s < steps);
+    wait_loads<0>();
+
+    // Every group keeps its own units and hands the others theirs, lane by lane.
+    v4i own[FN][UO];
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r) {
+        lds_barrier();
+        auto part = [&](int owner, int from, int j, int u) __attribute__((always_inline)) {
+            const int k = from < owner ? from : from - 1;
+            return (__attribute__((address_space(3))) v4i *)(uintptr_t)(
+                ring0 + ((((owner * (KG - 1) + k) * WN + wn) * FR + j) * UO + u) * 1024 + lane * 16);
+        };
+#pragma unroll
+        for (int q = 0; q < KG; ++q)
+#pragma unroll
+            for (int j = 0; j < FR; ++j)
+#pragma unroll
+                for (int u = 0; u < UO; ++u) {
+                    const int x = q * UO + u;
+                    v4i v;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] = acc[x / 4][r * FR + j][4 * (x % 4) + e];
+                    if (q == kg) own[r * FR + j][u] = v;
+                    else *part(q, kg, j, u) = v;
+                }
+        lds_barrier();
+#pragma unroll
+        for (int k = 0; k < KG - 1; ++k)
+#pragma unroll
+            for (int j = 0; j < FR; ++j)
+#pragma unroll
+                for (int u = 0; u < UO; ++u) own[r * FR + j][u] += *part(kg, k < kg ? k : k + 1, j, u);
+    }
+    const int row0 = 8 * UO * kg, col0 = wn * (FN * 32);
+    if (a.kc) {
+        int32_t *to = a.part + (int64_t)blockIdx.y * a.M * a.N;
+#pragma unroll
+        for (int u = 0; u < UO; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int64_t m = m0 + row0 + 8 * u + 4 * g + e;
+#pragma unroll
+                for (int j = 0; j < FN; ++j) {
+                    const int64_t n = n0 + col0 + j * 32 + rr;
+                    if (m < a.M && n < a.N) to[m * a.N + n] = own[j][u][e];
+                }
+            }
+        return;
+    }
+    const Out out(smem + FR * kPart + wave * Out::kBytes, m0 + row0, n0 + col0, lane);
+    if (a.res) out.load(a, a.res);
+#pragma unroll
+    for (int j = 0; j < FN; ++j) {
+        const float sb = sc.sb[col0 + j * 32 + rr], bias = sc.bias[col0 + j * 32 + rr];
+#pragma unroll
+        for (int u = 0; u < UO; ++u) {
+            const int lr = 8 * u + 4 * g;
+            const v4f sa = *reinterpret_cast<const v4f *>(sc.sa + row0 + lr);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                f16 &at = out.at(lr + e, j * 32 + rr);
+                float o = dequant(own[j][u][e], sa[e], sb) + bias;
+                if (a.res) o += (float)at;
+                at = f16_rn(o);
+            }
+        }
+    }
+    out.store(a);
+}
+
+// Many tiles: WM x WN waves with (BM / WM) x (BN / WN) of a tile each, whose sums leave no
+// registers for parts of K.  K in steps of 128 codes through a ring of NSTG stages (BM rows
+// of 128 bytes, then BN rows of 64).  The instructions bound it, at the power that the card
+// gives them: 2048 rows, 28672 columns, K = 4096 215 us, 2.2 POPS, on zeros 179 us.
 template <int BM, int BN, int WM, int WN, int NSTG>
 constexpr int ring_bytes() {
     return NSTG * (BM * 128 + BN * 64);
@@ -242,58 +510,43 @@ SRQ_DEV void tile_body(const A8Args &a, uint8_t *smem, Scales<BM, BN> &sc, int64
     constexpr int kStage = BM * 128 + BN * 64;
     constexpr int PA = BM / 8 / NW, PB = BN / 16 / NW, PER = PA + PB;
     static_assert(PA * NW * 8 == BM && PB * NW * 16 == BN, "loads of a stage");
-    static_assert(NSTG >= 2 && NSTG <= 8 && (NSTG - 2) * PER <= 63, "loads in flight");
-    constexpr int kTileW = 32 * FN + 8;                 // row stride of a wave's output rows
-    constexpr int kRing = NSTG * kStage;
-    static_assert(NW * 32 * FM * kTileW * 2 <= kRing, "output rows");
+    static_assert(NSTG >= 2, "a stage ahead");
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int64_t KB = a.K / 2;
-    const int64_t k_lo = a.kc ? (int64_t)blockIdx.y * a.kc : 0;
-    const int64_t k_hi = a.kc ? min(a.K, k_lo + a.kc) : a.K;
-    const int steps = (int)((k_hi - k_lo + 127) / 128);
+    const int steps = (int)((a.K + 127) / 128);
     // addresses behind a tile's last row are out of the buffer's range and read zeros
     const __amdgpu_buffer_rsrc_t ar = make_rsrc(a.a + m0 * a.K, rows_bytes(a.M - m0, BM, a.K));
     const __amdgpu_buffer_rsrc_t br = make_rsrc(a.w + n0 * KB, rows_bytes(a.N - n0, BN, KB));
     const uint32_t ring0 = lds_addr(smem);
 
-    // (ahead of the ring's loads, which are counted)
-    if (!a.kc) {
-        for (int i = threadIdx.x; i < BM; i += NW * 64) sc.sa[i] = m0 + i < a.M ? a.sa[m0 + i] : 0.f;
-        for (int i = threadIdx.x; i < BN; i += NW * 64) {
-            const bool in = n0 + i < a.N;
-            sc.sb[i] = in ? (float)a.sb[n0 + i] : 0.f;
-            sc.bias[i] = in && a.bias ? (float)a.bias[n0 + i] : 0.f;
-        }
-    }
-
+    load_scales(a, sc, m0, n0, NW * 64);   // ahead of the ring's loads, which are counted
     uint32_t aoff[PA], boff[PB];
 #pragma unroll
     for (int q = 0; q < PA; ++q) {
         const int r = 8 * (q * NW + wave) + (lane >> 3);
-        aoff[q] = (uint32_t)(r * a.K + k_lo) + 16 * ((lane & 7) ^ (r >> 1 & 7));
+        aoff[q] = (uint32_t)(r * a.K) + 16 * ((lane & 7) ^ (r >> 1 & 7));
     }
     const int bk = 16 * ((lane & 3) ^ ((lane >> 4) & 3));
 #pragma unroll
     for (int q = 0; q < PB; ++q)
-        boff[q] = (uint32_t)((16 * (q * NW + wave) + (lane >> 2)) * KB + k_lo / 2) + bk;
+        boff[q] = (uint32_t)((16 * (q * NW + wave) + (lane >> 2)) * KB) + bk;
     // loads q_lo .. q_hi of this wave's of step s, into the stage at dst
     auto issue = [&](int s, uint32_t dst, int q_lo, int q_hi) __attribute__((always_inline)) {
         // past K: zero weights cancel whatever the rows hold there
-        const bool in = k_lo / 2 + 64 * (int64_t)s + bk < KB;
+        const bool in = 64 * (int64_t)s + bk < KB;
         dst += ring0 + wave * 1024;
 #pragma unroll
         for (int q = 0; q < PER; ++q) {
             if (q < q_lo || q >= q_hi) continue;
             if (q < PA)
-                dma16(ar, aoff[q] + 128u * s, dst + q * NW * 1024);
+                dma16(ar, s < steps ? aoff[q] + 128u * s : kOob, dst + q * NW * 1024);
             else
                 dma16(br, in ? boff[q - PA] + 64u * s : kOob, dst + BM * 128 + (q - PA) * NW * 1024);
         }
     };
 #pragma unroll
-    for (int p = 0; p < NSTG; ++p)
-        if (p < steps) issue(p, p * kStage, 0, PER);
+    for (int p = 0; p < NSTG; ++p) issue(p, p * kStage, 0, p < NSTG - 1 ? PER : PER / 4);
 
     const int wm = wave / WN, wn = wave % WN;
     const int rr = lane & 31, g = lane >> 5;
@@ -328,16 +581,15 @@ SRQ_DEV void tile_body(const A8Args &a, uint8_t *smem, Scales<BM, BN> &sc, int64
     // The operands of a slice are read and unpacked beside the products of the one before,
     // across the steps too: the barrier stands ahead of a step's last products, when its
     // stage has been read and the next one is needed.
-    wait_ahead<PER>(min(NSTG - 1, steps - 1));
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
+    wait_loads<(NSTG - 2) * PER + PER / 4>();
+    lds_barrier();
     fetch_b(0, 0);
     fetch_a(0, 0);
     unpack(0);
     // A step's loads are spread over four slices, the first behind the barrier that frees
     // their stage: a wave stalls on a burst of them, and its products with it.
-    uint32_t st = 0, fst = 0;
-    int fill = steps;
+    uint32_t st = 0, fst = (NSTG - 1) * kStage;
+    int fill = NSTG - 1;
     for (int s = 0; s < steps; ++s) {
         const uint32_t nst = st == (NSTG - 1) * kStage ? 0 : st + kStage;
 #pragma unroll
@@ -345,19 +597,16 @@ SRQ_DEV void tile_body(const A8Args &a, uint8_t *smem, Scales<BM, BN> &sc, int64
             if (c < 3) {
                 if (c == 0) fetch_b(1, st);
                 fetch_a(c + 1, st);
-            } else if (s + 1 < steps) {
-                // step s + 1 has landed and this wave has read all of step s ..
-                wait_ahead<PER>(min(NSTG - 2, steps - 2 - s));
-                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-                // .. and so it is for all waves
-                __builtin_amdgcn_s_barrier();
-                asm volatile("" ::: "memory");
+            } else {
+                // step s + 1 has landed, step s has been read
+                wait_loads<(NSTG - 2) * PER>();
+                lds_barrier();
                 fetch_b(0, nst);
                 fetch_a(0, nst);
                 fill = s + NSTG;
                 fst = st;
             }
-            if (fill < steps) issue(fill, fst, PER * ((c + 1) & 3) / 4, PER * (((c + 1) & 3) + 1) / 4);
+            issue(fill, fst, PER * ((c + 1) & 3) / 4, PER * (((c + 1) & 3) + 1) / 4);
 #pragma unroll
             for (int j = 0; j < FN; ++j)
 #pragma unroll
@@ -376,114 +625,36 @@ SRQ_DEV void tile_body(const A8Args &a, uint8_t *smem, Scales<BM, BN> &sc, int64
         st = nst;
     }
 
-    const int64_t mw = m0 + wm * (FM * 32), nw = n0 + wn * (FN * 32);
-    if (a.kc) {
-        int32_t *part = a.part + (int64_t)blockIdx.y * a.M * a.N;
-#pragma unroll
-        for (int i = 0; i < FM; ++i)
-#pragma unroll
-            for (int v = 0; v < 16; ++v) {
-                const int64_t m = mw + i * 32 + 8 * (v / 4) + 4 * g + v % 4;
-#pragma unroll
-                for (int j = 0; j < FN; ++j) {
-                    const int64_t n = nw + j * 32 + rr;
-                    if (m < a.M && n < a.N) part[m * a.N + n] = acc[i][j][v];
-                }
-            }
-        return;
-    }
-    // The wave's rows pass through its own piece of LDS, so that they leave, and a residual
-    // comes, in 16 bytes a lane.
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    f16 *tile = reinterpret_cast<f16 *>(smem) + wave * (32 * FM) * kTileW;
-    constexpr int LPR = 4 * FN, RPI = 64 / LPR;   // lanes a row, rows an instruction
-    const int c8 = 8 * (lane % LPR);
-    const int64_t n8 = nw + c8;
-    if (a.res) {
-#pragma unroll
-        for (int r0 = 0; r0 < 32 * FM; r0 += RPI) {
-            const int lr = r0 + lane / LPR;
-            const int64_t m = mw + lr;
-            if (m >= a.M || n8 >= a.N) continue;
-            const f16 *src = a.res + m * a.N + n8;
-            v8h o;
-            if (n8 + 8 <= a.N) {
-                o = reinterpret_cast<const U8h *>(src)->v;
-            } else {
-#pragma unroll
-                for (int k = 0; k < 8; ++k) o[k] = n8 + k < a.N ? src[k] : (f16)0;
-            }
-            *reinterpret_cast<v8h *>(tile + lr * kTileW + c8) = o;
-        }
-        wave_fence();
-    }
+    wait_loads<0>();
+    lds_barrier();
+    using Out = OutRows<32 * FM, FN>;
+    static_assert(NW * Out::kBytes <= NSTG * kStage, "output rows");
+    const int row0 = wm * (FM * 32), col0 = wn * (FN * 32);
+    const Out out(smem + wave * Out::kBytes, m0 + row0, n0 + col0, lane);
+    if (a.res) out.load(a, a.res);
     float sbv[FN], biasv[FN];
 #pragma unroll
     for (int j = 0; j < FN; ++j) {
-        sbv[j] = sc.sb[wn * (FN * 32) + j * 32 + rr];
-        biasv[j] = sc.bias[wn * (FN * 32) + j * 32 + rr];
+        sbv[j] = sc.sb[col0 + j * 32 + rr];
+        biasv[j] = sc.bias[col0 + j * 32 + rr];
     }
 #pragma unroll
     for (int i = 0; i < FM; ++i)
 #pragma unroll
         for (int v4 = 0; v4 < 4; ++v4) {
             const int lr = i * 32 + 8 * v4 + 4 * g;
-            const v4f sa = *reinterpret_cast<const v4f *>(sc.sa + wm * (FM * 32) + lr);
+            const v4f sa = *reinterpret_cast<const v4f *>(sc.sa + row0 + lr);
 #pragma unroll
             for (int v = 0; v < 4; ++v)
 #pragma unroll
                 for (int j = 0; j < FN; ++j) {
-                    f16 &at = tile[(lr + v) * kTileW + j * 32 + rr];
+                    f16 &at = out.at(lr + v, j * 32 + rr);
                     float o = dequant(acc[i][j][4 * v4 + v], sa[v], sbv[j]) + biasv[j];
                     if (a.res) o += (float)at;
                     at = f16_rn(o);
                 }
         }
-    wave_fence();
-#pragma unroll
-    for (int r0 = 0; r0 < 32 * FM; r0 += RPI) {
-        const int lr = r0 + lane / LPR;
-        const int64_t m = mw + lr;
-        if (m >= a.M || n8 >= a.N) continue;
-        const v8h o = *reinterpret_cast<const v8h *>(tile + lr * kTileW + c8);
-        f16 *dst = a.out + m * a.N + n8;
-        if (n8 + 8 <= a.N) {
-            reinterpret_cast<U8h *>(dst)->v = o;
-        } else {
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-                if (n8 + k < a.N) dst[k] = o[k];
-        }
-    }
-}
-
-// Tile `idx` of tiles_m x tiles_n in bands of 8 rows of tiles, columns of a band one after
-// the other.
-SRQ_DEV void tile_place(uint32_t idx, uint32_t tiles_m, uint32_t tiles_n, uint32_t &tm,
-                        uint32_t &tn) {
-    const uint32_t band = uni(idx / (8 * tiles_n)), in_band = idx - band * 8 * tiles_n;
-    const uint32_t high = min(8u, tiles_m - 8 * band);
-    tn = uni(in_band / high);
-    tm = 8 * band + in_band - tn * high;
-}
-
-// Block b runs on XCD b % 8: each XCD takes a run of tiles, and with the bands the blocks
-// that share its L2 read a square of panels.
-SRQ_DEV uint32_t place_of(uint32_t b, uint32_t total) {
-    const uint32_t x = b % 8, per = total / 8, rem = total % 8;
-    return x * per + min(x, rem) + b / 8;
-}
-
-template <int BM, int BN, int WM, int WN, int NSTG>
-__global__ __launch_bounds__(64 * WM * WN) void w4a8_tile_kernel(A8Args a) {
-    __shared__ __attribute__((aligned(1024))) uint8_t smem[ring_bytes<BM, BN, WM, WN, NSTG>()];
-    __shared__ Scales<BM, BN> sc;
-    uint32_t tm, tn;
-    tile_place(place_of(blockIdx.x, gridDim.x), (uint32_t)srq_cdiv(a.M, BM),
-               (uint32_t)srq_cdiv(a.N, BN), tm, tn);
-    tile_body<BM, BN, WM, WN, NSTG>(a, smem, sc, (int64_t)tm * BM, (int64_t)tn * BN);
+    out.store(a);
 }
 
 // Many rows: `whole` tiles of 256 x 256, a multiple of the 256 CUs, and the rest, where it
@@ -543,48 +714,55 @@ __global__ __launch_bounds__(256) void w4a8_join_kernel(A8Args a, int splits) {
     }
 }
 
+// Of n tiles of the large kernel, those that stay whole.
+int64_t whole_tiles(int64_t n) { return n % 256 <= 128 ? n - n % 256 : n; }
+
 // How a product runs, by its sizes alone.
-enum { kStream, k64x128, k128x128, kLarge };
+enum { kStream, k64x64, k64x128, k128x128, kLarge };
 struct Plan {
     int kind;
     int splits;      // over K
     int64_t kc;
 };
 
+// More rows than the streams are for: the tile and the number of splits over K with the
+// shortest time, rounds of the 256 CUs times the steps of 256 codes times what a step of
+// such a tile takes (measured, whole rounds), and 5 us and the parts' bytes for a join.
+// us on one MI355X, 64 x 64 / 64 x 128 / 128 x 128 / large: 64 x 14336 x 4096 11.2 / 13.7 /
+// 17.9; 101 x 14336 x 4096 15.9 / 13.9 / 19.0 / 29.6; 128 x 28672 x 4096 32.6 / 30.4 / 23.5
+// / 35.1; 512 x 14336 x 4096 49.5 / 50.6 / 40.6 / 37.1.  64 x 4096 x 14336, 64 x 64 in one
+// / 2 / 4 parts 25 / 18.2 / 14.2.
 Plan plan_of(int64_t M, int64_t N, int64_t K) {
     Plan p{kStream, 1, 0};
-    if (M <= 32) return p;
-    // The largest tile of which there are enough for most of the 256 CUs: a CU takes in
-    // about 40 bytes a ns, and larger tiles need fewer.  us on one MI355X: 512 x 6144 x
-    // 4096, 128 x 128 / 64 x 128 21.3 / 24.6; 512 x 4096 x 4096 20.1 / 18.1 (128 and 256
-    // tiles); 200 x 28672 x 4096, 256 x 128 / 128 x 128 35.6 / 36.9.
-    const int64_t enough = 190, n128 = srq_cdiv(N, 128);
-    if (M > 128 && srq_cdiv(M, 256) * n128 >= enough) {
-        p.kind = kLarge;
-        return p;
+    // 32 x 8192 x 8192 11.6, in tiles 13.8; 32 x 28672 x 4096 20.2 and 17.1
+    if (M <= 16 || (M <= 32 && N <= 10240)) return p;
+    const int64_t steps = srq_cdiv(K, 256);
+    const struct {
+        int kind, rows, cols;
+        double us;
+    } tiles[] = {{k64x64, 64, 64, 0.33}, {k64x128, 64, 128, 0.57}, {k128x128, 128, 128, 0.98}};
+    double best = 1e30;
+    for (const auto &t : tiles) {
+        const int64_t n = srq_cdiv(M, t.rows) * srq_cdiv(N, t.cols);
+        for (int64_t s = 1; s <= 8 && (s == 1 || (n * s <= 512 && steps >= 4 * s)); ++s) {
+            const int64_t per = srq_cdiv(steps, s), parts = srq_cdiv(steps, per);
+            double us = (double)(srq_cdiv(n * parts, 256) * per) * t.us;
+            if (parts > 1) us += 5. + 2e-6 * (double)(M * N * parts);
+            if (us > best) continue;
+            best = us;
+            p = Plan{t.kind, (int)parts, parts > 1 ? per * 256 : 0};
+        }
     }
-    const int64_t t128 = srq_cdiv(M, 128) * n128, t64 = srq_cdiv(M, 64) * n128;
-    p.kind = M > 64 && (t128 >= enough || t64 < enough) ? k128x128 : k64x128;
-    const int64_t tiles = p.kind == k128x128 ? t128 : t64;
-    if (tiles >= enough) return p;
-    // Else K is split, at least 8 steps of 128 codes each: 128 x 4096 x 14336 in 8 parts
-    // 20.8, in 4 23.4; 64 x 4096 x 14336 16.6 (8 parts of 64 x 128).
-    const int64_t steps = srq_cdiv(K, 128);
-    int64_t s = (p.kind == k64x128 ? 512 : 256) / tiles;
-    if (s > steps / 8) s = steps / 8;
-    if (s > 8) s = 8;
-    if (s < 2) return p;
-    const int64_t per = srq_cdiv(steps, s);
-    if (srq_cdiv(steps, per) < 2) return p;
-    p.kc = per * 128;
-    p.splits = (int)srq_cdiv(steps, per);
+    const int64_t n = srq_cdiv(M, 256) * srq_cdiv(N, 256), whole = whole_tiles(n);
+    if ((double)steps * (2.86 * (double)srq_cdiv(whole, 256) + (whole < n ? 1.7 : 0.)) <= best)
+        p = Plan{kLarge, 1, 0};
     return p;
 }
 
-template <int BM, int BN, int WM, int WN, int NSTG>
+template <int BM, int BN, int NSTG>
 void launch_tile(const A8Args &a, int splits, hipStream_t st) {
     const dim3 grid((unsigned)(srq_cdiv(a.M, BM) * srq_cdiv(a.N, BN)), (unsigned)splits);
-    w4a8_tile_kernel<BM, BN, WM, WN, NSTG><<<grid, 64 * WM * WN, 0, st>>>(a);
+    w4a8_tile_kernel<BM, BN, 4, 2, NSTG><<<grid, 512, 0, st>>>(a);
 }
 
 template <int AR>
@@ -592,8 +770,8 @@ void launch_stream(const A8Args &a, hipStream_t st) {
     // 16 columns a block up to a block a CU (256), then 32, which halves what the rows
     // cost; more blocks than 256 run best two to a CU, which their LDS has to allow, and
     // at 17 rows and more with 64 columns.  us, 28672 x 4096: 1 row 14 (32 columns, 4
-    // stages and so one block a CU: 17.7; 16 columns 13 to 14), 16 rows 16.2 (19.7), 32
-    // rows 20 (23.4 with 32 columns); 8192 x 28672: 16 rows 28.8 (16 columns: 35.4).
+    // stages and so one block a CU: 17.7; 16 columns 13 to 14), 16 rows 16.2 (19.7);
+    // 10240 x 8192: 32 rows 16.4; 8192 x 28672: 16 rows 28.7 (16 columns: 35.4).
     const int64_t cb = srq_cdiv(a.N, 16);
     auto grid = [&](int nt) { return dim3((unsigned)srq_cdiv(cb, nt)); };
     if (cb <= 256)
@@ -644,11 +822,11 @@ extern "C" int srq_w4a8_linear(const void *a, const void *a_scale, const void *w
         M <= 8 ? launch_stream<8>(q, st) : M <= 16 ? launch_stream<16>(q, st)
                                                    : launch_stream<32>(q, st);
         break;
-    case k64x128: launch_tile<64, 128, 2, 4, 4>(q, p.splits, st); break;
-    case k128x128: launch_tile<128, 128, 2, 4, 3>(q, p.splits, st); break;
+    case k64x64: launch_tile<64, 64, 3>(q, p.splits, st); break;
+    case k64x128: launch_tile<64, 128, 4>(q, p.splits, st); break;
+    case k128x128: launch_tile<128, 128, 3>(q, p.splits, st); break;
     default: {
-        const int64_t tiles = srq_cdiv(M, 256) * srq_cdiv(N, 256), rest = tiles % 256;
-        const int64_t whole = rest <= 128 ? tiles - rest : tiles;
+        const int64_t tiles = srq_cdiv(M, 256) * srq_cdiv(N, 256), whole = whole_tiles(tiles);
         w4a8_large_kernel<<<(unsigned)(whole + 2 * (tiles - whole)), 512, 0, st>>>(q, (uint32_t)whole);
     }
     }

@@ -32,7 +32,11 @@ SHAPES = [(1, 1, 32), (1, 16, 128), (2, 17, 96), (7, 33, 160), (8, 48, 4096), (9
           (300, 515, 1024), (200, 8193, 512), (513, 128, 4096), (1000, 515, 2208),
           (257, 12800, 256), (1030, 12801, 288), (515, 17000, 128),
           # a round of large tiles and a rest of half ones
-          (1300, 13000, 160), (2049, 8300, 96)]
+          (1300, 13000, 160), (2049, 8300, 96),
+          # each tile, in one part and split over K, with tails of all three sizes
+          (100, 14340, 1056), (20, 16400, 2080), (24, 10250, 1056), (128, 28700, 352),
+          (129, 14339, 2016), (200, 4111, 9312), (130, 2050, 20512), (512, 2100, 14368),
+          (384, 3000, 16416), (256, 2048, 16384), (40, 600, 8224), (33, 1, 32)]
 
 
 @pytest.mark.parametrize("M,N,K", SHAPES)
