@@ -259,6 +259,38 @@ SRQ_DEV uint32_t place_of(uint32_t b, uint32_t total) {
     return x * per + min(x, rem) + b / 8;
 }
 
+// Which of the items at, at + stride, .. (kChain of them, fewer than `live`) lie in a tile
+// of 64 Q tokens with more than one adapter; a tile has gy items.
+constexpr int kChain = 4;
+
+template <int Q>
+SRQ_DEV uint32_t mixed_items(const LoraArgs &a, uint32_t at, uint32_t stride, uint32_t live,
+                             uint32_t gy, int lane) {
+    int id[kChain][Q];
+#pragma unroll
+    for (int c = 0; c < kChain; ++c) {
+        const uint32_t i = at + c * stride;
+        const int64_t m0 = (int64_t)uni(i / gy) * (64 * Q);
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+            const int64_t m = m0 + 64 * q + lane;
+            id[c][q] = i < live && m < a.M ? adapter_of(a, m) : -1;
+        }
+    }
+    uint32_t bits = 0;
+#pragma unroll
+    for (int c = 0; c < kChain; ++c) {
+        int first = -1;
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+            const uint64_t has = __ballot(id[c][q] >= 0);
+            if (first < 0 && has) first = __builtin_amdgcn_readlane(id[c][q], __builtin_ctzll(has));
+            if (__ballot(id[c][q] >= 0 && id[c][q] != first)) bits |= 1u << c;
+        }
+    }
+    return bits;
+}
+
 // t of 64 Q tokens x 16 RT rows of A, K in steps of 64 through a ring of NST stages in LDS
 // (64 Q rows of x, 16 RT of A, 128 bytes each, the 16-byte chunks of a row exchanged by its
 // number).  A block takes as many rows of A as there are, up to 192, so that x crosses the
@@ -266,10 +298,14 @@ SRQ_DEV uint32_t place_of(uint32_t b, uint32_t total) {
 // waves: 4 share the rows of A out, 2 the tokens.  The operands of half a step are read
 // beside the products of the half before, and the loads are spread over them: a wave
 // stalls on a burst of loads, and its products with it.  What a CU takes in bounds it,
-// about 40 bytes a ns: 4876 tokens x 192 rows of A, K = 8192, 42 us, 20 of them the second
-// adapters of three tiles.
+// about 50 bytes a ns: 4876 tokens x 192 rows of A, K = 8192, 31 us.
+// Where CUs stay idle, `helpers` blocks more take second adapters: helper e that of the
+// first of the items e, e + helpers, .. whose tile has one, and the item's own block goes by
+// the same rule.  Four requests there, three tiles of two: 47 us when the second adapters
+// wait for the first (in blocks of their own behind them, most of them idle, 42).
 template <int RT, int Q, int NST>
-__global__ __launch_bounds__(512) void lora_shrink_kernel(LoraArgs a, int groups, int nz) {
+__global__ __launch_bounds__(512) void lora_shrink_kernel(LoraArgs a, int groups, int nz,
+                                                          int helpers) {
     constexpr int kStage = (64 * Q + 16 * RT) * 128;
     constexpr int PX = Q, PA = RT / 4, PER = PX + PA;   // loads of a wave in a stage
     constexpr int FT = 2 * Q, FR = RT / 4;              // 16 x 16 products of a wave
@@ -278,10 +314,18 @@ __global__ __launch_bounds__(512) void lora_shrink_kernel(LoraArgs a, int groups
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     // the blocks of z = 0 first: of the others most find no adapter left
-    const uint32_t live = gridDim.x / nz, zb = uni(blockIdx.x / live);
-    const uint32_t at = place_of(blockIdx.x - zb * live, live);
-    const int z = (int)zb;
-    const uint32_t gy = groups * a.splits, tile = uni(at / gy), part = at - tile * gy;
+    const uint32_t gy = groups * a.splits;
+    const uint32_t live = uni((gridDim.x - helpers) / nz), zb = uni(blockIdx.x / live);
+    uint32_t at = place_of(blockIdx.x - zb * live, live);
+    const bool helper = helpers && zb;   // (nz is 1 then)
+    const int z = helper ? 0 : (int)zb;
+    if (helper) {
+        at = blockIdx.x - live;
+        const uint32_t bits = mixed_items<Q>(a, at, helpers, live, gy, lane);
+        if (!bits) return;
+        at += __builtin_ctz(bits) * helpers;
+    }
+    const uint32_t tile = uni(at / gy), part = at - tile * gy;
     const int split = (int)uni(part / (uint32_t)groups), rg = (int)(part - split * groups) * 16 * RT;
     const int64_t m0 = (int64_t)tile * (64 * Q);
     const int K = (int)a.K, k_lo = split * a.kc;
@@ -316,6 +360,17 @@ __global__ __launch_bounds__(512) void lora_shrink_kernel(LoraArgs a, int groups
     Turns<Q> turns(a, m0, lane);
     uint64_t same[Q];
     for (int id; (id = turns.next(z, nz, same)) >= 0;) {
+        if (helper && turns.j != 2) {
+            if (turns.j > 2) break;
+            continue;
+        }
+        if (helpers && !helper && turns.j == 2) {
+            const uint32_t c = uni(at / helpers);
+            if (c < kChain) {
+                const uint32_t bits = mixed_items<Q>(a, at - c * helpers, helpers, live, gy, lane);
+                if (bits && __builtin_ctz(bits) == (int)c) continue;
+            }
+        }
         const __amdgpu_buffer_rsrc_t ar =
             make_rsrc(a.a + ((int64_t)id * a.R + rg) * a.K, (int64_t)arows * a.K * 2);
         auto issue = [&](int s, uint32_t dst, int q_lo, int q_hi) __attribute__((always_inline)) {
@@ -324,7 +379,7 @@ __global__ __launch_bounds__(512) void lora_shrink_kernel(LoraArgs a, int groups
 #pragma unroll
             for (int q = 0; q < PER; ++q) {
                 if (q < q_lo || q >= q_hi) continue;
-                const uint32_t o = ck[q] < left ? off[q] + 128 * s : kOob;
+                const uint32_t o = s < steps && ck[q] < left ? off[q] + 128 * s : kOob;
                 if (q < PX) dma16(xr, o, dst + (PX * wave + q) * 1024);
                 else dma16(ar, o, dst + (8 * Q + PA * wave + q - PX) * 1024);
             }
@@ -341,47 +396,40 @@ __global__ __launch_bounds__(512) void lora_shrink_kernel(LoraArgs a, int groups
 #pragma unroll
             for (int f = 0; f < FR; ++f) av[h][f] = lds16(al[h] + st + f * 2048);
         };
-        auto wait = [&](int ahead) __attribute__((always_inline)) {   // loads of `ahead` steps stay
-            if (ahead >= 3) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(3 * PER) : "memory");
-            else if (ahead == 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * PER) : "memory");
-            else if (ahead == 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PER) : "memory");
-            else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        };
-        static_assert(NST <= 4, "wait");
+        // Steps past the last load zeros from outside the buffers: the waits are constants,
+        // and the loop has no branch but its end.
+        constexpr int HALF = (PER + 1) / 2;
 #pragma unroll
-        for (int p = 0; p < NST; ++p)
-            if (p < steps) issue(p, p * kStage, 0, PER);
-        wait(min(NST - 1, steps - 1));
+        for (int p = 0; p < NST; ++p) issue(p, p * kStage, 0, p < NST - 1 ? PER : HALF);
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NST - 2) * PER + HALF) : "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
         fetch(0, 0);
-        uint32_t st = 0, fst = 0;
-        int fill = steps;
-        for (int s = 0; s < steps; ++s) {
-            const uint32_t nst = st == (NST - 1) * kStage ? 0 : st + kStage;
+        int s = 0;
+        do {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                if (h == 0) {
-                    fetch(1, st);
-                } else {
-                    // this wave has read all of step s, and step s + 1 has landed ..
-                    if (s + 1 < steps) wait(min(NST - 2, steps - 2 - s));
-                    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-                    // .. and so it is for all waves
-                    __builtin_amdgcn_s_barrier();
-                    asm volatile("" ::: "memory");
-                    if (s + 1 < steps) fetch(0, nst);
-                    fill = s + NST;
-                    fst = st;
-                }
-                if (fill < steps) issue(fill, fst, h ? 0 : (PER + 1) / 2, h ? (PER + 1) / 2 : PER);
+            for (int p = 0; p < NST; ++p) {
+                fetch(1, p * kStage);
+                issue(s + NST - 1, (p + NST - 1) % NST * kStage, HALF, PER);
 #pragma unroll
                 for (int i = 0; i < FT; ++i)
 #pragma unroll
-                    for (int f = 0; f < FR; ++f) acc[i][f] = mfma16(xv[h][i], av[h][f], acc[i][f]);
+                    for (int f = 0; f < FR; ++f) acc[i][f] = mfma16(xv[0][i], av[0][f], acc[i][f]);
+                // step s + 1 has landed, and this wave has read all of step s ..
+                asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NST - 2) * PER) : "memory");
+                __builtin_amdgcn_s_waitcnt(0xC07F);   // lgkmcnt(0)
+                // .. and so it is for all waves
+                __builtin_amdgcn_s_barrier();
+                asm volatile("" ::: "memory");
+                fetch(0, (p + 1) % NST * kStage);
+                issue(s + NST, p * kStage, 0, HALF);
+#pragma unroll
+                for (int i = 0; i < FT; ++i)
+#pragma unroll
+                    for (int f = 0; f < FR; ++f) acc[i][f] = mfma16(xv[1][i], av[1][f], acc[i][f]);
+                if (++s == steps) break;
             }
-            st = nst;
-        }
+        } while (s < steps);
 #pragma unroll
         for (int i = 0; i < FT; ++i)
 #pragma unroll
@@ -396,6 +444,7 @@ __global__ __launch_bounds__(512) void lora_shrink_kernel(LoraArgs a, int groups
                 }
             }
     }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // no load into LDS outlives the block
 }
 
 // The splits' parts of t added in order, as an fp16 number, the fp16 rest and a factor
@@ -701,7 +750,7 @@ Plan plan_of(int64_t M, int64_t R, int64_t K) {
     p.groups = (int)srq_cdiv(R, 16 * p.rt);
     // blocks of at least 8 steps for four in five of the places on the 256 CUs (two of the
     // small ones fit one): the rest takes the second adapters of tiles that have two.
-    // 4875 tokens of four requests, rank 64 x 3, K = 8192: 89 us, with all places taken 97.
+    // 4876 tokens of four requests, rank 64 x 3, K = 8192: 87 us, with all places taken 97.
     const int64_t blocks = srq_cdiv(M, p.tokens) * p.groups, steps = srq_cdiv(K, 64);
     int64_t s = (p.rt == 4 ? 400 : 200) / blocks;
     if (s > steps / 8) s = steps / 8;
@@ -714,11 +763,13 @@ Plan plan_of(int64_t M, int64_t R, int64_t K) {
 }
 
 template <int RT>
-void launch_shrink(const LoraArgs &a, const Plan &p, unsigned blocks, int nz, hipStream_t st) {
+void launch_shrink(const LoraArgs &a, const Plan &p, unsigned blocks, int nz, int helpers,
+                   hipStream_t st) {
+    blocks = blocks * nz + helpers;
     if (p.tokens == 128)
-        lora_shrink_kernel<RT, 2, 3><<<blocks, 512, 0, st>>>(a, p.groups, nz);
+        lora_shrink_kernel<RT, 2, 3><<<blocks, 512, 0, st>>>(a, p.groups, nz, helpers);
     else
-        lora_shrink_kernel<RT, 1, RT == 8 ? 3 : 4><<<blocks, 512, 0, st>>>(a, p.groups, nz);
+        lora_shrink_kernel<RT, 1, RT == 8 ? 3 : 4><<<blocks, 512, 0, st>>>(a, p.groups, nz, helpers);
 }
 
 // t, and with many tokens its two halves and factors
@@ -841,13 +892,16 @@ extern "C" int srq_lora_add(const void *y, int64_t y_stride, const void *x, int6
         a.run_end[i] = (int)runs;
     }
     const int64_t b1 = srq_cdiv(M, p.tokens) * p.groups * p.splits, b2 = srq_cdiv(M, kTok) * runs;
-    const int z1 = shares(b1, 512), z2 = shares(b2, 1024);
+    // Where a block fills a CU, idle CUs are better given to a few second adapters.
+    const bool one = p.rt == 12 || (p.rt == 8 && p.tokens == 128);
+    const int z1 = shares(b1, one ? 256 : 512), z2 = shares(b2, 1024);
+    const int helpers = one && z1 == 1 && adapters > 1 && b1 < 256 ? (int)(256 - b1) : 0;
     // a launch has fewer than 2^32 threads in x
     SRQ_CHECK_ARG(b1 * z1 < 1 << 23 && b2 * z2 < 1 << 24, "lora_add: shape out of range");
     switch (p.rt) {
-    case 4: launch_shrink<4>(a, p, (unsigned)(b1 * z1), z1, st); break;
-    case 8: launch_shrink<8>(a, p, (unsigned)(b1 * z1), z1, st); break;
-    default: launch_shrink<12>(a, p, (unsigned)(b1 * z1), z1, st); break;
+    case 4: launch_shrink<4>(a, p, (unsigned)b1, z1, helpers, st); break;
+    case 8: launch_shrink<8>(a, p, (unsigned)b1, z1, helpers, st); break;
+    default: launch_shrink<12>(a, p, (unsigned)b1, z1, helpers, st); break;
     }
     SRQ_LAUNCH_CHECK("lora_add");
     lora_join_kernel<<<(unsigned)srq_cdiv(M * slices, 4), 256, 0, st>>>(a);

@@ -66,6 +66,24 @@ def test_matches(M, K, widths, r, L, kind):
     assert np.array_equal(got[none], y[none])
 
 
+@pytest.mark.parametrize("M,K,widths,r", [(1300, 8192, (300, 40), 96), (17000, 200, (9,), 136),
+                                          (20000, 72, (7, 2), 64), (29440, 72, (9,), 136),
+                                          (1100, 4160, (33,), 256)])
+@pytest.mark.parametrize("lo,hi", [(1, 30), (60, 400), (600, 2000)])
+def test_tiles_of_several_requests(M, K, widths, r, lo, hi):
+    """Sizes that leave CUs idle, whose blocks take a tile's second adapter: tiles of one
+    request, of two and of many, some tokens without an adapter."""
+    rng = np.random.default_rng(M + lo)
+    L = 6
+    y, x, la, lb, sc = _operands(rng, M, K, widths, r, L)
+    n = rng.integers(lo, hi, 2 * M // lo + 1)
+    ids = np.repeat(rng.integers(-1, L, n.size), n)[:M].astype(np.int32)
+    want, tol = ref.lora(y, x, la, lb, ids, sc, widths)
+    got = _run(y, x, la, lb, ids, sc, widths)
+    assert (np.abs(got - want) <= tol).all()
+    assert np.array_equal(got[ids < 0], y[ids < 0])
+
+
 @pytest.mark.parametrize("M,K", [(40, 512), (300, 512), (900, 2048), (1100, 512)])
 def test_integer_inputs_are_exact(M, K):
     """Whole numbers: t below 2^11 and every sum exact in fp32, so the result is the
