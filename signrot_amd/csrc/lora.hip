@@ -750,7 +750,8 @@ Plan plan_of(int64_t M, int64_t R, int64_t K) {
     p.groups = (int)srq_cdiv(R, 16 * p.rt);
     // blocks of at least 8 steps for four in five of the places on the 256 CUs (two of the
     // small ones fit one): the rest takes the second adapters of tiles that have two.
-    // 4876 tokens of four requests, rank 64 x 3, K = 8192: 87 us, with all places taken 97.
+    // 4876 tokens of four requests, rank 64 x 3, K = 8192: 89 us, with all places taken 97
+    // (87 since those blocks take only what is there).
     const int64_t blocks = srq_cdiv(M, p.tokens) * p.groups, steps = srq_cdiv(K, 64);
     int64_t s = (p.rt == 4 ? 400 : 200) / blocks;
     if (s > steps / 8) s = steps / 8;
