@@ -96,12 +96,12 @@ SRQ_DEV void lds_barrier() {
 }
 
 // ---------------------------------------------------------------------------
-// Up to 32 rows: the weights' bytes bound it.  A block of 8 waves takes 16 NT columns,
+// Few rows: the weights' bytes bound it.  A block of 8 waves takes 16 NT columns,
 // each wave an eighth of K in units of 128 codes, which it streams through its own ring
 // of S stages in LDS (AR activation rows of 128 bytes, then 16 NT weight rows of 64)
 // without a barrier; the waves' int32 sums are joined through LDS at the end.
-// 1 x 4096 x 4096 3.8 us, a launch and one round trip; 16 rows of 28672 codes on 8192
-// columns 28.5 us, 4.1 TB/s of weights (22 us where they are cached): what a CU takes in,
+// 1 x 4096 x 4096 3.6 us, a launch and one round trip; 16 rows of 28672 codes on 8192
+// columns 28.6 us, 4.1 TB/s of weights (20 us where they are cached): what a CU takes in,
 // with 16 rows as many bytes of rows as of weights.
 constexpr int W = 8;
 

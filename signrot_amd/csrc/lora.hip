@@ -298,7 +298,7 @@ SRQ_DEV uint32_t mixed_items(const LoraArgs &a, uint32_t at, uint32_t stride, ui
 // waves: 4 share the rows of A out, 2 the tokens.  The operands of half a step are read
 // beside the products of the half before, and the loads are spread over them: a wave
 // stalls on a burst of loads, and its products with it.  What a CU takes in bounds it,
-// about 50 bytes a ns: 4876 tokens x 192 rows of A, K = 8192, 31 us.
+// about 50 bytes a ns: 4876 tokens x 192 rows of A, K = 8192, 31 to 33 us.
 // Where CUs stay idle, `helpers` blocks more take second adapters: helper e that of the
 // first of the items e, e + helpers, .. whose tile has one, and the item's own block goes by
 // the same rule.  Four requests there, three tiles of two: 47 us when the second adapters
@@ -750,8 +750,7 @@ Plan plan_of(int64_t M, int64_t R, int64_t K) {
     p.groups = (int)srq_cdiv(R, 16 * p.rt);
     // blocks of at least 8 steps for four in five of the places on the 256 CUs (two of the
     // small ones fit one): the rest takes the second adapters of tiles that have two.
-    // 4876 tokens of four requests, rank 64 x 3, K = 8192: 89 us, with all places taken 97
-    // (87 since those blocks take only what is there).
+    // 4876 tokens of four requests, rank 64 x 3, K = 8192: 87 us, with all places taken 95.
     const int64_t blocks = srq_cdiv(M, p.tokens) * p.groups, steps = srq_cdiv(K, 64);
     int64_t s = (p.rt == 4 ? 400 : 200) / blocks;
     if (s > steps / 8) s = steps / 8;
