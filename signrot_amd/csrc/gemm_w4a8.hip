@@ -95,21 +95,29 @@ SRQ_DEV void lds_barrier() {
     asm volatile("" ::: "memory");
 }
 
+// An LDS row of C chunks of 16 bytes holds them exchanged by this number, so that 8
+// lanes that read one chunk of 8 rows meet all banks.
+template <int C>
+SRQ_DEV int swizzle(int row) { return C >= 16 ? row & 15 : C == 8 ? row >> 1 & 7 : row >> 2 & 3; }
+
 // ---------------------------------------------------------------------------
 // Few rows: the weights' bytes bound it.  A block of 8 waves takes 16 NT columns,
-// each wave an eighth of K in units of 128 codes, which it streams through its own ring
-// of S stages in LDS (AR activation rows of 128 bytes, then 16 NT weight rows of 64)
-// without a barrier; the waves' int32 sums are joined through LDS at the end.
+// each wave one in eight units of 128 U codes, which it streams through its own ring of S
+// stages in LDS (AR activation rows of 128 U bytes, then 16 NT weight rows of 64 U) without
+// a barrier; the waves' int32 sums are joined through LDS at the end.
 // 1 x 4096 x 4096 3.6 us, a launch and one round trip; 16 rows of 28672 codes on 8192
-// columns 28.6 us, 4.1 TB/s of weights (20 us where they are cached): what a CU takes in,
-// with 16 rows as many bytes of rows as of weights.
+// columns 24.5 us, 4.8 TB/s of weights: units in turn, so that a block's waves read
+// neighbouring lines, and whole cache lines of weights (U = 2).  An eighth of K in one piece
+// 27 us, in half lines 28.6.
 constexpr int W = 8;
 
-template <int AR, int NT, int S>
+template <int AR, int NT, int S, int U>
 __global__ __launch_bounds__(W * 64) void w4a8_stream_kernel(A8Args a) {
     constexpr int MT = AR == 32 ? 2 : 1;
-    constexpr int kStage = AR * 128 + NT * 1024;
-    constexpr int PER = AR / 8 + NT;
+    constexpr int CA = 8 * U, CB = 4 * U;       // chunks of a row
+    constexpr int RA = 64 / CA, RB = 64 / CB;   // rows of a load
+    constexpr int PA = AR / RA, PB = 16 * NT / RB, PER = PA + PB;
+    constexpr int kA = PA * 1024, kStage = PER * 1024;
     constexpr int kPart = W * 16 * MT * 16 * NT * 4;
     constexpr int kRing = W * S * kStage;
     __shared__ __attribute__((aligned(1024))) uint8_t smem[kRing > kPart ? kRing : kPart];
@@ -117,8 +125,7 @@ __global__ __launch_bounds__(W * 64) void w4a8_stream_kernel(A8Args a) {
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int64_t n0 = (int64_t)blockIdx.x * 16 * NT;
     const int64_t KB = a.K / 2;
-    const int units = (int)((a.K + 127) / 128), per = (units + W - 1) / W;
-    const int u0 = wave * per, cnt = max(0, min(per, units - u0));
+    const int units = (int)((a.K + 128 * U - 1) / (128 * U)), cnt = (units - wave + W - 1) / W;
     const __amdgpu_buffer_rsrc_t ar = make_rsrc(a.a, a.M * a.K);
     const __amdgpu_buffer_rsrc_t br = make_rsrc(a.w + n0 * KB, rows_bytes(a.N - n0, 16 * NT, KB));
     uint8_t *ring = smem + wave * S * kStage;
@@ -126,26 +133,28 @@ __global__ __launch_bounds__(W * 64) void w4a8_stream_kernel(A8Args a) {
 
     // rows past M stay as LDS has them and columns past N read zeros: neither is stored.
     // A chunk past K reads zeros on the weights' side, which cancels the other.
-    uint32_t aoff[AR / 8], boff[NT];
-    int bk;
+    uint32_t aoff[PA], boff[PB];
+    int bk[PB];
 #pragma unroll
-    for (int i = 0; i < AR / 8; ++i) {
-        const int r = 8 * i + (lane >> 3);
-        aoff[i] = r < a.M ? (uint32_t)(r * a.K) + 16 * ((lane & 7) ^ (r >> 1 & 7)) : kOob;
+    for (int i = 0; i < PA; ++i) {
+        const int r = RA * i + lane / CA;
+        aoff[i] = r < a.M ? (uint32_t)(r * a.K) + 16 * ((lane % CA) ^ swizzle<CA>(r)) : kOob;
     }
-    bk = 16 * ((lane & 3) ^ ((lane >> 4) & 3));
 #pragma unroll
-    for (int t = 0; t < NT; ++t) boff[t] = (uint32_t)((16 * t + (lane >> 2)) * KB) + bk;
+    for (int t = 0; t < PB; ++t) {
+        const int r = RB * t + lane / CB;
+        bk[t] = 16 * ((lane % CB) ^ swizzle<CB>(r));
+        boff[t] = (uint32_t)(r * KB) + bk[t];
+    }
     auto issue = [&](int u, int slot) __attribute__((always_inline)) {
         const uint32_t dst = ring0 + slot * kStage;
-        const uint32_t ka = (uint32_t)(u0 + u) * 128u, kb = ka / 2;
+        const uint32_t ka = (uint32_t)(u * W + wave) * (128u * U), kb = ka / 2;
 #pragma unroll
-        for (int i = 0; i < AR / 8; ++i)
+        for (int i = 0; i < PA; ++i)
             dma16(ar, u >= cnt || aoff[i] == kOob ? kOob : aoff[i] + ka, dst + i * 1024);
-        const bool in = u < cnt && kb + bk < KB;
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
-            dma16(br, in ? boff[t] + kb : kOob, dst + AR * 128 + t * 1024);
+        for (int t = 0; t < PB; ++t)
+            dma16(br, u < cnt && kb + bk[t] < KB ? boff[t] + kb : kOob, dst + kA + t * 1024);
     };
 
     v4i acc[MT][NT];
@@ -156,8 +165,7 @@ __global__ __launch_bounds__(W * 64) void w4a8_stream_kernel(A8Args a) {
     const int m = lane & 15, g = lane >> 4;
     const int mr = AR == 8 ? m & 7 : m;   // with 8 rows staged the upper 8 results are not stored
 #pragma unroll
-    for (int p = 0; p < S - 1; ++p)
-        issue(p, p);
+    for (int p = 0; p < S - 1; ++p) issue(p, p);
     int slot = 0, free = S - 1;
     for (int u = 0; u < cnt; ++u) {
         // the reads of the stage that is filled next have returned
@@ -165,22 +173,25 @@ __global__ __launch_bounds__(W * 64) void w4a8_stream_kernel(A8Args a) {
         issue(u + S - 1, free);
         wait_loads<(S - 1) * PER>();
         const uint8_t *st = ring + slot * kStage;
-        v4i av[MT][2];
 #pragma unroll
-        for (int i = 0; i < MT; ++i)
+        for (int z = 0; z < U; ++z) {
+            v4i av[MT][2];
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-                av[i][h] = *reinterpret_cast<const v4i *>(
-                    st + (16 * i + mr) * 128 + 16 * ((2 * g + h) ^ (mr >> 1)));
+            for (int i = 0; i < MT; ++i)
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            const v4i w = *reinterpret_cast<const v4i *>(
-                st + AR * 128 + t * 1024 + m * 64 + 16 * (g ^ ((m >> 2) & 3)));
-            const v4i b0 = codes16((u32)w[0], (u32)w[1]), b1 = codes16((u32)w[2], (u32)w[3]);
+                for (int h = 0; h < 2; ++h)
+                    av[i][h] = *reinterpret_cast<const v4i *>(
+                        st + ((16 * i + mr) * CA + ((8 * z + 2 * g + h) ^ swizzle<CA>(16 * i + mr))) * 16);
 #pragma unroll
-            for (int i = 0; i < MT; ++i) {
-                acc[i][t] = mfma16x64(av[i][0], b0, acc[i][t]);
-                acc[i][t] = mfma16x64(av[i][1], b1, acc[i][t]);
+            for (int t = 0; t < NT; ++t) {
+                const v4i w = *reinterpret_cast<const v4i *>(
+                    st + kA + ((16 * t + m) * CB + ((4 * z + g) ^ swizzle<CB>(16 * t + m))) * 16);
+                const v4i b0 = codes16((u32)w[0], (u32)w[1]), b1 = codes16((u32)w[2], (u32)w[3]);
+#pragma unroll
+                for (int i = 0; i < MT; ++i) {
+                    acc[i][t] = mfma16x64(av[i][0], b0, acc[i][t]);
+                    acc[i][t] = mfma16x64(av[i][1], b1, acc[i][t]);
+                }
             }
         }
         slot = slot == S - 1 ? 0 : slot + 1;
@@ -298,11 +309,6 @@ SRQ_DEV uint32_t place_of(uint32_t b, uint32_t total) {
     const uint32_t x = b % 8, per = total / 8, rem = total % 8;
     return x * per + min(x, rem) + b / 8;
 }
-
-// A step's LDS row of C chunks of 16 bytes holds them exchanged by this number, so that 8
-// lanes that read one chunk of 8 rows meet all banks.
-template <int C>
-SRQ_DEV int swizzle(int row) { return C >= 16 ? row & 15 : C == 8 ? row >> 1 & 7 : row >> 2 & 3; }
 
 // Up to a few rounds of tiles of BM x BN: K in steps of 64 KG codes through a ring of NSTG
 // stages (BM rows of 64 KG bytes, then BN of 32 KG) that every wave fills with its share of
@@ -768,20 +774,21 @@ void launch_tile(const A8Args &a, int splits, hipStream_t st) {
 template <int AR>
 void launch_stream(const A8Args &a, hipStream_t st) {
     // 16 columns a block up to a block a CU (256), then 32, which halves what the rows
-    // cost; more blocks than 256 run best two to a CU, which their LDS has to allow, and
-    // at 17 rows and more with 64 columns.  us, 28672 x 4096: 1 row 14 (32 columns, 4
-    // stages and so one block a CU: 17.7; 16 columns 13 to 14), 16 rows 16.2 (19.7);
-    // 10240 x 8192: 32 rows 16.4; 8192 x 28672: 16 rows 28.7 (16 columns: 35.4).
+    // cost, in units of 256 codes as long as that is a block a CU; more run best two to a
+    // CU, which their LDS has to allow, and at 17 rows and more with 64 columns.  us, 28672
+    // x 4096: 1 row 13.5 (units of 256, one block a CU: 17), 16 rows 16.0 (19); 10240 x
+    // 8192: 32 rows 16.4; 8192 x 28672: 16 rows 24.5 (16 columns: 33).
     const int64_t cb = srq_cdiv(a.N, 16);
     auto grid = [&](int nt) { return dim3((unsigned)srq_cdiv(cb, nt)); };
     if (cb <= 256)
-        w4a8_stream_kernel<AR, 1, AR == 32 ? 2 : 4><<<grid(1), W * 64, 0, st>>>(a);
-    else if (cb <= 512 || AR == 8)
-        w4a8_stream_kernel<AR, 2, 3><<<grid(2), W * 64, 0, st>>>(a);
-    else if constexpr (AR == 16)
-        w4a8_stream_kernel<AR, 2, 2><<<grid(2), W * 64, 0, st>>>(a);
+        w4a8_stream_kernel<AR, 1, AR == 32 ? 2 : 4, 1><<<grid(1), W * 64, 0, st>>>(a);
+    else if (AR < 32 && cb <= 512)
+        w4a8_stream_kernel<AR, 2, 2, AR < 32 ? 2 : 1><<<grid(2), W * 64, 0, st>>>(a);
     else if constexpr (AR == 32)
-        w4a8_stream_kernel<AR, 4, 2><<<grid(4), W * 64, 0, st>>>(a);
+        cb <= 512 ? w4a8_stream_kernel<AR, 2, 3, 1><<<grid(2), W * 64, 0, st>>>(a)
+                  : w4a8_stream_kernel<AR, 4, 2, 1><<<grid(4), W * 64, 0, st>>>(a);
+    else
+        w4a8_stream_kernel<AR, 2, AR == 8 ? 3 : 2, 1><<<grid(2), W * 64, 0, st>>>(a);
 }
 
 }  // namespace

@@ -36,7 +36,10 @@ SHAPES = [(1, 1, 32), (1, 16, 128), (2, 17, 96), (7, 33, 160), (8, 48, 4096), (9
           # each tile, in one part and split over K, with tails of all three sizes
           (100, 14340, 1056), (20, 16400, 2080), (24, 10250, 1056), (128, 28700, 352),
           (129, 14339, 2016), (200, 4111, 9312), (130, 2050, 20512), (512, 2100, 14368),
-          (384, 3000, 16416), (256, 2048, 16384), (40, 600, 8224), (33, 1, 32)]
+          (384, 3000, 16416), (256, 2048, 16384), (40, 600, 8224), (33, 1, 32),
+          # streams in units of 256 codes, of 128 beside them
+          (3, 4100, 32), (16, 8192, 1120), (11, 5000, 2464), (8, 6001, 96), (16, 4500, 5024),
+          (16, 8193, 1120), (30, 5000, 2464)]
 
 
 @pytest.mark.parametrize("M,N,K", SHAPES)
